@@ -111,30 +111,28 @@ __device__ __forceinline__ float gelu_erf_fast(float x) {
   return x * phi;
 }
 
-// N pairs in lockstep (v_pk_* math): the Horner chain of one pair is serial and a drain has one
-// wave per SIMD -- chain by chain the compiler pads every step with an s_nop
+// N pairs in lockstep: the Horner chain of one value is serial and a drain has one wave per SIMD --
+// chain by chain the compiler pads every step with an s_nop.  Single f32 instructions throughout
+// (the library is built without packed f32 instructions)
 template <int N>
 __device__ __forceinline__ void gelu_erf_fast2_n(f32x2 (&x)[N]) {
   constexpr float q[GELU_POLY_DEG + 1] = GELU_POLY_Q;
-  const f32x2 rc = {GELU_POLY_RC, GELU_POLY_RC};
-  const f32x2 half = {0.5f, 0.5f};
-  f32x2 u[N], y[N], t[N];
+  float u[2 * N], y[2 * N], t[2 * N];
 #pragma unroll
-  for (int c = 0; c < N; ++c) u[c] = x[c] * rc;
+  for (int c = 0; c < 2 * N; ++c) u[c] = x[c >> 1][c & 1] * GELU_POLY_RC;
 #pragma unroll
-  for (int c = 0; c < N; ++c) asm("v_pk_mul_f32 %0, %1, %1 clamp" : "=v"(y[c]) : "v"(u[c]));
+  for (int c = 0; c < 2 * N; ++c) asm("v_mul_f32_e64 %0, %1, %1 clamp" : "=v"(y[c]) : "v"(u[c]));
 #pragma unroll
-  for (int c = 0; c < N; ++c) t[c] = y[c] * (f32x2){q[GELU_POLY_DEG], q[GELU_POLY_DEG]} +
-                                     (f32x2){q[GELU_POLY_DEG - 1], q[GELU_POLY_DEG - 1]};
+  for (int c = 0; c < 2 * N; ++c) t[c] = fmaf(q[GELU_POLY_DEG], y[c], q[GELU_POLY_DEG - 1]);
 #pragma unroll
   for (int k = GELU_POLY_DEG - 2; k >= 0; --k)
 #pragma unroll
-    for (int c = 0; c < N; ++c) t[c] = t[c] * y[c] + (f32x2){q[k], q[k]};
+    for (int c = 0; c < 2 * N; ++c) t[c] = fmaf(t[c], y[c], q[k]);
 #pragma unroll
-  for (int c = 0; c < N; ++c)
-    asm("v_pk_fma_f32 %0, %1, %2, %3 clamp" : "=v"(t[c]) : "v"(u[c]), "v"(t[c]), "v"(half));
+  for (int c = 0; c < 2 * N; ++c)
+    asm("v_fma_f32 %0, %1, %2, 0.5 clamp" : "=v"(t[c]) : "v"(u[c]), "v"(t[c]));
 #pragma unroll
-  for (int c = 0; c < N; ++c) x[c] = x[c] * t[c];
+  for (int c = 0; c < 2 * N; ++c) x[c >> 1][c & 1] *= t[c];
 }
 
 template <bool EXACT>
