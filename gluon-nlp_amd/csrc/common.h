@@ -111,28 +111,33 @@ __device__ __forceinline__ float gelu_erf_fast(float x) {
   return x * phi;
 }
 
-// N pairs in lockstep: the Horner chain of one value is serial and a drain has one wave per SIMD --
-// chain by chain the compiler pads every step with an s_nop.  Single f32 instructions throughout
-// (the library is built without packed f32 instructions)
+// N pairs, two (four values) in lockstep: the Horner chain of one value is serial, and all 2 N side by
+// side take registers that a drain does not have.  Single f32 instructions throughout (the library
+// is built without packed f32 instructions)
 template <int N>
 __device__ __forceinline__ void gelu_erf_fast2_n(f32x2 (&x)[N]) {
+  static_assert(N % 2 == 0, "two pairs at a time");
   constexpr float q[GELU_POLY_DEG + 1] = GELU_POLY_Q;
-  float u[2 * N], y[2 * N], t[2 * N];
 #pragma unroll
-  for (int c = 0; c < 2 * N; ++c) u[c] = x[c >> 1][c & 1] * GELU_POLY_RC;
+  for (int h = 0; h < N; h += 2) {
+    float u[4], y[4], t[4];
 #pragma unroll
-  for (int c = 0; c < 2 * N; ++c) asm("v_mul_f32_e64 %0, %1, %1 clamp" : "=v"(y[c]) : "v"(u[c]));
+    for (int c = 0; c < 4; ++c) u[c] = x[h + (c >> 1)][c & 1] * GELU_POLY_RC;
 #pragma unroll
-  for (int c = 0; c < 2 * N; ++c) t[c] = fmaf(q[GELU_POLY_DEG], y[c], q[GELU_POLY_DEG - 1]);
+    for (int c = 0; c < 4; ++c) asm("v_mul_f32_e64 %0, %1, %1 clamp" : "=v"(y[c]) : "v"(u[c]));
 #pragma unroll
-  for (int k = GELU_POLY_DEG - 2; k >= 0; --k)
+    for (int c = 0; c < 4; ++c) t[c] = fmaf(q[GELU_POLY_DEG], y[c], q[GELU_POLY_DEG - 1]);
 #pragma unroll
-    for (int c = 0; c < 2 * N; ++c) t[c] = fmaf(t[c], y[c], q[k]);
+    for (int k = GELU_POLY_DEG - 2; k >= 0; --k)
 #pragma unroll
-  for (int c = 0; c < 2 * N; ++c)
-    asm("v_fma_f32 %0, %1, %2, 0.5 clamp" : "=v"(t[c]) : "v"(u[c]), "v"(t[c]));
+      for (int c = 0; c < 4; ++c) t[c] = fmaf(t[c], y[c], q[k]);
 #pragma unroll
-  for (int c = 0; c < 2 * N; ++c) x[c >> 1][c & 1] *= t[c];
+    for (int c = 0; c < 4; ++c)
+      asm("v_fma_f32 %0, %1, %2, 0.5 clamp" : "=v"(t[c]) : "v"(u[c]), "v"(t[c]));
+#pragma unroll
+    for (int c = 0; c < 4; ++c) x[h + (c >> 1)][c & 1] *= t[c];
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
 template <bool EXACT>

@@ -480,7 +480,7 @@ dense_bf16_w4_kernel(DenseW4Args a) {
 #pragma unroll
           for (int it = 0; it < 2; ++it) {
             float v[8];
-            // pairs throughout (v_pk_add_f32 / v_cvt_pk_bf16_f32): left to itself the compiler
+            // pairs throughout (v_cvt_pk_bf16_f32): left to itself the compiler
             // shuffles the identity epilogue through v_perm / v_alignbit (600 instead of 256
             // vector-ALU instructions per tile)
             f32x2 g[4];   // columns 0 1 | 2 3 | 4 5 | 6 7
@@ -653,8 +653,10 @@ dense_bf16_w4_kernel(DenseW4Args a) {
 #pragma unroll
           for (int pp = 0; pp < PPN; ++pp) {
             const int p = hn * 2 + pp;
+            // (the copies out of the accumulator registers stay here, 8 at a time: registers)
+            asm volatile("" : "+a"(acc[2 * p][s]), "+a"(acc[2 * p + 1][s]));
             const f32x4 a0 = acc[2 * p][s], a1 = acc[2 * p + 1][s];
-            // pairs throughout (v_pk_fma_f32 / v_cvt_pk_bf16_f32)
+            // pairs throughout (v_cvt_pk_bf16_f32)
             f32x2 gg[4] = {(f32x2){a0[0], a0[1]}, (f32x2){a0[2], a0[3]}, (f32x2){a1[0], a1[1]},
                            (f32x2){a1[2], a1[3]}};
 #pragma unroll
@@ -663,16 +665,11 @@ dense_bf16_w4_kernel(DenseW4Args a) {
                 gg[c] = gg[c] * r2 + (cv[pp][c] * nm2 + bv[pp][c]);
               else
                 gg[c] = gg[c] + bv[pp][c];
-            }
-            if (ACT == GNLP_ACT_GELU_ERF) {
-              gelu_erf_fast2_n<4>(gg);
-            } else {
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
+              if constexpr (ACT != GNLP_ACT_GELU_ERF)
                 gg[c] = (f32x2){apply_act<false>(gg[c][0], ACT), apply_act<false>(gg[c][1], ACT)};
-                if constexpr (ACT == GNLP_ACT_GELU_TANH) W4_SB();   // (registers)
-              }
+              if constexpr (ACT == GNLP_ACT_GELU_TANH) W4_SB();   // (registers)
             }
+            if (ACT == GNLP_ACT_GELU_ERF) gelu_erf_fast2_n<4>(gg);
             float v[8];
 #pragma unroll
             for (int c = 0; c < 4; ++c) { v[2 * c] = gg[c][0]; v[2 * c + 1] = gg[c][1]; }
