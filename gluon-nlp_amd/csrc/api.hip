@@ -1720,4 +1720,229 @@ int gnlp_profile_dense_read(float *ms, int capacity) {
   return n;
 }
 
+// ---- incremental decoding: 4-bit cache, beam search ----
+namespace {
+int check_cache(const gnlp_kv4_cache *c) {
+  REQUIRE(c != nullptr, "cache is NULL");
+  REQUIRE(c->B >= 0 && c->H >= 0 && c->slots >= 0, "negative shape");
+  REQUIRE(c->d >= 1 && c->d <= 128, "4-bit cache: head dim %lld outside [1, 128]", (long long)c->d);
+  REQUIRE(c->slots % 32 == 0 && c->slots < (1LL << 30),
+          "4-bit cache: slots=%lld must be a multiple of 32 below 2^30", (long long)c->slots);
+  REQUIRE(c->B <= 65535 && c->H <= 65535, "4-bit cache: more than 65535 sequences or heads");
+  if (c->B * c->H * c->slots == 0) return GNLP_OK;
+  REQUIRE(c->k_codes && c->v_codes && c->k_par && c->v_par, "4-bit cache: NULL array");
+  REQUIRE((((uintptr_t)c->k_codes | (uintptr_t)c->v_codes | (uintptr_t)c->k_par |
+            (uintptr_t)c->v_par) & 15) == 0, "4-bit cache: arrays must be 16-byte aligned");
+  return GNLP_OK;
+}
+
+int kv4_io(const gnlp_kv4_cache *c, void *k, void *v, int dtype, int64_t L, const int64_t *ks,
+           const int64_t *vs, const void *length, int length_dtype, const void *count,
+           int count_dtype, int write, hipStream_t s) {
+  REQUIRE(dtype_ok(dtype), "unsupported dtype %d", dtype);
+  if (int rc = check_cache(c)) return rc;
+  REQUIRE(L >= 0 && L < (1LL << 30), "4-bit cache: L=%lld out of range", (long long)L);
+  REQUIRE((!length || vl_ok(length_dtype)) && (!count || vl_ok(count_dtype)),
+          "lengths must be int32 or int64");
+  if (c->B * c->H * L == 0 || (write && c->slots == 0)) return GNLP_OK;
+  REQUIRE(k && v && ks && vs, "NULL tensor");
+  REQUIRE(c->slots > 0, "reading a cache without slots");
+  Kv4Io a = {};
+  a.k_codes = c->k_codes; a.v_codes = c->v_codes; a.k_par = c->k_par; a.v_par = c->v_par;
+  a.B = c->B; a.H = c->H; a.S = c->slots; a.d = c->d; a.L = L;
+  a.g_shift = c->d > 64 ? 1 : 0;
+  a.DP = 64 << a.g_shift;
+  a.nblk = (uint32_t)((L + 6) / 8 + 1);
+  REQUIRE((((int64_t)a.nblk * a.H) << a.g_shift) < (1LL << 31),
+          "4-bit cache: L * heads too large for one call");
+  a.k = k; a.v = v;
+  for (int i = 0; i < 3; ++i) { a.k_stride[i] = ks[i]; a.v_stride[i] = vs[i]; }
+  a.length = length; a.length_dtype = length_dtype;
+  a.count = count; a.count_dtype = count_dtype;
+  a.write = write;
+  launch_kv4_io(a, dtype, s);
+  return check_launch(write ? "gnlp_kv4_write" : "gnlp_kv4_read");
+}
+
+int kv4_splits(const gnlp_kv4_cache *c, const gnlp_kv4_attn_desc *d) {
+  int64_t keys = d->keys > 0 && d->keys < c->slots ? d->keys : c->slots;
+  if ((d->edge_scores || d->mask) && d->Lm < keys) keys = d->Lm;
+  return kv4_attn_plan(c->B, c->H, d->Lq * d->share, keys, c->d);
+}
+bool kv4_desc_sane(const gnlp_kv4_cache *c, const gnlp_kv4_attn_desc *d) {
+  return c && d && d->Lq >= 0 && d->share >= 1 && c->B >= 0 && c->H >= 0 && c->slots >= 0 &&
+         d->Lq <= (1LL << 24) && d->share <= (1LL << 24) && c->B <= 65535 && c->H <= 65535 &&
+         c->B * c->H * d->Lq * d->share > 0;
+}
+}  // namespace
+
+int gnlp_kv4_write(const gnlp_kv4_cache *cache, const void *key, const void *value, int dtype,
+                   int64_t L, const int64_t key_stride[3], const int64_t value_stride[3],
+                   const void *length, int length_dtype, const void *new_length,
+                   int new_length_dtype, gnlp_stream_t stream) {
+  return kv4_io(cache, const_cast<void *>(key), const_cast<void *>(value), dtype, L, key_stride,
+                value_stride, length, length_dtype, new_length, new_length_dtype, 1, S(stream));
+}
+
+int gnlp_kv4_read(const gnlp_kv4_cache *cache, void *key, void *value, int dtype, int64_t L,
+                  const int64_t key_stride[3], const int64_t value_stride[3], const void *length,
+                  int length_dtype, const void *start, int start_dtype, gnlp_stream_t stream) {
+  return kv4_io(cache, key, value, dtype, L, key_stride, value_stride, length, length_dtype, start,
+                start_dtype, 0, S(stream));
+}
+
+size_t gnlp_kv4_attn_workspace_bytes(const gnlp_kv4_cache *cache, const gnlp_kv4_attn_desc *d) {
+  if (!kv4_desc_sane(cache, d)) return 0;
+  const size_t n = (size_t)kv4_splits(cache, d);
+  const size_t rows = (size_t)(cache->B * cache->H * d->Lq * d->share);
+  return n <= 1 ? 0 : align256(rows * n * (cache->d > 64 ? 130 : 66) * sizeof(float));
+}
+
+int gnlp_kv4_attn(void *ctx, const void *q, const gnlp_kv4_cache *cache,
+                  const gnlp_kv4_attn_desc *d, int dtype, void *workspace, size_t workspace_bytes,
+                  gnlp_stream_t stream) {
+  REQUIRE(dtype_ok(dtype), "unsupported dtype %d", dtype);
+  if (int rc = check_cache(cache)) return rc;
+  REQUIRE(d != nullptr, "descriptor is NULL");
+  REQUIRE(d->Lq >= 0 && d->share >= 1, "Lq must not be negative, share must be positive");
+  REQUIRE(d->Lq <= (1LL << 24) && d->share <= (1LL << 24) && d->Lq * d->share <= (1LL << 30),
+          "4-bit attention: too many query rows");
+  REQUIRE(!(d->edge_scores && d->edge_table), "edge_scores and edge_table exclude each other");
+  REQUIRE(!d->edge_table || d->table_len > 0, "edge_table without entries");
+  REQUIRE(!(d->edge_scores || d->mask) || d->Lm >= 0, "negative Lm");
+  REQUIRE(vl_ok((int)d->length_dtype) && (!d->q_length || vl_ok((int)d->q_length_dtype)),
+          "lengths must be int32 or int64");
+  if (cache->B * cache->H * d->Lq == 0) return GNLP_OK;
+  REQUIRE(ctx && q && d->length, "NULL tensor");
+  REQUIRE(cache->slots > 0, "attention over a cache without slots");
+  Kv4Attn a = {};
+  a.k_codes = cache->k_codes; a.v_codes = cache->v_codes;
+  a.k_par = cache->k_par; a.v_par = cache->v_par;
+  a.B = cache->B; a.H = cache->H; a.S = cache->slots; a.d = cache->d;
+  a.Lq = d->Lq; a.share = (int)d->share;
+  a.q = q; a.out = ctx;
+  for (int i = 0; i < 3; ++i) {
+    a.q_stride[i] = d->q_stride[i];
+    a.o_stride[i] = d->o_stride[i];
+    a.mask_stride[i] = d->mask_stride[i];
+  }
+  for (int i = 0; i < 4; ++i) a.edge_stride[i] = d->edge_stride[i];
+  a.length = d->length; a.length_dtype = (int)d->length_dtype;
+  a.q_length = d->q_length; a.q_length_dtype = (int)d->q_length_dtype;
+  a.causal = d->causal != 0;
+  a.edge = d->edge_scores; a.table = d->edge_table; a.table_len = d->table_len;
+  a.mask = d->mask;
+  a.Lm = d->edge_scores || d->mask ? d->Lm : cache->slots;
+  a.inv_temperature = d->temperature > 0 ? (float)(1.0 / d->temperature) : 1.0f;
+  const int64_t rows = d->Lq * d->share;
+  a.row_tiles = (int)((rows + 15) / 16);
+  a.splits = kv4_splits(cache, d);
+  REQUIRE(cache->B * cache->H * a.row_tiles * a.splits < (1LL << 31),
+          "4-bit attention: too many workgroups");
+  if (a.splits > 1) {
+    const size_t need = gnlp_kv4_attn_workspace_bytes(cache, d);
+    REQUIRE(workspace && workspace_bytes >= need, "workspace too small: %zu < %zu",
+            workspace_bytes, need);
+    REQUIRE(((uintptr_t)workspace & 15) == 0, "workspace must be 16-byte aligned");
+    a.part_o = (float *)workspace;
+    a.part_ml = a.part_o + cache->B * cache->H * rows * a.splits * (cache->d > 64 ? 128 : 64);
+  }
+  launch_kv4_attn(a, dtype, S(stream));
+  return check_launch("gnlp_kv4_attn");
+}
+
+size_t gnlp_beam_select_workspace_bytes(const gnlp_beam_desc *d) {
+  if (!d || d->N <= 0 || d->K <= 0 || d->K > BEAM_MAX || d->V <= 0 || d->N > 65535 ||
+      d->V >= (1LL << 31))
+    return 0;
+  return align256(beam_workspace_bytes(d->N * d->K, d->V, (int)d->K));
+}
+
+int gnlp_beam_select(float *out_scores, int32_t *out_parents, int32_t *out_tokens,
+                     uint8_t *out_finished, const void *outputs, int dtype, const float *scores,
+                     const uint8_t *finished, const gnlp_beam_desc *d, void *workspace,
+                     size_t workspace_bytes, gnlp_stream_t stream) {
+  REQUIRE(dtype_ok(dtype), "unsupported dtype %d", dtype);
+  REQUIRE(d != nullptr, "descriptor is NULL");
+  REQUIRE(d->N >= 0, "negative number of items");
+  REQUIRE(d->K >= 1 && d->K <= BEAM_MAX, "beam size %lld outside [1, %d]", (long long)d->K, BEAM_MAX);
+  REQUIRE(d->V >= 1 && d->V < (1LL << 31) - 4096, "vocabulary size %lld out of range",
+          (long long)d->V);
+  REQUIRE(d->row_stride >= d->V, "row stride %lld < V", (long long)d->row_stride);
+  REQUIRE(d->N * d->K <= 65535, "more than 65535 beams in one call");
+  REQUIRE(d->temperature > 0 && isfinite(d->temperature), "temperature must be positive");
+  REQUIRE(isfinite(d->alpha) && isfinite(d->length_base) && d->length_base > -1,
+          "alpha / length_base out of range");
+  REQUIRE(d->step_dev ? vl_ok((int)d->step_dtype) : d->length_base + d->step > 1.0,
+          "step: a device int32 / int64, or length_base + step > 1");
+  if (d->N == 0) return GNLP_OK;
+  REQUIRE(out_scores && out_parents && out_tokens && out_finished && outputs && scores,
+          "NULL tensor");
+  const size_t need = gnlp_beam_select_workspace_bytes(d);
+  REQUIRE(workspace && workspace_bytes >= need, "workspace too small: %zu < %zu", workspace_bytes,
+          need);
+  REQUIRE(((uintptr_t)workspace & 15) == 0, "workspace must be 16-byte aligned");
+  BeamSelect a = {};
+  a.outputs = outputs; a.row_stride = d->row_stride; a.V = d->V; a.K = (int)d->K;
+  a.scores = scores; a.finished = finished;
+  a.normalize = d->normalize != 0;
+  a.inv_temperature = 1.0 / d->temperature;
+  a.exp_scale = (float)(1.4426950408889634 * a.inv_temperature);
+  a.alpha = d->alpha; a.length_base = d->length_base;
+  a.step = d->step_dev; a.step_dtype = (int)d->step_dtype;
+  if (!d->step_dev) {
+    a.lp_prev = pow((d->length_base + d->step - 1.0) / (d->length_base + 1.0), d->alpha);
+    a.lp_new = pow((d->length_base + d->step) / (d->length_base + 1.0), d->alpha);
+  }
+  a.has_eos = d->eos >= 0; a.eos = d->eos;
+  a.out_scores = out_scores; a.out_parents = out_parents; a.out_tokens = out_tokens;
+  a.out_finished = out_finished;
+  launch_beam_select(a, d->N, dtype, workspace, S(stream));
+  return check_launch("gnlp_beam_select");
+}
+
+int gnlp_reorder_states(const gnlp_state *states, int count, int64_t N, int64_t K,
+                        const void *parents, int parents_dtype, const void *length,
+                        int length_dtype, gnlp_stream_t stream) {
+  REQUIRE(count >= 0 && N >= 0 && K >= 1, "negative shape");
+  REQUIRE(N <= (1LL << 30) && K <= (1LL << 30) && N * K <= (1LL << 30), "too many rows");
+  REQUIRE(vl_ok(parents_dtype) && (!length || vl_ok(length_dtype)),
+          "parents / length must be int32 or int64");
+  if (count == 0 || N == 0) return GNLP_OK;
+  REQUIRE(states && parents, "NULL argument");
+  int seen = 0;
+  bool in_place = false;
+  for (int i = 0; i < count; ++i) {
+    const gnlp_state &t = states[i];
+    REQUIRE(t.outer >= 0 && t.nseg >= 0 && t.seg_bytes >= 0, "state %d: negative extent", i);
+    if (t.outer * t.nseg * t.seg_bytes == 0) continue;
+    REQUIRE(t.src && t.dst, "state %d: NULL tensor", i);
+    if (seen++ == 0) in_place = t.src == t.dst;
+    REQUIRE((t.src == t.dst) == in_place, "state %d: all in place or none", i);
+    REQUIRE(t.slots_per_unit == 0 || (t.slots_per_unit > 0 && t.unit_bytes > 0),
+            "state %d: bad units", i);
+  }
+  REQUIRE(!in_place || K <= BEAM_MAX, "in place: beam size %lld outside [1, %d]", (long long)K,
+          BEAM_MAX);
+  for (int first = 0; first < count; first += REORDER_MAX) {
+    Reorder a = {};
+    a.N = N; a.K = (int)K;
+    a.parents = parents; a.parents_dtype = parents_dtype;
+    a.length = length; a.length_dtype = length_dtype;
+    for (int i = first; i < count && i < first + REORDER_MAX; ++i) {
+      const gnlp_state &t = states[i];
+      if (t.outer * t.nseg * t.seg_bytes == 0) continue;
+      ReorderEntry &e = a.e[a.n++];
+      e.src = t.src; e.dst = t.dst;
+      e.outer = t.outer; e.outer_stride = t.outer_stride; e.row_stride = t.row_stride;
+      e.nseg = t.nseg; e.seg_stride = t.seg_stride; e.seg_bytes = t.seg_bytes;
+      e.slots_per_unit = t.slots_per_unit; e.unit_bytes = t.unit_bytes;
+    }
+    if (a.n == 0) continue;
+    REQUIRE(launch_reorder(a, in_place, S(stream)), "states too large for one call");
+    if (int rc = check_launch("gnlp_reorder_states")) return rc;
+  }
+  return GNLP_OK;
+}
+
 }  // extern "C"

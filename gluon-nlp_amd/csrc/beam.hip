@@ -1,0 +1,501 @@
+// One step of a beam search on the device: the choice of the K best continuations of each item's K
+// beams over the vocabulary, and the reordering of the decoding states that follows it, gfx950.
+//
+// Selection.  With z = outputs / temperature (sanitised: NaN counts as -inf, +inf as the largest
+// finite number) a candidate of an unfinished beam k and token v scores
+//   (prev[k] * lp_prev + z[k, v] - logsumexp(z[k])) / lp_new
+// (logsumexp 0 when the outputs are log-probabilities already), a finished beam has one candidate,
+// itself with its old score.  The K best of an item are returned in order, ties to the lowest index
+// k V + v (finished beams: K V + k).  A beam whose previous score is not above -1e15 is dead: all
+// its candidates count as -inf.
+//
+// Candidates of one beam are ordered by their logits alone, so the K best of every 4096 logits are
+// found first (beam_chunk_kernel, one pass over the logits, which also leaves the maximum and the
+// sum of exponentials), and the few that are left are scored in 64 bits (beam_merge_kernel: beams
+// that come near each other are told apart by the logsumexp's last digits).
+//   The K best of a chunk: a wave's 64 lane maxima are bisected, by ballots over the 16 high bits of
+//   an order-preserving integer, for a bound that K lanes reach; the best bound of the four waves
+//   leaves little more than K values, which a list in LDS ranks by counting.  Where ties overfill
+//   the list (a constant row), K rounds of a block-wide maximum do it.
+// Bound by memory: the logits once.
+//
+// Reordering.  out[row] = in[parent's row] for a list of tensors of any size, in one launch.  In
+// place, a thread holds its 16 bytes of all K beams before it writes any, and rows that keep their
+// place are not written.  Bound by memory: the chosen rows once, the changed rows once.
+#include "common.h"
+#include "kernels.h"
+
+namespace gnlp {
+namespace {
+
+constexpr int CH_E = 16;                        // values of a thread
+constexpr int CH = 256 * CH_E;                  // values of a workgroup
+constexpr int CAP = 512;                        // list of survivors
+constexpr float NEG = -__builtin_inff();
+
+// larger float <-> larger unsigned
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t ordered(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  return (u >> 63) ? ~u : u | 0x8000000000000000ull;
+}
+// -0 and +0 are one score
+__device__ __forceinline__ float plain_zero(float x) { return x + 0.0f; }
+
+__device__ __forceinline__ float sane(float x) {   // fmaxf(NaN, y) = y
+  return fminf(fmaxf(x, NEG), 3.4028234663852886e38f);
+}
+
+// a bound, of 16 high bits of the keys, that at least K of the wave's 64 keys reach (0 if fewer
+// than K are above 0)
+__device__ __forceinline__ uint32_t wave_bound(uint32_t key, int K) {
+  uint32_t bound = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 16; --bit) {
+    const uint32_t next = bound | (1u << bit);
+    if ((int)__popcll(__ballot(key >= next)) >= K) bound = next;
+  }
+  return bound;
+}
+
+__device__ __forceinline__ bool better(float x, uint32_t i, float y, uint32_t j) {
+  return x > y || (x == y && i < j);
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) beam_chunk_kernel(BeamSelect a) {
+  __shared__ float lx[CAP];
+  __shared__ uint32_t li[CAP];
+  __shared__ uint32_t sh_n, sh_bound[4];
+  __shared__ float sh_m[4], sh_s[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row = blockIdx.y;
+  const uint32_t chunk = blockIdx.x, base = chunk * CH, V = (uint32_t)a.V;
+  if (a.finished && a.finished[row]) return;
+  const bool dead = !(a.scores[row] > -1e15f);
+  const T *src = (const T *)a.outputs + row * a.row_stride;
+  if (tid == 0) sh_n = 0;
+
+  // value e of a thread is element base + at(e)
+  constexpr int PER = VEC ? 16 / (int)sizeof(T) : 1;
+  auto at = [&](int e) -> uint32_t { return base + (e / PER) * (256 * PER) + tid * PER + e % PER; };
+  float x[CH_E];
+#pragma unroll
+  for (int v = 0; v < CH_E / PER; ++v) {
+    const uint32_t i = at(v * PER);
+    if (VEC) {
+      if (i < V) {
+        const typename VecOf<T>::type w = *reinterpret_cast<const typename VecOf<T>::type *>(src + i);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) x[v * PER + e] = to_f32((T)w[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) x[v * PER + e] = NEG;
+      }
+    } else {
+      x[v] = i < V ? to_f32(src[i]) : NEG;
+    }
+  }
+  float most = NEG;
+  uint32_t any = 0;                                      // whether the lane holds an element at all
+#pragma unroll
+  for (int e = 0; e < CH_E; ++e) {
+    x[e] = dead ? NEG : plain_zero(sane(x[e]));
+    most = fmaxf(most, x[e]);
+    any |= at(e) < V;
+  }
+  const uint32_t bound = wave_bound(any ? ordered(most) : 0u, a.K);
+  const float wm = wave_max(most);
+  float s = 0.f;
+  if (wm > NEG) {
+#pragma unroll
+    for (int e = 0; e < CH_E; ++e) s += __builtin_amdgcn_exp2f((x[e] - wm) * a.exp_scale);
+  }
+  s = wave_sum(s);
+  if (lane == 0) {
+    sh_bound[wave] = bound;
+    sh_m[wave] = wm;
+    sh_s[wave] = s;
+  }
+  __syncthreads();
+  const int64_t slot = row * a.chunks + chunk;
+  if (tid == 0) {
+    const float m = fmaxf(fmaxf(sh_m[0], sh_m[1]), fmaxf(sh_m[2], sh_m[3]));
+    double t = 0;
+    for (int w = 0; w < 4; ++w)
+      if (sh_m[w] > NEG) t += (double)sh_s[w] * exp2((double)(sh_m[w] - m) * (double)a.exp_scale);
+    a.stats[slot * 2] = m;
+    a.stats[slot * 2 + 1] = (float)t;
+  }
+  const uint32_t least = max(max(sh_bound[0], sh_bound[1]), max(sh_bound[2], sh_bound[3]));
+#pragma unroll
+  for (int e = 0; e < CH_E; ++e) {
+    const bool in = at(e) < V && ordered(x[e]) >= least;
+    const uint64_t on = __ballot(in);
+    if (on) {
+      uint32_t start = 0;
+      if (lane == 0) start = atomicAdd(&sh_n, (uint32_t)__popcll(on));
+      start = __builtin_amdgcn_readfirstlane(start);
+      const uint32_t pos = start + __builtin_amdgcn_mbcnt_hi((uint32_t)(on >> 32),
+                                                             __builtin_amdgcn_mbcnt_lo((uint32_t)on, 0));
+      if (in && pos < CAP) {
+        lx[pos] = x[e];
+        li[pos] = at(e);
+      }
+    }
+  }
+  __syncthreads();
+  const uint32_t n = sh_n;
+  float *ox = a.cand_x + slot * a.K;
+  int32_t *oi = a.cand_i + slot * a.K;
+  if (n <= CAP) {
+    for (uint32_t c = tid; c < n; c += 256) {
+      const float mx = lx[c];
+      const uint32_t mi = li[c];
+      int rank = 0;
+      for (uint32_t o = 0; o < n; ++o) rank += better(lx[o], li[o], mx, mi);
+      if (rank < a.K) {
+        ox[rank] = mx;
+        oi[rank] = (int32_t)mi;
+      }
+    }
+    for (int r = (int)n + tid; r < a.K; r += 256) oi[r] = -1;
+    return;
+  }
+  // ties overfill the list: K times the best of what is left, over the whole workgroup
+  float tx = __builtin_inff();
+  uint32_t ti = 0;
+  for (int r = 0; r < a.K; ++r) {
+    float bx = NEG;
+    uint32_t bi = 0xffffffffu;
+#pragma unroll
+    for (int e = 0; e < CH_E; ++e) {
+      const uint32_t i = at(e);
+      const bool left = i < V && (r == 0 || better(tx, ti, x[e], i));
+      if (left && better(x[e], i, bx, bi)) { bx = x[e]; bi = i; }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const float yx = __shfl_xor(bx, o, 64);
+      const uint32_t yi = __shfl_xor(bi, o, 64);
+      if (better(yx, yi, bx, bi)) { bx = yx; bi = yi; }
+    }
+    __syncthreads();
+    if (lane == 0) { lx[wave] = bx; li[wave] = bi; }
+    __syncthreads();
+    tx = lx[0];
+    ti = li[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w)
+      if (better(lx[w], li[w], tx, ti)) { tx = lx[w]; ti = li[w]; }
+    if (tid == 0) { ox[r] = tx; oi[r] = (int32_t)ti; }   // 0xffffffff: none left
+    if (ti == 0xffffffffu) {
+      for (int q = r + 1 + tid; q < a.K; q += 256) oi[q] = -1;
+      return;
+    }
+  }
+}
+
+__device__ __forceinline__ bool better(double x, int64_t i, double y, int64_t j) {
+  return x > y || (x == y && i < j);
+}
+
+__global__ void __launch_bounds__(256) beam_merge_kernel(BeamSelect a) {
+  constexpr int LIST = 1024;
+  __shared__ double lse[BEAM_MAX], sx[LIST];     // lse: the maximum of z taken off
+  __shared__ float peak[BEAM_MAX];
+  __shared__ int64_t si[LIST];
+  __shared__ uint32_t sh_n, sh_bound[4];
+  __shared__ double bx4[4];
+  __shared__ int64_t bi4[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t item = blockIdx.x;
+  const int K = a.K;
+  if (tid == 0) sh_n = 0;
+  // ---- logsumexp of each beam from its chunks ----
+  for (int k = wave; k < K; k += 4) {
+    const int64_t row = item * K + k;
+    double out = 0;
+    float m = 0.f;
+    if (a.normalize && !(a.finished && a.finished[row])) {
+      const float *st = a.stats + row * a.chunks * 2;
+      m = NEG;
+      for (uint32_t c = lane; c < a.chunks; c += 64) m = fmaxf(m, st[2 * c]);
+      m = wave_max(m);
+      double t = 0;
+      for (uint32_t c = lane; c < a.chunks; c += 64)
+        if (st[2 * c] > NEG)
+          t += (double)st[2 * c + 1] * exp(((double)st[2 * c] - (double)m) * a.inv_temperature);
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+      if (m > NEG) out = log(t);
+      else m = 0.f;
+    }
+    if (lane == 0) {
+      lse[k] = out;
+      peak[k] = m;
+    }
+  }
+  __syncthreads();
+  double lp_prev = a.lp_prev, lp_new = a.lp_new;
+  if (a.step) {
+    const double s = (double)load_len(a.step, a.step_dtype, 0);
+    lp_prev = pow((a.length_base + s - 1.0) / (a.length_base + 1.0), a.alpha);
+    lp_new = pow((a.length_base + s) / (a.length_base + 1.0), a.alpha);
+  }
+  const int64_t per = (int64_t)a.chunks * K, n = K * per + K;
+  const int64_t none = 0x7fffffffffffffffLL;
+  // candidate c -> score and index (index `none`: there is no such candidate)
+  auto get = [&](int64_t c, double &x, int64_t &i) {
+    x = -__builtin_inf();
+    i = none;
+    const int k = (int)(c < K * per ? (uint32_t)c / (uint32_t)per : c - K * per);
+    const int64_t row = item * K + k;
+    const bool fin = a.finished && a.finished[row];
+    const float prev = a.scores[row];
+    const bool dead = !(prev > -1e15f);
+    if (c >= K * per) {
+      if (fin) {
+        i = (int64_t)K * a.V + k;
+        if (!dead) x = (double)prev;
+      }
+    } else if (!fin) {
+      const int32_t v = a.cand_i[row * per + (c - k * per)];
+      if (v >= 0) {
+        i = (int64_t)k * a.V + v;
+        const float z = a.cand_x[row * per + (c - k * per)];
+        if (z > NEG && !dead)
+          x = ((double)prev * lp_prev +
+               (((double)z - (double)peak[k]) * a.inv_temperature - lse[k])) / lp_new;
+      }
+    }
+  };
+  double mx = -__builtin_inf();
+  int64_t mi = none;
+  for (int64_t c = tid; c < n; c += 256) {
+    double x;
+    int64_t i;
+    get(c, x, i);
+    if (better(x, i, mx, mi)) { mx = x; mi = i; }
+  }
+  const uint32_t bound = wave_bound(mi != none ? (uint32_t)(ordered(mx) >> 32) : 0u, K);
+  if (lane == 0) sh_bound[wave] = bound;
+  __syncthreads();
+  const uint32_t least = max(max(sh_bound[0], sh_bound[1]), max(sh_bound[2], sh_bound[3]));
+  for (int64_t c = tid; c < n; c += 256) {
+    double x;
+    int64_t i;
+    get(c, x, i);
+    if (i != none && (uint32_t)(ordered(x) >> 32) >= least) {
+      const uint32_t pos = atomicAdd(&sh_n, 1u);
+      if (pos < LIST) { sx[pos] = x; si[pos] = i; }
+    }
+  }
+  __syncthreads();
+  const uint32_t found = sh_n;
+  auto put = [&](int rank, double x, int64_t i) {
+    const int64_t to = item * K + rank, KV = (int64_t)K * a.V;
+    const bool was = i >= KV;
+    const int64_t k = was ? i - KV : i / a.V, v = was ? -1 : i - k * a.V;
+    a.out_scores[to] = (float)x;
+    a.out_parents[to] = (int32_t)k;
+    a.out_tokens[to] = (int32_t)v;
+    a.out_finished[to] = was || (a.has_eos && v == a.eos);
+  };
+  if (found <= LIST) {
+    for (uint32_t c = tid; c < found; c += 256) {
+      const double x = sx[c];
+      const int64_t i = si[c];
+      int rank = 0;
+      for (uint32_t o = 0; o < found; ++o) rank += better(sx[o], si[o], x, i);
+      if (rank < K) put(rank, x, i);
+    }
+    return;
+  }
+  double tx = __builtin_inf();
+  int64_t ti = -1;
+  for (int r = 0; r < K; ++r) {
+    double bx = -__builtin_inf();
+    int64_t bi = none;
+    for (int64_t c = tid; c < n; c += 256) {
+      double x;
+      int64_t i;
+      get(c, x, i);
+      if (i != none && (r == 0 || better(tx, ti, x, i)) && better(x, i, bx, bi)) { bx = x; bi = i; }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const double yx = __shfl_xor(bx, o, 64);
+      const int64_t yi = __shfl_xor((long long)bi, o, 64);
+      if (better(yx, yi, bx, bi)) { bx = yx; bi = yi; }
+    }
+    __syncthreads();
+    if (lane == 0) { bx4[wave] = bx; bi4[wave] = bi; }
+    __syncthreads();
+    tx = bx4[0];
+    ti = bi4[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w)
+      if (better(bx4[w], bi4[w], tx, ti)) { tx = bx4[w]; ti = bi4[w]; }
+    if (tid == 0) put(r, tx, ti);
+  }
+}
+
+// ---- reordering ----
+constexpr int REORDER_UNROLL = 4;
+
+template <int VB> struct Piece;
+template <> struct Piece<16> { typedef f32x4 type; };
+template <> struct Piece<4> { typedef float type; };
+template <> struct Piece<1> { typedef uint8_t type; };
+
+// bytes of a segment that the row's length covers
+__device__ __forceinline__ int64_t live_bytes(const Reorder &a, const ReorderEntry &e, int64_t src) {
+  if (!a.length || e.slots_per_unit == 0) return e.seg_bytes;
+  int64_t n = load_len(a.length, a.length_dtype, src);
+  n = n < 0 ? 0 : n;
+  const int64_t used = (n + e.slots_per_unit - 1) / e.slots_per_unit * e.unit_bytes;
+  return used < e.seg_bytes ? used : e.seg_bytes;
+}
+__device__ __forceinline__ int parent_of(const Reorder &a, int64_t row) {
+  const int64_t p = load_len(a.parents, a.parents_dtype, row);
+  return (int)(p < 0 ? 0 : (p >= a.K ? a.K - 1 : p));
+}
+
+// KM = 0: source and destination apart; a thread = UN pieces of one row, or of one piece column over
+// rows where a row's segment is short.
+// KM > 0: in place; a thread = one piece of all K <= KM rows of an item.
+template <int VB, int KM>
+__device__ __forceinline__ void reorder_piece(const Reorder &a, const ReorderEntry &e, int64_t block) {
+  typedef typename Piece<VB>::type P;
+  constexpr int UN = KM ? 1 : REORDER_UNROLL;
+  const int64_t rows = KM ? a.N : a.N * a.K, pieces = e.seg_bytes / VB;
+  const int64_t span = e.flat ? rows * pieces : pieces, nb = (span + 256 * UN - 1) / (256 * UN);
+  const int64_t first = (block % nb) * (256 * UN) + threadIdx.x;
+  block /= nb;
+  int64_t row = 0;
+  if (!e.flat) {
+    row = block % rows;
+    block /= rows;
+  }
+  const int64_t seg = block % e.nseg, outer = block / e.nseg;
+  const int64_t off = outer * e.outer_stride + seg * e.seg_stride;
+  const char *src = (const char *)e.src + off;
+  char *dst = (char *)e.dst + off;
+  if (KM == 0) {
+    P v[UN];
+    int64_t to[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int64_t at = first + u * 256;
+      int64_t r = row, p = at;
+      if (e.flat) {
+        r = (uint32_t)at / (uint32_t)pieces;
+        p = at - r * pieces;
+      }
+      to[u] = -1;
+      if (at < span) {
+        const int64_t from = r / a.K * a.K + parent_of(a, r);
+        if (p * VB < live_bytes(a, e, from)) {
+          v[u] = *reinterpret_cast<const P *>(src + from * e.row_stride + p * VB);
+          to[u] = r * e.row_stride + p * VB;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+      if (to[u] >= 0) *reinterpret_cast<P *>(dst + to[u]) = v[u];
+  } else {
+    int64_t r = row, p = first;
+    if (first >= span) return;
+    if (e.flat) {
+      r = (uint32_t)first / (uint32_t)pieces;
+      p = first - r * pieces;
+    }
+    P v[KM ? KM : 1];
+    const int64_t r0 = r * a.K;
+#pragma unroll
+    for (int k = 0; k < KM; ++k)
+      if (k < a.K) {
+        const int f = parent_of(a, r0 + k);
+        if (f != k && p * VB < live_bytes(a, e, r0 + f))
+          v[k] = *reinterpret_cast<const P *>(src + (r0 + f) * e.row_stride + p * VB);
+      }
+#pragma unroll
+    for (int k = 0; k < KM; ++k)
+      if (k < a.K) {
+        const int f = parent_of(a, r0 + k);
+        if (f != k && p * VB < live_bytes(a, e, r0 + f))
+          *reinterpret_cast<P *>(dst + (r0 + k) * e.row_stride + p * VB) = v[k];
+      }
+  }
+}
+
+template <int KM>
+__global__ void __launch_bounds__(256) reorder_kernel(Reorder a) {
+  int64_t block = blockIdx.x;
+  int i = 0;
+  while (i + 1 < a.n && block >= a.e[i].blocks) block -= a.e[i++].blocks;
+  const ReorderEntry &e = a.e[i];
+  if (e.piece == 16) reorder_piece<16, KM>(a, e, block);
+  else if (e.piece == 4) reorder_piece<4, KM>(a, e, block);
+  else reorder_piece<1, KM>(a, e, block);
+}
+
+}  // namespace
+
+size_t beam_workspace_bytes(int64_t rows, int64_t V, int K) {
+  const int64_t slots = rows * ((V + CH - 1) / CH);
+  return (size_t)slots * (8 + 8 * (size_t)K);
+}
+
+void launch_beam_select(BeamSelect a, int64_t items, int dtype, void *ws, hipStream_t s) {
+  const int64_t rows = items * a.K;
+  a.chunks = (uint32_t)((a.V + CH - 1) / CH);
+  a.stats = (float *)ws;
+  a.cand_x = a.stats + rows * a.chunks * 2;
+  a.cand_i = (int32_t *)(a.cand_x + rows * a.chunks * a.K);
+  const int per = dtype == GNLP_BF16 ? 8 : 4;
+  const bool vec = ((uintptr_t)a.outputs & 15) == 0 && a.row_stride % per == 0 && a.V % per == 0;
+  const dim3 grid(a.chunks, (unsigned)rows), block(256);
+  if (dtype == GNLP_BF16) {
+    if (vec) hipLaunchKernelGGL((beam_chunk_kernel<bf16, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((beam_chunk_kernel<bf16, false>), grid, block, 0, s, a);
+  } else {
+    if (vec) hipLaunchKernelGGL((beam_chunk_kernel<float, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((beam_chunk_kernel<float, false>), grid, block, 0, s, a);
+  }
+  hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)items), block, 0, s, a);
+}
+
+// The caller has filled everything but piece and blocks.
+bool launch_reorder(Reorder a, bool in_place, hipStream_t s) {
+  int64_t total = 0;
+  for (int i = 0; i < a.n; ++i) {
+    ReorderEntry &e = a.e[i];
+    // (a length that ends inside a piece copies the whole piece: the slots behind it are free)
+    const uint64_t all = (uint64_t)(uintptr_t)e.src | (uint64_t)(uintptr_t)e.dst |
+                         (uint64_t)e.outer_stride | (uint64_t)e.row_stride |
+                         (uint64_t)e.seg_stride | (uint64_t)e.seg_bytes;
+    e.piece = (all & 15) == 0 ? 16 : (all & 3) == 0 ? 4 : 1;
+    const int64_t pieces = e.seg_bytes / e.piece, rows = in_place ? a.N : a.N * a.K;
+    const int64_t un = in_place ? 1 : REORDER_UNROLL;
+    e.flat = pieces < 256 * un && rows * pieces < (1LL << 31);
+    const int64_t span = e.flat ? rows * pieces : pieces;
+    e.blocks = (span + 256 * un - 1) / (256 * un) * (e.flat ? 1 : rows) * e.nseg * e.outer;
+    total += e.blocks;
+  }
+  if (total > 0x7fffffffLL) return false;
+  const dim3 grid((unsigned)total), block(256);
+  if (!in_place) hipLaunchKernelGGL(reorder_kernel<0>, grid, block, 0, s, a);
+  else if (a.K <= 4) hipLaunchKernelGGL(reorder_kernel<4>, grid, block, 0, s, a);
+  else if (a.K <= 8) hipLaunchKernelGGL(reorder_kernel<8>, grid, block, 0, s, a);
+  else if (a.K <= 16) hipLaunchKernelGGL(reorder_kernel<16>, grid, block, 0, s, a);
+  else hipLaunchKernelGGL(reorder_kernel<BEAM_MAX>, grid, block, 0, s, a);
+  return true;
+}
+
+}  // namespace gnlp

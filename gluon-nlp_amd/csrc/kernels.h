@@ -299,4 +299,82 @@ void launch_l2_normalize_bwd(void *dx, const void *g, const void *x, int dtype, 
                              int64_t d, float eps, hipStream_t s);
 void launch_cast_f32(void *out, int dtype, const float *in, int64_t n, hipStream_t s);
 
+// kv4.hip: 4-bit key / value cache (layout there)
+struct Kv4Io {
+  void *k_codes, *v_codes, *k_par, *v_par;
+  int64_t B, H, S, d, DP, L;          // L: time extent of k / v
+  int g_shift;                        // log2 of the groups of a token: DP == 64 << g_shift
+  uint32_t nblk;                      // blocks of 8 slots that L tokens can touch
+  void *k, *v;                        // write: source, read: destination (b, h, t strides)
+  int64_t k_stride[3], v_stride[3];
+  const void *length; int length_dtype;   // tokens held by each sequence (write: after this call)
+  const void *count; int count_dtype;     // write: how many of L are stored; read: first slot
+  int write;
+};
+void launch_kv4_io(const Kv4Io &a, int dtype, hipStream_t s);
+
+// kv4_attn.hip: attention over it
+struct Kv4Attn {
+  const void *k_codes, *v_codes, *k_par, *v_par;
+  int64_t B, H, S, d;
+  int64_t Lq; int share;              // queries; query heads per cached head
+  const void *q; int64_t q_stride[3]; // (b, query head, t)
+  void *out; int64_t o_stride[3];
+  const void *length; int length_dtype;
+  const void *q_length; int q_length_dtype;
+  int causal;
+  const void *edge; int64_t edge_stride[4];        // (b, query head, i, j); or
+  const void *table; int64_t table_len;            // (query heads, table_len), anchored at the query
+  const uint8_t *mask; int64_t mask_stride[3];
+  int64_t Lm;                         // keys that edge and mask reach (S when neither is given)
+  float inv_temperature;
+  int row_tiles, splits;
+  float *part_o, *part_ml;            // splits > 1: (row, split, DP) and (row, split, 2) in float
+};
+int kv4_attn_plan(int64_t B, int64_t H, int64_t rows, int64_t keys, int64_t d);   // splits
+void launch_kv4_attn(const Kv4Attn &a, int dtype, hipStream_t s);
+
+// beam.hip
+constexpr int BEAM_MAX = 32;          // beams of an item
+struct BeamSelect {
+  const void *outputs; int64_t row_stride;   // (items * K, V), rows row_stride elements apart
+  int64_t V; int K;
+  const float *scores;
+  const uint8_t *finished;            // or NULL
+  int normalize;                      // subtract the logsumexp
+  float exp_scale;                    // log2(e) / temperature
+  double inv_temperature, lp_prev, lp_new;
+  const void *step; int step_dtype;   // given: the length penalties come from it
+  double alpha, length_base;
+  int has_eos; int64_t eos;
+  uint32_t chunks;
+  float *stats, *cand_x;              // workspace: (row, chunk, 2), (row, chunk, K)
+  int32_t *cand_i;                    // (row, chunk, K), -1: none
+  float *out_scores;
+  int32_t *out_parents, *out_tokens;
+  uint8_t *out_finished;
+};
+size_t beam_workspace_bytes(int64_t rows, int64_t V, int K);
+void launch_beam_select(BeamSelect a, int64_t items, int dtype, void *ws, hipStream_t s);
+
+constexpr int REORDER_MAX = 32;       // tensors of a launch
+struct ReorderEntry {
+  const void *src; void *dst;
+  int64_t outer, outer_stride;        // rows lie under `outer` leading indices (bytes apart)
+  int64_t row_stride;                 // bytes
+  int64_t nseg, seg_stride, seg_bytes;   // a row = nseg segments
+  int64_t slots_per_unit, unit_bytes; // segments that hold tokens: slots share a unit (0: all copied)
+  int64_t blocks;
+  int piece;                          // bytes a thread moves at once
+  int flat;                           // short segments: a block runs over rows too
+};
+struct Reorder {
+  int64_t N; int K;
+  const void *parents; int parents_dtype;
+  const void *length; int length_dtype;   // per row, or NULL
+  int n;
+  ReorderEntry e[REORDER_MAX];
+};
+bool launch_reorder(Reorder a, bool in_place, hipStream_t s);
+
 }  // namespace gnlp

@@ -6,7 +6,7 @@ host tensors, an error is raised.  Build the library with ``python __graft_entry
 """
 import ctypes
 import os
-from ctypes import (POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t,
+from ctypes import (POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t,
                     c_uint8, c_void_p)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -79,6 +79,37 @@ class T5Cfg(Structure):
     _fields_ = [('d_model', c_int64), ('d_kv', c_int64), ('d_ff', c_int64), ('heads', c_int64),
                 ('gated', c_int), ('dtype', c_int), ('time_major', c_int), ('ln_eps', c_float),
                 ('bias_toeplitz', c_int)]
+
+
+class Kv4Cache(Structure):
+    _fields_ = [('B', c_int64), ('H', c_int64), ('slots', c_int64), ('d', c_int64),
+                ('k_codes', c_void_p), ('v_codes', c_void_p), ('k_par', c_void_p),
+                ('v_par', c_void_p)]
+
+
+class Kv4AttnDesc(Structure):
+    _fields_ = [('Lq', c_int64), ('share', c_int64), ('causal', c_int64), ('keys', c_int64),
+                ('q_stride', c_int64 * 3), ('o_stride', c_int64 * 3),
+                ('length', c_void_p), ('length_dtype', c_int64),
+                ('q_length', c_void_p), ('q_length_dtype', c_int64),
+                ('edge_scores', c_void_p), ('edge_stride', c_int64 * 4),
+                ('edge_table', c_void_p), ('table_len', c_int64),
+                ('mask', c_void_p), ('mask_stride', c_int64 * 3), ('Lm', c_int64),
+                ('temperature', c_double)]
+
+
+class BeamDesc(Structure):
+    _fields_ = [('N', c_int64), ('K', c_int64), ('V', c_int64), ('row_stride', c_int64),
+                ('normalize', c_int64), ('eos', c_int64), ('step', c_int64),
+                ('step_dev', c_void_p), ('step_dtype', c_int64),
+                ('temperature', c_double), ('alpha', c_double), ('length_base', c_double)]
+
+
+class State(Structure):
+    _fields_ = [('src', c_void_p), ('dst', c_void_p), ('outer', c_int64),
+                ('outer_stride', c_int64), ('row_stride', c_int64), ('nseg', c_int64),
+                ('seg_stride', c_int64), ('seg_bytes', c_int64), ('slots_per_unit', c_int64),
+                ('unit_bytes', c_int64)]
 
 
 I64x3 = c_int64 * 3
@@ -194,6 +225,20 @@ PROTOTYPES = {
                                                POINTER(T5BlockFolded), c_int, c_void_p, c_void_p,
                                                POINTER(T5Cfg), c_int64, c_int64, c_void_p, c_int,
                                                c_void_p, c_void_p, c_size_t, c_void_p]),
+    'gnlp_kv4_write': (c_int, [POINTER(Kv4Cache), c_void_p, c_void_p, c_int, c_int64,
+                               POINTER(c_int64), POINTER(c_int64), c_void_p, c_int, c_void_p,
+                               c_int, c_void_p]),
+    'gnlp_kv4_read': (c_int, [POINTER(Kv4Cache), c_void_p, c_void_p, c_int, c_int64,
+                              POINTER(c_int64), POINTER(c_int64), c_void_p, c_int, c_void_p,
+                              c_int, c_void_p]),
+    'gnlp_kv4_attn_workspace_bytes': (c_size_t, [POINTER(Kv4Cache), POINTER(Kv4AttnDesc)]),
+    'gnlp_kv4_attn': (c_int, [c_void_p, c_void_p, POINTER(Kv4Cache), POINTER(Kv4AttnDesc), c_int,
+                              c_void_p, c_size_t, c_void_p]),
+    'gnlp_beam_select_workspace_bytes': (c_size_t, [POINTER(BeamDesc)]),
+    'gnlp_beam_select': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                                 c_void_p, POINTER(BeamDesc), c_void_p, c_size_t, c_void_p]),
+    'gnlp_reorder_states': (c_int, [POINTER(State), c_int, c_int64, c_int64, c_void_p, c_int,
+                                    c_void_p, c_int, c_void_p]),
 }
 
 _lib = None

@@ -95,6 +95,18 @@ def stream(dev):
     return torch.cuda.current_stream(dev).cuda_stream
 
 
+def launch(dev, fn, *args):
+    """Call a C entry point whose last argument is the stream, on torch's current stream of ``dev``
+    and with ``dev`` as the current device; a non-zero status raises."""
+    if dev.index is None or torch.cuda.current_device() == dev.index:
+        rc = fn(*args, stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream(dev))
+    if rc:
+        _lib.check(rc)
+
+
 def valid_length_arg(vl, dev=None):
     """-> (tensor kept alive, pointer, int dtype code)."""
     if vl is None:

@@ -13,7 +13,8 @@ from .autograd import AttnFn, RelScoreFn, wants_grad
 from .op import l2_normalize
 
 __all__ = ['gen_self_attn_mask', 'gen_mem_attn_mask', 'masked_softmax', 'masked_logsoftmax',
-           'multi_head_dot_attn', 'MultiHeadAttentionCell', 'gen_rel_position',
+           'multi_head_dot_attn', 'multi_head_dot_attn_cached', 'MultiHeadAttentionCell',
+           'gen_rel_position',
            'RelAttentionScoreCell']
 
 
@@ -308,6 +309,97 @@ def multi_head_dot_attn(query, key, value, mask=None, edge_scores=None, dropout:
     return (T.like_caller(ctx, query),
             [T.like_caller(scores, query) if scores is not None else None,
              T.like_caller(weights, query) if weights is not None else None])
+
+
+def _expand_keys(x, lead, slots):
+    """Broadcast ``x`` (..., Lm) to lead + (Lm,); a last axis of 1 reaches every key."""
+    Lm = x.shape[-1] if x.dim() and x.shape[-1] != 1 else slots
+    return torch.broadcast_to(x, lead + (Lm,)), Lm
+
+
+def multi_head_dot_attn_cached(query, cache, layer=0, *, causal: bool = True, edge_scores=None,
+                               edge_table=None, mask=None, query_length=None, scaled: bool = True,
+                               query_head_units: Optional[int] = None, layout=None):
+    """``multi_head_dot_attn`` of a few queries over the keys and values of a ``QuantKVCache``
+    (incremental decoding; no counterpart in the reference, whose caches are float tensors).
+
+    query (B, Lq, H, d) in ``layout`` (default: the cache's), float32 or bfloat16; H a multiple of
+    the cached heads (query head h reads cached head h // (H / num_heads)).  ``causal``: the queries
+    are the last ``query_length`` (B,) (default Lq) tokens held, each sees the tokens up to its own;
+    otherwise every query sees all ``cache.length`` tokens.  Queries from ``query_length`` on, and
+    queries that see nothing, give zeros.
+
+    edge_scores, broadcastable to (B, H, Lq, Lm), is added before the scaling; edge_table (H, R) is
+    a bias by distance instead: a key adds entry R - 1 - (query position - key position), clamped to
+    the table (T5: ``RelAttentionScoreCell.self_attn_bias_table(R)[:, :R]``).  mask, broadcastable to
+    (B, Lq, Lm): true = attend.  Keys from Lm on are not seen.  scaled: divide by
+    sqrt(query_head_units) (default: the head's channels).
+
+    Returns context_vec (B, Lq, H * d) / (Lq, B, H * d).  There is no gradient: a query that asks
+    for one is refused."""
+    q = _inner_contig(T.as_tensor(query))
+    layout = cache.layout if layout is None else layout
+    if layout not in _LAYOUT_PERM:
+        raise NotImplementedError('layout="{}" is not supported! '
+                                  'We only support layout = "NKT", "NTK", and "TNK".'
+                                  .format(layout))
+    e, table, m = T.as_tensor(edge_scores), T.as_tensor(edge_table), T.as_tensor(mask)
+    dev = T.require_device(cache.length, q, e, table, m)
+    if q.dim() != 4:
+        raise ValueError('query {} is not 4-dimensional'.format(tuple(q.shape)))
+    B, H, Lq = _bht_shape(q, layout)
+    d = q.shape[-1]
+    if B != cache.batch_size or d != cache.head_units or H % cache.num_heads or H == 0:
+        raise ValueError('query {} (layout {}) does not match {}'.format(tuple(q.shape), layout,
+                                                                        cache))
+    if wants_grad(q, e, table):
+        raise NotImplementedError('attention over a 4-bit cache has no gradient: decode under '
+                                  'torch.no_grad()')
+    a = _lib.Kv4AttnDesc()
+    a.Lq, a.share, a.causal, a.keys = Lq, H // cache.num_heads, bool(causal), cache._bound
+    a.q_stride[:] = _bht_strides(q, layout)
+    if layout == 'TNK':
+        ctx = torch.empty((Lq, B, H * d), dtype=q.dtype, device=dev)
+        a.o_stride[:] = (H * d, d, B * H * d)
+    else:
+        ctx = torch.empty((B, Lq, H * d), dtype=q.dtype, device=dev)
+        a.o_stride[:] = (Lq * H * d, d, H * d)
+    a.length, a.length_dtype = cache.length.data_ptr(), _lib.I32
+    if query_length is not None:
+        ql = cache._lengths(query_length, 'query_length')
+        a.q_length = ql.data_ptr()
+        a.q_length_dtype = _lib.I64 if ql.dtype == torch.int64 else _lib.I32
+    slots = Lm = cache._slots
+    if e is not None:
+        if table is not None:
+            raise ValueError('edge_scores and edge_table exclude each other')
+        if e.dtype != q.dtype:
+            e = e.to(q.dtype)
+        e, Lm = _expand_keys(e, (B, H, Lq), slots)
+        a.edge_scores, a.edge_stride[:] = e.data_ptr(), e.stride()
+    elif table is not None:
+        if table.dim() != 2 or table.shape[0] != H or table.shape[1] < 1:
+            raise ValueError('edge_table {} != (heads = {}, R >= 1)'.format(tuple(table.shape), H))
+        table = table.to(q.dtype).contiguous()
+        a.edge_table, a.table_len = table.data_ptr(), table.shape[1]
+    if m is not None:
+        if m.dtype != torch.bool:
+            m = m != 0
+        m, Lmm = _expand_keys(m, (B, Lq), slots)
+        if e is not None and Lm != Lmm and slots not in (Lm, Lmm):
+            raise ValueError('edge_scores reach {} keys, mask {}'.format(Lm, Lmm))
+        Lm = min(Lm, Lmm)
+        a.mask, a.mask_stride[:] = m.data_ptr(), m.stride()
+    a.Lm = Lm
+    if scaled:
+        a.temperature = math.sqrt(d if query_head_units is None else query_head_units)
+    lib = _lib.load()
+    desc = ctypes.byref(cache.layer_desc(layer))
+    nws = lib.gnlp_kv4_attn_workspace_bytes(desc, ctypes.byref(a))
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    T.launch(dev, lib.gnlp_kv4_attn, ctx.data_ptr(), q.data_ptr(), desc, ctypes.byref(a),
+             T.code(q), T.ptr(ws), nws)
+    return T.like_caller(ctx, query)
 
 
 class MultiHeadAttentionCell(torch.nn.Module):

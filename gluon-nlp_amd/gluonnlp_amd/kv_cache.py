@@ -1,0 +1,216 @@
+"""Key / value cache of incremental decoding, held in 4 bits.
+
+The decoders' own states are float tensors that grow by concatenation (reference
+models/transformer.py:607-734, models/t5.py:374-490).  ``QuantKVCache`` keeps the same keys and
+values in 72 bytes a token and head of 64 channels where bfloat16 takes 256, in buffers that do not
+move: a decoding step neither allocates nor copies the past, and can be captured in a graph.
+``attention_cell.multi_head_dot_attn_cached`` attends over it.
+
+The format (include/gluonnlp_amd.h): 64 channels of a token and head share a scale and a minimum in
+bfloat16, a value is ``code * scale + minimum`` with a code of 0 .. 15; the error of a value is at
+most half a scale, (max - min) / 30, plus the roundings of scale and minimum to bfloat16.
+"""
+import ctypes
+
+import torch
+
+from . import _lib
+from . import _tensor as T
+from .autograd import wants_grad
+
+__all__ = ['QuantKVCache']
+
+_TIME = {'NKT': 2, 'NTK': 1, 'TNK': 0}
+_PERM = {'NKT': (0, 1, 2), 'NTK': (0, 2, 1), 'TNK': (1, 2, 0)}
+
+
+class QuantKVCache:
+    """Keys and values of ``num_layers`` attention layers, ``max_length`` tokens of ``batch_size``
+    sequences, ``num_heads`` cached heads of ``head_units`` (1 .. 128) channels.
+
+    A step: ``cache.extend(n)`` counts the n new tokens of every sequence in, then each layer
+    stores them with ``cache.write(key, value, layer)`` and attends.  All layers share ``length``,
+    a device int32 vector (batch_size,) of the tokens held: nothing is read back to the host, and a
+    captured graph replays with the lengths of its time.  ``layout`` is that of the keys and values
+    ('NTK', 'NKT' or 'TNK' as in ``multi_head_dot_attn``).
+
+    Tokens that would lie beyond ``max_length`` are not stored; ``extend`` refuses what it can see
+    (inside a graph it cannot).  Two writes, or a write and a reading call, on different streams
+    have to be ordered by the caller, like any two uses of a tensor."""
+
+    def __init__(self, batch_size, num_heads, head_units, max_length, num_layers=1, ctx=None,
+                 layout='NTK'):
+        if layout not in _PERM:
+            raise NotImplementedError('layout="{}" is not supported! We only support layout = '
+                                      '"NKT", "NTK", and "TNK".'.format(layout))
+        for name, v, lo, hi in (('batch_size', batch_size, 1, 65535),
+                                ('num_heads', num_heads, 1, 65535),
+                                ('head_units', head_units, 1, 128),
+                                ('max_length', max_length, 1, 2 ** 30 - 32),
+                                ('num_layers', num_layers, 1, 65535)):
+            if not lo <= int(v) <= hi:
+                raise ValueError('{}={} is outside [{}, {}]'.format(name, v, lo, hi))
+        self.batch_size, self.num_heads, self.head_units = batch_size, num_heads, head_units
+        self.max_length, self.num_layers, self.layout = max_length, num_layers, layout
+        dev = torch.device('cuda' if ctx is None else ctx)
+        if dev.type == 'cuda' and dev.index is None:
+            dev = torch.device('cuda', torch.cuda.current_device())
+        self.device = dev
+        self._slots = slots = (max_length + 31) // 32 * 32
+        self._padded = padded = 64 if head_units <= 64 else 128
+        groups = padded // 64
+        lead = (num_layers, batch_size, num_heads)
+        self._k_codes = torch.zeros(lead + (slots, padded // 2), dtype=torch.uint8, device=dev)
+        self._v_codes = torch.zeros(lead + (slots // 8, padded), dtype=torch.int32, device=dev)
+        self._k_par = torch.zeros(lead + (groups, slots), dtype=torch.int32, device=dev)
+        self._v_par = torch.zeros(lead + (groups, slots), dtype=torch.int32, device=dev)
+        self.length = torch.zeros(batch_size, dtype=torch.int32, device=dev)
+        self._bound = 0            # no sequence holds more tokens
+        self._desc = []
+        for i in range(num_layers):
+            c = _lib.Kv4Cache()
+            c.B, c.H, c.slots, c.d = batch_size, num_heads, slots, head_units
+            c.k_codes, c.v_codes = self._k_codes[i].data_ptr(), self._v_codes[i].data_ptr()
+            c.k_par, c.v_par = self._k_par[i].data_ptr(), self._v_par[i].data_ptr()
+            self._desc.append(c)
+
+    def __repr__(self):
+        return '{}(batch_size={}, num_heads={}, head_units={}, max_length={}, num_layers={}, ' \
+               'layout="{}")'.format(self.__class__.__name__, self.batch_size, self.num_heads,
+                                     self.head_units, self.max_length, self.num_layers, self.layout)
+
+    def layer_desc(self, layer):
+        if not 0 <= layer < self.num_layers:
+            raise IndexError('layer {} of {}'.format(layer, self.num_layers))
+        return self._desc[layer]
+
+    def _lengths(self, v, name):
+        """A (batch_size,) device vector of whole numbers."""
+        v = T.as_tensor(v)
+        if v.dtype not in (torch.int32, torch.int64):
+            raise TypeError('{} must be int32 or int64, got {}'.format(name, v.dtype))
+        if v.dim() != 1 or v.shape[0] != self.batch_size:
+            raise ValueError('{} {} != (batch_size,) = ({},)'.format(name, tuple(v.shape),
+                                                                     self.batch_size))
+        T.require_device(self.length, v)
+        return v.contiguous()
+
+    # ---- lengths ----
+    def reset(self):
+        """Forget all tokens."""
+        self.length.zero_()
+        self._bound = 0
+
+    def set_length(self, length):
+        """Set the number of tokens held, an int or a (batch_size,) vector."""
+        if isinstance(length, int):
+            if not 0 <= length <= self.max_length:
+                raise ValueError('length={} is outside [0, {}]'.format(length, self.max_length))
+            self.length.fill_(length)
+            self._bound = length
+        else:
+            self.length.copy_(self._lengths(length, 'length'))
+            self._bound = self.max_length
+
+    def extend(self, n, new_length=None):
+        """Count in n new tokens of every sequence (``new_length``: its own number of each, at most
+        n).  They are stored by the ``write`` calls that follow."""
+        if n < 0 or n > self.max_length:
+            raise ValueError('n={} is outside [0, max_length={}]'.format(n, self.max_length))
+        if new_length is not None:
+            new_length = self._lengths(new_length, 'new_length')
+        capturing = self.device.type == 'cuda' and torch.cuda.is_current_stream_capturing()
+        if self._bound + n > self.max_length and not capturing:
+            # the bound is loose after ragged steps: look (the one place that waits for the device)
+            self._bound = max(0, int(self.length.max()))
+            grown = self._bound + n if new_length is None else \
+                int((self.length + new_length.clamp(0, n)).max())
+            if grown > self.max_length:
+                raise ValueError('{} tokens do not fit max_length={}'.format(grown,
+                                                                            self.max_length))
+        if new_length is None:
+            self.length.add_(n)
+        else:
+            self.length.add_(new_length.clamp(0, n))
+        self._bound = min(self._bound + n, self.max_length)
+
+    # ---- tokens ----
+    def _strides(self, x):
+        st, p = x.stride(), _PERM[self.layout]
+        return _lib.I64x3(st[p[0]], st[p[1]], st[p[2]])
+
+    def _check_tokens(self, x, name):
+        p = _PERM[self.layout]
+        if x.dim() != 4 or x.shape[p[0]] != self.batch_size or x.shape[p[1]] != self.num_heads \
+                or x.shape[3] != self.head_units:
+            raise ValueError('{} {} does not match {}'.format(name, tuple(x.shape), self))
+        return x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous()
+
+    def write(self, key, value, layer=0, new_length=None):
+        """Store the last tokens counted in: key / value (batch_size, n, num_heads, head_units) in
+        the cache's layout go to the last n of the ``length`` tokens of each sequence.  With
+        ``new_length`` (batch_size,), sequence b stores its first new_length[b] tokens as its last
+        new_length[b] (the others, padding, are not read).  Other tokens keep their values."""
+        k = self._check_tokens(T.as_tensor(key), 'key')
+        v = self._check_tokens(T.as_tensor(value), 'value')
+        dev = T.require_device(self.length, k, v)
+        if wants_grad(k, v):
+            raise NotImplementedError('a 4-bit cache has no gradient: decode under torch.no_grad()')
+        if k.dtype != v.dtype or k.shape != v.shape:
+            raise ValueError('key and value must share shape and dtype')
+        n = k.shape[_TIME[self.layout]]
+        if new_length is None and n > self._bound:
+            raise ValueError('write of {} tokens, {} are counted in: call extend() first'
+                             .format(n, self._bound))
+        nl, code = None, 0
+        if new_length is not None:
+            nl = self._lengths(new_length, 'new_length')
+            code = _lib.I64 if nl.dtype == torch.int64 else _lib.I32
+        T.launch(dev, _lib.load().gnlp_kv4_write, ctypes.byref(self.layer_desc(layer)),
+                 k.data_ptr(), v.data_ptr(), T.code(k), n, self._strides(k), self._strides(v),
+                 self.length.data_ptr(), _lib.I32, T.ptr(nl), code)
+
+    def read(self, n=None, start=None, layer=0, dtype='float32'):
+        """The values held: (key, value) of n tokens (default: max_length) from ``start``
+        (batch_size,) on (default 0), in the cache's layout; zeros where no token is held."""
+        n = self.max_length if n is None else int(n)
+        if n < 0:
+            raise ValueError('n={} is negative'.format(n))
+        dev = T.require_device(self.length)
+        st, code = None, 0
+        if start is not None:
+            st = self._lengths(start, 'start')
+            code = _lib.I64 if st.dtype == torch.int64 else _lib.I32
+        B, H, d = self.batch_size, self.num_heads, self.head_units
+        shape = {'NKT': (B, H, n, d), 'NTK': (B, n, H, d), 'TNK': (n, B, H, d)}[self.layout]
+        dt = T.torch_dtype(dtype)
+        key = torch.empty(shape, dtype=dt, device=dev)
+        value = torch.empty(shape, dtype=dt, device=dev)
+        T.launch(dev, _lib.load().gnlp_kv4_read, ctypes.byref(self.layer_desc(layer)),
+                 key.data_ptr(), value.data_ptr(), T.code(key), n, self._strides(key),
+                 self._strides(value), self.length.data_ptr(), _lib.I32, T.ptr(st), code)
+        return key, value
+
+    def reorder(self, parents):
+        """Beam search: sequence n K + k goes on from sequence n K + parents[n, k]; ``parents``
+        (items, K) whole numbers in [0, K), K <= 32.  In place, all layers in one launch; only the
+        tokens held are moved."""
+        from .sequence_sampler import check_parents, launch_reorder
+        p, N, K = check_parents(parents, self.batch_size)
+        dev = T.require_device(self.length, p)
+        if K > 32:
+            raise ValueError('beam size {} > 32'.format(K))
+        flat = []
+        L, B, H, S = self.num_layers, self.batch_size, self.num_heads, self._slots
+        groups = self._padded // 64
+        for t, nseg, per, unit in ((self._k_codes, H, 1, self._padded // 2),
+                                   (self._v_codes, H, 8, self._padded * 4),
+                                   (self._k_par, H * groups, 1, 4),
+                                   (self._v_par, H * groups, 1, 4)):
+            seg = S // per * unit
+            row = nseg * seg
+            flat += [t.data_ptr(), t.data_ptr(), L, B * row, row, nseg, seg, seg, per, unit]
+        launch_reorder(dev, flat, N, K, p, self.length)
+        # (a launch of its own: the one above reads the lengths)
+        at = self.length.data_ptr()
+        launch_reorder(dev, [at, at, 1, 4 * B, 4, 1, 4, 4, 0, 0], N, K, p, None)

@@ -574,6 +574,114 @@ int gnlp_profile_dense_arm(int64_t M, int64_t N, int64_t K, int capacity);
 int gnlp_profile_dense_read(float *ms, int capacity);
 int gnlp_profile_dense_disarm(void);
 
+/* ---------------------------------------------------------------------------------------------
+ * Incremental decoding with a key / value cache held in 4 bits, and beam search (the callers of
+ * incremental_decode, models/transformer.py:637-734, models/t5.py:391-490; the reference's own
+ * caches are float tensors grown by concatenation).  Inference only.
+ *
+ * Format: 64 consecutive channels of one token and head (the last group may be shorter) share
+ *   scale = bf16((max - min) * fl32(1 / 15)),  minimum = bf16(min),
+ *   code = clamp(rint((x - minimum) / scale), 0, 15),  value = code * scale + minimum
+ * (32-bit arithmetic).  scale < 2^-126 counts as 0.  A group that holds a NaN or an infinity, or
+ * whose range is not finite, reads back as NaN.
+ * gnlp_kv4_cache names the arrays of ONE layer, each contiguous, 16-byte aligned, DP = 64 if
+ * d <= 64 else 128, G = DP / 64, slots a multiple of 32 (slot = token position):
+ *   k_codes [B][H][slots][DP / 2] bytes     8 channels of a token to a 32-bit word
+ *   v_codes [B][H][slots / 8][DP] words     8 tokens of a channel to a 32-bit word
+ *   k_par, v_par [B][H][G][slots] words     scale in the low 16 bits, minimum in the high
+ * Element e of a word: nibble (e >> 1) + 4 (e & 1).  Lengths are device vectors of B entries (int32
+ * or int64): no call synchronises with the host.  A length beyond `slots` counts as `slots`.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct {
+  int64_t B, H, slots, d;   /* sequences, cached heads, slots, head dim 1 .. 128 */
+  void *k_codes, *v_codes, *k_par, *v_par;
+} gnlp_kv4_cache;
+
+/* Store tokens: token i < n[b] of key / value goes to slot length[b] - n[b] + i, n[b] =
+ * new_length[b] clamped to [0, L] (L when new_length is NULL); length[b] counts the tokens held
+ * AFTER the call (NULL: L).  Slots outside [0, slots) are not written; tokens from n[b] on are not
+ * read; every other slot keeps its contents.  key / value: element (b, h, t, c) at
+ * b * stride[0] + h * stride[1] + t * stride[2] + c.  Two calls on one cache must be ordered: two
+ * neighbouring tokens share a word. */
+int gnlp_kv4_write(const gnlp_kv4_cache *cache, const void *key, const void *value, int dtype,
+                   int64_t L, const int64_t key_stride[3], const int64_t value_stride[3],
+                   const void *length, int length_dtype, const void *new_length,
+                   int new_length_dtype, gnlp_stream_t stream);
+
+/* Read back: token i < L of the outputs = slot start[b] + i (start NULL: 0); 0 where that slot is
+ * outside [0, length[b]) (length NULL: all slots). */
+int gnlp_kv4_read(const gnlp_kv4_cache *cache, void *key, void *value, int dtype, int64_t L,
+                  const int64_t key_stride[3], const int64_t value_stride[3], const void *length,
+                  int length_dtype, const void *start, int start_dtype, gnlp_stream_t stream);
+
+/* ctx = softmax((q k^T + edge) / temperature, over the keys the query sees) v for Lq queries of
+ * H * share query heads; query head hq reads cached head hq / share.
+ *   causal = 0: every query sees the length[b] tokens held;
+ *   causal = 1: the queries are the last q_length[b] (NULL: Lq) tokens held, query i at position
+ *               length[b] - q_length[b] + i sees the tokens up to its own.
+ *   Queries i >= q_length[b], and queries that see nothing, give 0.
+ * edge_scores: element (b, hq, i, j) by edge_stride (0 = broadcast), dtype like q; or edge_table
+ *   (H * share, table_len): key j adds entry table_len - 1 - (position of query i - j), clamped to
+ *   the table (a bias by distance, as T5's decoder has; position as for causal = 1).  Not both.
+ * mask: bytes (b, i, j) by mask_stride, 1 = attend.  edge_scores and mask reach keys j < Lm; keys
+ *   from Lm on are not seen (Lm is ignored when neither is given).
+ * Nothing of a slot that no query sees can reach ctx, whatever it holds.
+ * temperature <= 0 means 1.  keys: the longest length to expect, a hint from which the number of
+ * workgroups follows; any length gives right results.
+ * workspace: gnlp_kv4_attn_workspace_bytes, contents need not be kept. */
+typedef struct {
+  int64_t Lq, share, causal, keys;
+  int64_t q_stride[3], o_stride[3];      /* (b, query head, t) */
+  const void *length; int64_t length_dtype;
+  const void *q_length; int64_t q_length_dtype;
+  const void *edge_scores; int64_t edge_stride[4];
+  const void *edge_table; int64_t table_len;
+  const uint8_t *mask; int64_t mask_stride[3];
+  int64_t Lm;
+  double temperature;
+} gnlp_kv4_attn_desc;
+size_t gnlp_kv4_attn_workspace_bytes(const gnlp_kv4_cache *cache, const gnlp_kv4_attn_desc *d);
+int gnlp_kv4_attn(void *ctx, const void *q, const gnlp_kv4_cache *cache,
+                  const gnlp_kv4_attn_desc *d, int dtype, void *workspace, size_t workspace_bytes,
+                  gnlp_stream_t stream);
+
+/* One selection of a beam search over N items of K beams (1 <= K <= 32) and V tokens.  A candidate
+ * of an unfinished beam k and token v scores
+ *   (scores[k] * lp(step - 1) + z[k, v] - lse[k]) / lp(step),  z = outputs / temperature,
+ *   lp(s) = ((length_base + s) / (length_base + 1)) ^ alpha,
+ * lse = logsumexp of z over v (0 when normalize = 0); a finished beam has one candidate, itself
+ * with scores[k] (token -1, parent k).  The K best of an item in order, ties to the lowest k V + v,
+ * finished beams last.  NaN outputs count as -inf, +inf as the largest float; a beam whose score is
+ * not above -1e15 is dead: its candidates count as -inf.  outputs of finished beams are not read.
+ * out_finished = parent finished or token == eos (eos < 0: none).  step_dev: the step as a device
+ * integer (graphs), else NULL and `step`.  Outputs must not alias inputs. */
+typedef struct {
+  int64_t N, K, V, row_stride;           /* outputs: (N * K, V), rows row_stride elements apart */
+  int64_t normalize, eos, step;
+  const void *step_dev; int64_t step_dtype;
+  double temperature, alpha, length_base;
+} gnlp_beam_desc;
+size_t gnlp_beam_select_workspace_bytes(const gnlp_beam_desc *d);
+int gnlp_beam_select(float *out_scores, int32_t *out_parents, int32_t *out_tokens,
+                     uint8_t *out_finished, const void *outputs, int dtype, const float *scores,
+                     const uint8_t *finished, const gnlp_beam_desc *d, void *workspace,
+                     size_t workspace_bytes, gnlp_stream_t stream);
+
+/* Reorder decoding states after a selection: row n K + k of every tensor becomes its row
+ * n K + parents[n K + k] (parents outside [0, K) are clamped).  Each of the `count` tensors: rows
+ * row_stride bytes apart, under `outer` leading indices (outer_stride bytes), a row = nseg segments
+ * of seg_bytes (seg_stride bytes apart).  slots_per_unit > 0 (with `length`, the tokens that each
+ * row holds): a segment holds tokens, slots_per_unit of them to unit_bytes, and only what the
+ * source row's length covers has to move.  dst == src for all of them: in place (K <= 32);
+ * otherwise no dst may overlap any src.  `length` may not be among the tensors. */
+typedef struct {
+  const void *src; void *dst;
+  int64_t outer, outer_stride, row_stride, nseg, seg_stride, seg_bytes, slots_per_unit, unit_bytes;
+} gnlp_state;
+int gnlp_reorder_states(const gnlp_state *states, int count, int64_t N, int64_t K,
+                        const void *parents, int parents_dtype, const void *length,
+                        int length_dtype, gnlp_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
