@@ -1764,6 +1764,12 @@ int kv4_io(const gnlp_kv4_cache *c, void *k, void *v, int dtype, int64_t L, cons
   return check_launch(write ? "gnlp_kv4_write" : "gnlp_kv4_read");
 }
 
+// bytes from a state's first to its last (strides are not negative)
+int64_t state_span(const gnlp_state &t, int64_t rows) {
+  return (t.outer - 1) * t.outer_stride + (rows - 1) * t.row_stride + (t.nseg - 1) * t.seg_stride +
+         t.seg_bytes;
+}
+
 int kv4_splits(const gnlp_kv4_cache *c, const gnlp_kv4_attn_desc *d) {
   int64_t keys = d->keys > 0 && d->keys < c->slots ? d->keys : c->slots;
   if ((d->edge_scores || d->mask) && d->Lm < keys) keys = d->Lm;
@@ -1827,6 +1833,9 @@ int gnlp_kv4_attn(void *ctx, const void *q, const gnlp_kv4_cache *cache,
     a.mask_stride[i] = d->mask_stride[i];
   }
   for (int i = 0; i < 4; ++i) a.edge_stride[i] = d->edge_stride[i];
+  const int64_t per16 = dtype == GNLP_BF16 ? 8 : 4;
+  a.q_vec = cache->d % 8 == 0 && ((uintptr_t)q & 15) == 0 && d->q_stride[0] % per16 == 0 &&
+            d->q_stride[1] % per16 == 0 && d->q_stride[2] % per16 == 0;
   a.length = d->length; a.length_dtype = (int)d->length_dtype;
   a.q_length = d->q_length; a.q_length_dtype = (int)d->q_length_dtype;
   a.causal = d->causal != 0;
@@ -1915,6 +1924,8 @@ int gnlp_reorder_states(const gnlp_state *states, int count, int64_t N, int64_t 
   for (int i = 0; i < count; ++i) {
     const gnlp_state &t = states[i];
     REQUIRE(t.outer >= 0 && t.nseg >= 0 && t.seg_bytes >= 0, "state %d: negative extent", i);
+    REQUIRE(t.outer_stride >= 0 && t.row_stride >= 0 && t.seg_stride >= 0,
+            "state %d: negative stride", i);
     if (t.outer * t.nseg * t.seg_bytes == 0) continue;
     REQUIRE(t.src && t.dst, "state %d: NULL tensor", i);
     if (seen++ == 0) in_place = t.src == t.dst;
@@ -1922,6 +1933,17 @@ int gnlp_reorder_states(const gnlp_state *states, int count, int64_t N, int64_t 
     REQUIRE(t.slots_per_unit == 0 || (t.slots_per_unit > 0 && t.unit_bytes > 0),
             "state %d: bad units", i);
   }
+  // no destination may be read by another row, or written twice
+  for (int i = 0; i < count; ++i)
+    for (int j = 0; j < count; ++j) {
+      const gnlp_state &s = states[i], &t = states[j];
+      const int64_t n = s.outer * s.nseg * s.seg_bytes, m = t.outer * t.nseg * t.seg_bytes;
+      if (n == 0 || m == 0) continue;
+      const char *d = (const char *)s.dst, *x = (const char *)t.src, *y = (const char *)t.dst;
+      const int64_t ds = state_span(s, N * K), ts = state_span(t, N * K);
+      if (j < i) REQUIRE(d + ds <= y || y + ts <= d, "states %d and %d: destinations overlap", j, i);
+      if (!in_place) REQUIRE(d + ds <= x || x + ts <= d, "state %d written over state %d", i, j);
+    }
   REQUIRE(!in_place || K <= BEAM_MAX, "in place: beam size %lld outside [1, %d]", (long long)K,
           BEAM_MAX);
   for (int first = 0; first < count; first += REORDER_MAX) {

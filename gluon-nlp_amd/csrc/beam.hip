@@ -9,15 +9,19 @@
 // k V + v (finished beams: K V + k).  A beam whose previous score is not above -1e15 is dead: all
 // its candidates count as -inf.
 //
-// Candidates of one beam are ordered by their logits alone, so the K best of every 4096 logits are
-// found first (beam_chunk_kernel, one pass over the logits, which also leaves the maximum and the
-// sum of exponentials), and the few that are left are scored in 64 bits (beam_merge_kernel: beams
-// that come near each other are told apart by the logsumexp's last digits).
-//   The K best of a chunk: a wave's 64 lane maxima are bisected, by ballots over the 16 high bits of
-//   an order-preserving integer, for a bound that K lanes reach; the best bound of the four waves
+// Candidates of one beam are ordered by their logits alone, so the K best of every chunk of 4096 or
+// 8192 logits are found first (beam_chunk_kernel, one pass over the logits, which also leaves the
+// maximum and the sum of exponentials), and the few that are left are scored in 64 bits
+// (beam_merge_kernel: beams that come near each other are told apart by the logsumexp's last
+// digits).
+//   The K best of a chunk: a wave's 64 lane maxima are bisected, by ballots over the high bits of an
+//   order-preserving integer, for a bound that K lanes reach; the best bound of the four waves
 //   leaves little more than K values, which a list in LDS ranks by counting.  Where ties overfill
 //   the list (a constant row), K rounds of a block-wide maximum do it.
-// Bound by memory: the logits once.
+//   The merge does the same with the chunks' best candidates and walks down a chunk's list only
+//   while it stays above the bound.
+// Bound by memory (the logits once) and by the instructions of the pass: 10 a logit, of which the
+// exponential's 4; a workgroup of 8192 logits spreads the 400 or so that it spends on top.
 //
 // Reordering.  out[row] = in[parent's row] for a list of tensors of any size, in one launch.  In
 // place, a thread holds its 16 bytes of all K beams before it writes any, and rows that keep their
@@ -28,8 +32,6 @@
 namespace gnlp {
 namespace {
 
-constexpr int CH_E = 16;                        // values of a thread
-constexpr int CH = 256 * CH_E;                  // values of a workgroup
 constexpr int CAP = 512;                        // list of survivors
 constexpr float NEG = -__builtin_inff();
 
@@ -42,19 +44,52 @@ __device__ __forceinline__ uint64_t ordered(double x) {
   const uint64_t u = __builtin_bit_cast(uint64_t, x);
   return (u >> 63) ? ~u : u | 0x8000000000000000ull;
 }
-// -0 and +0 are one score
-__device__ __forceinline__ float plain_zero(float x) { return x + 0.0f; }
-
-__device__ __forceinline__ float sane(float x) {   // fmaxf(NaN, y) = y
-  return fminf(fmaxf(x, NEG), 3.4028234663852886e38f);
+// a number whose ordered() is at most `bits` (low bits of the integer cleared by the bisection)
+__device__ __forceinline__ float unordered(uint32_t bits) {
+  if (bits <= 0x007fffffu) return NEG;                  // (below every number: -inf)
+  return __builtin_bit_cast(float, (bits & 0x80000000u) ? bits & 0x7fffffffu : ~bits);
 }
 
-// a bound, of 16 high bits of the keys, that at least K of the wave's 64 keys reach (0 if fewer
-// than K are above 0)
+// NaN counts as -inf (the median of three with a NaN is the smaller of the others), +inf as the
+// largest number
+__device__ __forceinline__ float sane(float x) {
+  return __builtin_amdgcn_fmed3f(x, NEG, 3.4028234663852886e38f);
+}
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_else(float other, float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+      __builtin_bit_cast(int, other), __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float lane63(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+__device__ __forceinline__ float all_max(float x) {      // row shifts, then the rows' last lanes
+  x = fmaxf(x, dpp_else<0x111, 0xf>(NEG, x));
+  x = fmaxf(x, dpp_else<0x112, 0xf>(NEG, x));
+  x = fmaxf(x, dpp_else<0x114, 0xf>(NEG, x));
+  x = fmaxf(x, dpp_else<0x118, 0xf>(NEG, x));
+  x = fmaxf(x, dpp_else<0x142, 0xa>(NEG, x));
+  x = fmaxf(x, dpp_else<0x143, 0xc>(NEG, x));
+  return lane63(x);
+}
+__device__ __forceinline__ float all_sum(float x) {
+  x += dpp_else<0x111, 0xf>(0.f, x);
+  x += dpp_else<0x112, 0xf>(0.f, x);
+  x += dpp_else<0x114, 0xf>(0.f, x);
+  x += dpp_else<0x118, 0xf>(0.f, x);
+  x += dpp_else<0x142, 0xa>(0.f, x);
+  x += dpp_else<0x143, 0xc>(0.f, x);
+  return lane63(x);
+}
+
+// a bound, of the high bits of the keys down to LOW, that at least K of the wave's 64 keys reach (0
+// if fewer than K are above 0)
+template <int LOW>
 __device__ __forceinline__ uint32_t wave_bound(uint32_t key, int K) {
   uint32_t bound = 0;
 #pragma unroll
-  for (int bit = 31; bit >= 16; --bit) {
+  for (int bit = 31; bit >= LOW; --bit) {
     const uint32_t next = bound | (1u << bit);
     if ((int)__popcll(__ballot(key >= next)) >= K) bound = next;
   }
@@ -65,15 +100,16 @@ __device__ __forceinline__ bool better(float x, uint32_t i, float y, uint32_t j)
   return x > y || (x == y && i < j);
 }
 
-template <typename T, bool VEC>
+// E: values of a thread
+template <typename T, bool VEC, int E>
 __global__ void __launch_bounds__(256) beam_chunk_kernel(BeamSelect a) {
-  __shared__ float lx[CAP];
-  __shared__ uint32_t li[CAP];
+  __shared__ uint64_t list[CAP];           // ordered value above, complement of the index below
   __shared__ uint32_t sh_n, sh_bound[4];
   __shared__ float sh_m[4], sh_s[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t row = blockIdx.y;
-  const uint32_t chunk = blockIdx.x, base = chunk * CH, V = (uint32_t)a.V;
+  const uint32_t chunk = blockIdx.x, base = chunk * (256 * E), V = (uint32_t)a.V;
   if (a.finished && a.finished[row]) return;
   const bool dead = !(a.scores[row] > -1e15f);
   const T *src = (const T *)a.outputs + row * a.row_stride;
@@ -82,39 +118,41 @@ __global__ void __launch_bounds__(256) beam_chunk_kernel(BeamSelect a) {
   // value e of a thread is element base + at(e)
   constexpr int PER = VEC ? 16 / (int)sizeof(T) : 1;
   auto at = [&](int e) -> uint32_t { return base + (e / PER) * (256 * PER) + tid * PER + e % PER; };
-  float x[CH_E];
+  float x[E];
+  const bool whole = base + 256 * E <= V;
 #pragma unroll
-  for (int v = 0; v < CH_E / PER; ++v) {
+  for (int v = 0; v < E / PER; ++v) {
     const uint32_t i = at(v * PER);
     if (VEC) {
-      if (i < V) {
-        const typename VecOf<T>::type w = *reinterpret_cast<const typename VecOf<T>::type *>(src + i);
+      typename VecOf<T>::type w;
+      if (whole || i < V) w = *reinterpret_cast<const typename VecOf<T>::type *>(src + i);
 #pragma unroll
-        for (int e = 0; e < PER; ++e) x[v * PER + e] = to_f32((T)w[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < PER; ++e) x[v * PER + e] = NEG;
-      }
+      for (int e = 0; e < PER; ++e) x[v * PER + e] = whole || i < V ? to_f32((T)w[e]) : NEG;
     } else {
-      x[v] = i < V ? to_f32(src[i]) : NEG;
+      x[v] = whole || i < V ? to_f32(src[i]) : NEG;
     }
   }
   float most = NEG;
-  uint32_t any = 0;                                      // whether the lane holds an element at all
 #pragma unroll
-  for (int e = 0; e < CH_E; ++e) {
-    x[e] = dead ? NEG : plain_zero(sane(x[e]));
+  for (int e = 0; e < E; ++e) {
+    x[e] = dead ? NEG : sane(x[e]);
     most = fmaxf(most, x[e]);
-    any |= at(e) < V;
   }
-  const uint32_t bound = wave_bound(any ? ordered(most) : 0u, a.K);
-  const float wm = wave_max(most);
+  const uint32_t bound = wave_bound<16>(at(0) < V ? ordered(most) : 0u, a.K);
+  const float wm = all_max(most);
   float s = 0.f;
-  if (wm > NEG) {
+  if (wm > NEG && wm < 1e37f) {
+    // exp2(x scale - c), c = wm scale rounded: one fma; what the rounding of c adds to every term
+    // comes off the sum, r = wm scale - c exactly
+    const float c = wm * a.exp_scale, r = fmaf(wm, a.exp_scale, -c);
 #pragma unroll
-    for (int e = 0; e < CH_E; ++e) s += __builtin_amdgcn_exp2f((x[e] - wm) * a.exp_scale);
+    for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f(fmaf(x[e], a.exp_scale, -c));
+    s = all_sum(s) * (1.f - 0.6931471806f * r);
+  } else if (wm > NEG) {                   // (the product could overflow)
+#pragma unroll
+    for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((x[e] - wm) * a.exp_scale);
+    s = all_sum(s);
   }
-  s = wave_sum(s);
   if (lane == 0) {
     sh_bound[wave] = bound;
     sh_m[wave] = wm;
@@ -124,16 +162,16 @@ __global__ void __launch_bounds__(256) beam_chunk_kernel(BeamSelect a) {
   const int64_t slot = row * a.chunks + chunk;
   if (tid == 0) {
     const float m = fmaxf(fmaxf(sh_m[0], sh_m[1]), fmaxf(sh_m[2], sh_m[3]));
-    double t = 0;
+    float t = 0.f;
     for (int w = 0; w < 4; ++w)
-      if (sh_m[w] > NEG) t += (double)sh_s[w] * exp2((double)(sh_m[w] - m) * (double)a.exp_scale);
+      if (sh_m[w] > NEG) t += sh_s[w] * __builtin_amdgcn_exp2f((sh_m[w] - m) * a.exp_scale);
     a.stats[slot * 2] = m;
-    a.stats[slot * 2 + 1] = (float)t;
+    a.stats[slot * 2 + 1] = t;
   }
-  const uint32_t least = max(max(sh_bound[0], sh_bound[1]), max(sh_bound[2], sh_bound[3]));
+  const float least = unordered(max(max(sh_bound[0], sh_bound[1]), max(sh_bound[2], sh_bound[3])));
 #pragma unroll
-  for (int e = 0; e < CH_E; ++e) {
-    const bool in = at(e) < V && ordered(x[e]) >= least;
+  for (int e = 0; e < E; ++e) {
+    const bool in = x[e] >= least && (whole || at(e) < V);
     const uint64_t on = __ballot(in);
     if (on) {
       uint32_t start = 0;
@@ -141,10 +179,8 @@ __global__ void __launch_bounds__(256) beam_chunk_kernel(BeamSelect a) {
       start = __builtin_amdgcn_readfirstlane(start);
       const uint32_t pos = start + __builtin_amdgcn_mbcnt_hi((uint32_t)(on >> 32),
                                                              __builtin_amdgcn_mbcnt_lo((uint32_t)on, 0));
-      if (in && pos < CAP) {
-        lx[pos] = x[e];
-        li[pos] = at(e);
-      }
+      if (in && pos < CAP)                 // (x + 0: -0 and +0 are one value)
+        list[pos] = ((uint64_t)ordered(x[e] + 0.0f) << 32) | (uint32_t)~at(e);
     }
   }
   __syncthreads();
@@ -153,26 +189,29 @@ __global__ void __launch_bounds__(256) beam_chunk_kernel(BeamSelect a) {
   int32_t *oi = a.cand_i + slot * a.K;
   if (n <= CAP) {
     for (uint32_t c = tid; c < n; c += 256) {
-      const float mx = lx[c];
-      const uint32_t mi = li[c];
+      const uint64_t key = list[c];
       int rank = 0;
-      for (uint32_t o = 0; o < n; ++o) rank += better(lx[o], li[o], mx, mi);
+#pragma unroll 4
+      for (uint32_t o = 0; o < n; ++o) rank += list[o] > key;
       if (rank < a.K) {
-        ox[rank] = mx;
-        oi[rank] = (int32_t)mi;
+        ox[rank] = unordered((uint32_t)(key >> 32));
+        oi[rank] = (int32_t)~(uint32_t)key;
       }
     }
     for (int r = (int)n + tid; r < a.K; r += 256) oi[r] = -1;
     return;
   }
   // ties overfill the list: K times the best of what is left, over the whole workgroup
+  __syncthreads();
   float tx = __builtin_inff();
   uint32_t ti = 0;
+  float *lx = (float *)list;
+  uint32_t *li = (uint32_t *)list + 4;
   for (int r = 0; r < a.K; ++r) {
     float bx = NEG;
     uint32_t bi = 0xffffffffu;
 #pragma unroll
-    for (int e = 0; e < CH_E; ++e) {
+    for (int e = 0; e < E; ++e) {
       const uint32_t i = at(e);
       const bool left = i < V && (r == 0 || better(tx, ti, x[e], i));
       if (left && better(x[e], i, bx, bi)) { bx = x[e]; bi = i; }
@@ -211,20 +250,22 @@ __global__ void __launch_bounds__(256) beam_merge_kernel(BeamSelect a) {
   __shared__ uint32_t sh_n, sh_bound[4];
   __shared__ double bx4[4];
   __shared__ int64_t bi4[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t item = blockIdx.x;
   const int K = a.K;
+  const uint8_t *fin = a.finished ? a.finished + item * K : nullptr;
+  const float *prevs = a.scores + item * K;
   if (tid == 0) sh_n = 0;
   // ---- logsumexp of each beam from its chunks ----
   for (int k = wave; k < K; k += 4) {
-    const int64_t row = item * K + k;
     double out = 0;
     float m = 0.f;
-    if (a.normalize && !(a.finished && a.finished[row])) {
-      const float *st = a.stats + row * a.chunks * 2;
+    if (a.normalize && !(fin && fin[k])) {
+      const float *st = a.stats + (item * K + k) * a.chunks * 2;
       m = NEG;
       for (uint32_t c = lane; c < a.chunks; c += 64) m = fmaxf(m, st[2 * c]);
-      m = wave_max(m);
+      m = all_max(m);
       double t = 0;
       for (uint32_t c = lane; c < a.chunks; c += 64)
         if (st[2 * c] > NEG)
@@ -246,58 +287,63 @@ __global__ void __launch_bounds__(256) beam_merge_kernel(BeamSelect a) {
     lp_prev = pow((a.length_base + s - 1.0) / (a.length_base + 1.0), a.alpha);
     lp_new = pow((a.length_base + s) / (a.length_base + 1.0), a.alpha);
   }
-  const int64_t per = (int64_t)a.chunks * K, n = K * per + K;
-  const int64_t none = 0x7fffffffffffffffLL;
-  // candidate c -> score and index (index `none`: there is no such candidate)
-  auto get = [&](int64_t c, double &x, int64_t &i) {
+  const double per_lp = 1.0 / lp_new;
+  const int64_t none = 0x7fffffffffffffffLL, KV = (int64_t)K * a.V;
+  // candidate j of list c (c = beam * chunks + chunk; from K chunks on: finished beams, of one
+  // candidate) -> score and index (index `none`: there is no such candidate)
+  const uint32_t lists = K * a.chunks + K;
+  auto get = [&](uint32_t c, int j, double &x, int64_t &i) {
     x = -__builtin_inf();
     i = none;
-    const int k = (int)(c < K * per ? (uint32_t)c / (uint32_t)per : c - K * per);
-    const int64_t row = item * K + k;
-    const bool fin = a.finished && a.finished[row];
-    const float prev = a.scores[row];
+    const bool self = c >= K * a.chunks;
+    const uint32_t k = self ? c - K * a.chunks : c / a.chunks;
+    const bool done = fin && fin[k];
+    const float prev = prevs[k];
     const bool dead = !(prev > -1e15f);
-    if (c >= K * per) {
-      if (fin) {
-        i = (int64_t)K * a.V + k;
+    if (self) {
+      if (done && j == 0) {
+        i = KV + k;
         if (!dead) x = (double)prev;
       }
-    } else if (!fin) {
-      const int32_t v = a.cand_i[row * per + (c - k * per)];
+    } else if (!done) {
+      const int64_t at = (item * K * a.chunks + c) * K + j;
+      const int32_t v = a.cand_i[at];
       if (v >= 0) {
         i = (int64_t)k * a.V + v;
-        const float z = a.cand_x[row * per + (c - k * per)];
+        const float z = a.cand_x[at];
         if (z > NEG && !dead)
           x = ((double)prev * lp_prev +
-               (((double)z - (double)peak[k]) * a.inv_temperature - lse[k])) / lp_new;
+               (((double)z - (double)peak[k]) * a.inv_temperature - lse[k])) * per_lp;
       }
     }
   };
+  // ---- a bound that K lists' best candidates reach ----
   double mx = -__builtin_inf();
-  int64_t mi = none;
-  for (int64_t c = tid; c < n; c += 256) {
+  bool any = false;
+  for (uint32_t c = tid; c < lists; c += 256) {
     double x;
     int64_t i;
-    get(c, x, i);
-    if (better(x, i, mx, mi)) { mx = x; mi = i; }
+    get(c, 0, x, i);
+    any |= i != none;
+    mx = fmax(mx, x);
   }
-  const uint32_t bound = wave_bound(mi != none ? (uint32_t)(ordered(mx) >> 32) : 0u, K);
+  const uint32_t bound = wave_bound<8>(any ? (uint32_t)(ordered(mx) >> 32) : 0u, K);
   if (lane == 0) sh_bound[wave] = bound;
   __syncthreads();
   const uint32_t least = max(max(sh_bound[0], sh_bound[1]), max(sh_bound[2], sh_bound[3]));
-  for (int64_t c = tid; c < n; c += 256) {
-    double x;
-    int64_t i;
-    get(c, x, i);
-    if (i != none && (uint32_t)(ordered(x) >> 32) >= least) {
+  for (uint32_t c = tid; c < lists; c += 256)
+    for (int j = 0; j < K; ++j) {                // (best first)
+      double x;
+      int64_t i;
+      get(c, j, x, i);
+      if (i == none || (uint32_t)(ordered(x) >> 32) < least) break;
       const uint32_t pos = atomicAdd(&sh_n, 1u);
       if (pos < LIST) { sx[pos] = x; si[pos] = i; }
     }
-  }
   __syncthreads();
   const uint32_t found = sh_n;
   auto put = [&](int rank, double x, int64_t i) {
-    const int64_t to = item * K + rank, KV = (int64_t)K * a.V;
+    const int64_t to = item * K + rank;
     const bool was = i >= KV;
     const int64_t k = was ? i - KV : i / a.V, v = was ? -1 : i - k * a.V;
     a.out_scores[to] = (float)x;
@@ -320,12 +366,14 @@ __global__ void __launch_bounds__(256) beam_merge_kernel(BeamSelect a) {
   for (int r = 0; r < K; ++r) {
     double bx = -__builtin_inf();
     int64_t bi = none;
-    for (int64_t c = tid; c < n; c += 256) {
-      double x;
-      int64_t i;
-      get(c, x, i);
-      if (i != none && (r == 0 || better(tx, ti, x, i)) && better(x, i, bx, bi)) { bx = x; bi = i; }
-    }
+    for (uint32_t c = tid; c < lists; c += 256)
+      for (int j = 0; j < K; ++j) {
+        double x;
+        int64_t i;
+        get(c, j, x, i);
+        if (i == none) break;
+        if ((r == 0 || better(tx, ti, x, i)) && better(x, i, bx, bi)) { bx = x; bi = i; }
+      }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
       const double yx = __shfl_xor(bx, o, 64);
@@ -447,27 +495,40 @@ __global__ void __launch_bounds__(256) reorder_kernel(Reorder a) {
 
 }  // namespace
 
+// Values of a thread: 32 where that still gives every CU a few workgroups, 16 otherwise
+// (256 rows of 32128 float32 logits: MEASURED; 4 rows: MEASURED).
+static int chunk_values(int64_t rows, int64_t V) {
+  return rows * ((V + 8191) / 8192) >= 1024 ? 32 : 16;
+}
+
 size_t beam_workspace_bytes(int64_t rows, int64_t V, int K) {
-  const int64_t slots = rows * ((V + CH - 1) / CH);
+  const int64_t ch = 256 * chunk_values(rows, V), slots = rows * ((V + ch - 1) / ch);
   return (size_t)slots * (8 + 8 * (size_t)K);
 }
 
 void launch_beam_select(BeamSelect a, int64_t items, int dtype, void *ws, hipStream_t s) {
   const int64_t rows = items * a.K;
-  a.chunks = (uint32_t)((a.V + CH - 1) / CH);
+  const int values = chunk_values(rows, a.V);
+  a.chunks = (uint32_t)((a.V + 256 * values - 1) / (256 * values));
   a.stats = (float *)ws;
   a.cand_x = a.stats + rows * a.chunks * 2;
   a.cand_i = (int32_t *)(a.cand_x + rows * a.chunks * a.K);
   const int per = dtype == GNLP_BF16 ? 8 : 4;
   const bool vec = ((uintptr_t)a.outputs & 15) == 0 && a.row_stride % per == 0 && a.V % per == 0;
   const dim3 grid(a.chunks, (unsigned)rows), block(256);
+#define GO(T, E) \
+  do { \
+    if (vec) hipLaunchKernelGGL((beam_chunk_kernel<T, true, E>), grid, block, 0, s, a); \
+    else hipLaunchKernelGGL((beam_chunk_kernel<T, false, E>), grid, block, 0, s, a); \
+  } while (0)
   if (dtype == GNLP_BF16) {
-    if (vec) hipLaunchKernelGGL((beam_chunk_kernel<bf16, true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((beam_chunk_kernel<bf16, false>), grid, block, 0, s, a);
+    if (values == 32) GO(bf16, 32);
+    else GO(bf16, 16);
   } else {
-    if (vec) hipLaunchKernelGGL((beam_chunk_kernel<float, true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((beam_chunk_kernel<float, false>), grid, block, 0, s, a);
+    if (values == 32) GO(float, 32);
+    else GO(float, 16);
   }
+#undef GO
   hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)items), block, 0, s, a);
 }
 

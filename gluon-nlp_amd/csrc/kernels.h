@@ -319,6 +319,7 @@ struct Kv4Attn {
   int64_t B, H, S, d;
   int64_t Lq; int share;              // queries; query heads per cached head
   const void *q; int64_t q_stride[3]; // (b, query head, t)
+  int q_vec;                          // 8 channels of q can be loaded as 16-byte vectors
   void *out; int64_t o_stride[3];
   const void *length; int length_dtype;
   const void *q_length; int q_length_dtype;

@@ -13,22 +13,28 @@
 // Roundings: bf16 queries are exact operands, float32 ones are split into three bf16 parts; p s_v
 // is split into two (bf16 tensors: 16 bits) or three parts (float32: all 24 bits).  What the parts
 // lose multiplies n - 7.5, not n: the rest of p s_v goes into the per-row sum with 7.5.  For float32
-// the 23.5 = 16 + 7.5 is also taken off inside the matrix product, 32 tokens at a time (a product
-// with a constant operand starts the accumulators): sums over a long context would otherwise grow
-// to 23.5 sum(p s_v) and lose the digits of a result that averages out.
+// the 23.5 = 16 + 7.5 is also taken off inside the matrix products (a product with a constant
+// operand starts the accumulators, every 32 channels or tokens): sums over a long context would
+// otherwise grow to 23.5 sum(p s_v) and lose the digits of a result that averages out.
 //
 // Work: a wave takes tiles of TT = 128 (head dim 64) or 64 tokens, 8 KB of codes, on its own, with
 // its own running maximum; four waves of a workgroup and, for few heads, several workgroups
 // (`splits`, joined by kv4_join_kernel) share a sequence.
 //   S^T = K Q^T: operand A = 16 cached tokens as they lie in memory, operand B = 16 query rows.
 //   O^T = V^T P^T: operand A = 16 channels x 32 tokens, again as they lie in memory.
-// With fewer than 16 query rows (one, in plain decoding) most columns of S^T are idle; the scores
-// therefore go through LDS, where the wave spreads the R rows that exist over its 64 lanes: the
-// softmax costs R tokens x 128 / 64 instead of 32 evaluations a lane.  R = 1, 2, 4, 8, 16.
+// The rows of K are taken in an order in which a lane's part of S^T is its part of operand B of the
+// second product, so that with 5 to 16 query rows (R = 16) the softmax runs where the scores are.
+// With fewer rows (one, in plain decoding) most columns of S^T are idle; the scores then go through
+// LDS, where the wave spreads the R = 1, 2 or 4 rows over its 64 lanes: the softmax costs 2 R
+// evaluations a lane and 128 tokens instead of 32.
 // The running maximum moves only when a score exceeds it by 8 (exp(8) is harmless in float32):
 // noticing that is one vote, the reduction over lanes is the exception.
+// The next tile's K codes are requested when this one's scores are done, its V codes when this
+// one's products are: a code is dequantised out of the register that it was loaded into.
 //
 // Bound by memory: 72 bytes a token and cached head at head dim 64 (256 in bf16).
+#include <type_traits>
+
 #include "common.h"
 #include "kernels.h"
 
@@ -64,26 +70,51 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
+// base: the same in all lanes
+template <typename V>
+__device__ __forceinline__ V load_at(const void *base, uint32_t off) {
+  return *reinterpret_cast<const V *>((const char *)base + off);
+}
+
+// x = sum of its PS bf16 parts (the last one rounded), returns that sum
+template <int PS>
+__device__ __forceinline__ float split(float x, bf16 (&part)[PS]) {
+  float rest = x, sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < PS; ++k) {
+    part[k] = (bf16)rest;
+    sum += (float)part[k];
+    rest -= (float)part[k];
+  }
+  return sum;
+}
+
 template <typename T, int DP, int R>
 __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a) {
   constexpr int G = DP / 64;             // groups of a token
   constexpr int TT = 128 / G;            // tokens of a tile
   constexpr int NSUB = TT / 32;
+  constexpr bool DIRECT = R == 16;       // softmax in the layout of the scores
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int QS = F32 ? 3 : 1;        // bf16 parts of a query value
   constexpr int PS = F32 ? 3 : 2;        // bf16 parts of p s_v
-  constexpr int LPR = 64 / R;            // lanes of a row in the softmax
-  constexpr int TPL = TT / LPR;          // tokens of a lane there (R == 1, TT == 64: one)
+  constexpr int LPR = DIRECT ? 4 : 64 / R;        // lanes of a row in the softmax
+  constexpr int TPL = TT / LPR;          // tokens of a lane there
   constexpr int VW = TPL < 4 ? TPL : 4;  // ... in vectors of
   constexpr int NV = TPL / VW;
+  constexpr int NP = TT / 64;            // tokens whose parameters a lane fetches
+  constexpr bool OWN_PAR = R == 1;       // ... which are the ones that it evaluates
   constexpr int SROW = TT + 4, PROW = TT + 8;
   constexpr float NEG = -__builtin_inff();
   constexpr float STEP = 8.0f, LOG2E = 1.4426950408889634f;
+  constexpr float CENTER = F32 ? 23.5f : 16.f;    // taken off a code inside the first product
+  constexpr int KROW = DP / 2, VROW = DP * 4;     // bytes of a token's K, of 8 tokens' V
 
   // per wave: scores (G, R, SROW) float, P (G, PS, R, PROW) bf16, parameters (2, G, TT), alpha (R)
-  constexpr int S_BYTES = G * R * SROW * 4, P_BYTES = G * PS * R * PROW * 2;
-  constexpr int PAR_BYTES = R > 1 ? 2 * G * TT * 4 : 0;
-  constexpr int WAVE_BYTES = (S_BYTES + P_BYTES + PAR_BYTES + 16 * 4 + 15) / 16 * 16;
+  constexpr int S_BYTES = DIRECT ? 0 : G * R * SROW * 4;
+  constexpr int P_BYTES = DIRECT ? 0 : G * PS * R * PROW * 2;
+  constexpr int PAR_BYTES = OWN_PAR ? 0 : 2 * G * TT * 4;
+  constexpr int WAVE_BYTES = (S_BYTES + P_BYTES + PAR_BYTES + 2 * 16 * 4 + 15) / 16 * 16;
   constexpr int OUT_BYTES = 4 * R * (DP + 2 + G) * 4;
   __shared__ __attribute__((aligned(16)))
       unsigned char smem[4 * WAVE_BYTES > OUT_BYTES ? 4 * WAVE_BYTES : OUT_BYTES];
@@ -97,82 +128,190 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a) {
 
   // ---- which rows, which tokens ----
   uint32_t lin = blockIdx.x;
-  const uint32_t rt = lin % a.row_tiles;
-  lin /= a.row_tiles;
-  const uint32_t split = lin % a.splits;
-  lin /= a.splits;
-  const uint32_t h = lin % (uint32_t)a.H;
-  const int64_t b = lin / (uint32_t)a.H;
-  const int rows = (int)(a.Lq * a.share) - (int)rt * 16;   // of this tile: row = query * share + r
-  int64_t len = load_len(a.length, a.length_dtype, b);
-  len = len < 0 ? 0 : (len > a.S ? a.S : len);
-  int64_t ql = a.q_length ? load_len(a.q_length, a.q_length_dtype, b) : a.Lq;
-  ql = ql < 0 ? 0 : (ql > a.Lq ? a.Lq : ql);
-  auto seen = [&](int64_t i) -> int {                      // keys that query i sees
-    int64_t n = a.causal ? len - ql + i + 1 : len;
-    n = n > a.Lm ? a.Lm : n;
-    return i < ql && n > 0 ? (int)n : 0;
-  };
+  const uint32_t rt = a.row_tiles == 1 ? 0 : lin % (uint32_t)a.row_tiles;
+  if (a.row_tiles > 1) lin /= (uint32_t)a.row_tiles;
+  const uint32_t split_no = a.splits == 1 ? 0 : lin % (uint32_t)a.splits;
+  if (a.splits > 1) lin /= (uint32_t)a.splits;
+  const int b = (int)(lin / (uint32_t)a.H), h = (int)(lin - (uint32_t)b * (uint32_t)a.H);
+  const int Lq = (int)a.Lq, S = (int)a.S, row0 = (int)rt * 16;
+  const int rows = Lq * a.share - row0;                    // of this tile: row = query * share + r
   const int tile_rows = rows < 16 ? rows : 16;
-  int64_t last = ((int64_t)rt * 16 + tile_rows - 1) / a.share;   // the row that sees most
+  int64_t len64 = load_len(a.length, a.length_dtype, b);
+  const int len = len64 < 0 ? 0 : (len64 > S ? S : (int)len64);
+  int64_t ql64 = a.q_length ? load_len(a.q_length, a.q_length_dtype, b) : Lq;
+  const int ql = ql64 < 0 ? 0 : (ql64 > Lq ? Lq : (int)ql64);
+  const int reach = a.Lm < S ? (int)a.Lm : S;
+  auto seen = [&](int i) -> int {                          // keys that query i sees
+    int n = a.causal ? len - ql + i + 1 : len;
+    n = n > reach ? reach : n;
+    return i < ql && n > 0 ? n : 0;
+  };
+  int last = (int)((uint32_t)(row0 + tile_rows - 1) / (uint32_t)a.share);   // sees most
   last = last >= ql ? ql - 1 : last;
-  const int top = last * a.share + a.share > (int64_t)rt * 16 && last >= 0 ? seen(last) : 0;
-  const int ntiles = (top + TT - 1) / TT, per = (ntiles + a.splits - 1) / a.splits;
-  const int t_begin = split * per, t_end = t_begin + per < ntiles ? t_begin + per : ntiles;
+  const int top = last >= 0 && (last + 1) * a.share > row0 ? seen(last) : 0;
+  const int ntiles = (top + TT - 1) / TT;
+  int t_begin = 0, t_end = ntiles;
+  if (a.splits > 1) {
+    const int per = (int)((uint32_t)(ntiles + a.splits - 1) / (uint32_t)a.splits);
+    t_begin = (int)split_no * per;
+    t_end = t_begin + per < ntiles ? t_begin + per : ntiles;
+  }
   const int sub_last = top > 0 ? (top - 1) / 32 : 0;       // last 32 tokens that are read
 
-  const int64_t head = b * a.H + h;
-  const uint32_t *kc = (const uint32_t *)a.k_codes + head * a.S * (DP / 8);
-  const uint32_t *vc = (const uint32_t *)a.v_codes + head * a.S * (DP / 8);
+  const int64_t head = (int64_t)b * a.H + h;
+  const char *kc = (const char *)a.k_codes + head * a.S * KROW;
+  const char *vc = (const char *)a.v_codes + head * a.S * KROW;
   const uint32_t *kp = (const uint32_t *)a.k_par + head * G * a.S;
   const uint32_t *vp = (const uint32_t *)a.v_par + head * G * a.S;
 
+  u32x2 kw[NSUB][2][G];
+  u32x4 vw[NSUB][G];
+  uint32_t kpw[G][NP], vpw[G][NP];
+  const uint32_t k_off = (8 * (col >> 2) + (col & 3)) * KROW + 8 * g;
+  const uint32_t v_off = g * VROW + 16 * col;
+  auto fetch_k = [&](int t) {
+#pragma unroll
+    for (int s = 0; s < NSUB; ++s) {
+      int sub = t * NSUB + s;
+      sub = sub < sub_last ? sub : sub_last;               // (past the end: the last ones again)
+      const char *base = kc + (int64_t)sub * 32 * KROW;
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+        for (int grp = 0; grp < G; ++grp)
+          kw[s][blk][grp] = load_at<u32x2>(base + blk * 4 * KROW + grp * 32, k_off);
+    }
+    const uint32_t tok = (uint32_t)t * TT + NP * lane, most = S - NP;
+    const uint32_t off = (tok < most ? tok : most) * 4;
+#pragma unroll
+    for (int grp = 0; grp < G; ++grp)
+#pragma unroll
+      for (int e = 0; e < NP; ++e) {
+        kpw[grp][e] = load_at<uint32_t>(kp + grp * a.S + e, off);
+        vpw[grp][e] = load_at<uint32_t>(vp + grp * a.S + e, off);
+      }
+  };
+  auto fetch_v = [&](int t) {
+#pragma unroll
+    for (int s = 0; s < NSUB; ++s) {
+      int sub = t * NSUB + s;
+      sub = sub < sub_last ? sub : sub_last;
+      const char *base = vc + (int64_t)sub * 4 * VROW;
+#pragma unroll
+      for (int grp = 0; grp < G; ++grp) vw[s][grp] = load_at<u32x4>(base + grp * 256, v_off);
+    }
+  };
+  int t = t_begin + wave;
+  if (t < t_end) {
+    fetch_k(t);
+    fetch_v(t);
+  }
+
   // ---- queries: operand B of K Q^T, channel 64 grp + 16 g + 8 s + j of row col ----
   bf16x8 qf[G][2][QS];
+  f32x4 start[G][F32 ? 2 : 1];           // what the accumulators start with: -CENTER sum(q)
+  float qsum[G];
   {
-    float qsum[G];
-    const int rr = (int)rt * 16 + col;
-    const int64_t i = rr / a.share, hq = (int64_t)h * a.share + rr % a.share;
+    const int qr = row0 + col, i = (int)((uint32_t)qr / (uint32_t)a.share);
+    const int64_t hq = (int64_t)h * a.share + (qr - i * a.share);
     const T *qp = (const T *)a.q + b * a.q_stride[0] + hq * a.q_stride[1] + i * a.q_stride[2];
+    const bool live = col < tile_rows;
 #pragma unroll
     for (int grp = 0; grp < G; ++grp) {
       qsum[grp] = 0.f;
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < 2; ++s) {
+        const int c0 = 64 * grp + 16 * g + 8 * s;
+        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (a.q_vec) {
+          if (live && c0 < a.d) {
+            if (F32) {
+              const f32x4 lo = *reinterpret_cast<const f32x4 *>(qp + c0);
+              const f32x4 hi = *reinterpret_cast<const f32x4 *>(qp + c0 + 4);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) { x[j] = lo[j]; x[4 + j] = hi[j]; }
+            } else {
+              const bf16x8 w = *reinterpret_cast<const bf16x8 *>(qp + c0);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) x[j] = (float)w[j];
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (live && c0 + j < a.d) x[j] = to_f32(qp[c0 + j]);
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int c = 64 * grp + 16 * g + 8 * s + j;
-          float x = 0.f;
-          if (col < tile_rows && c < a.d) x = to_f32(qp[c]);
-          qsum[grp] += x;
+          qsum[grp] += x[j];
+          bf16 part[QS];
+          split<QS>(x[j], part);
 #pragma unroll
-          for (int k = 0; k < QS; ++k) {
-            const bf16 part = (bf16)x;
-            qf[grp][s][k][j] = part;
-            x -= (float)part;
-          }
+          for (int k = 0; k < QS; ++k) qf[grp][s][k][j] = part[k];
         }
+      }
       qsum[grp] += __shfl_xor(qsum[grp], 16, 64);
       qsum[grp] += __shfl_xor(qsum[grp], 32, 64);
-      if (lane < R) sc[grp * 16 + lane] = qsum[grp];
+      if (!DIRECT && lane < R) sc[grp * 16 + lane] = qsum[grp];
     }
   }
-  wave_lds_sync();
-  const int row = lane / LPR, sl = lane % LPR;             // the lane's row in the softmax
-  float qs[G];
+  const bf16 cen = (bf16)(-23.5f);
+  const bf16x8 center = {cen, cen, cen, cen, cen, cen, cen, cen};
 #pragma unroll
-  for (int grp = 0; grp < G; ++grp) qs[grp] = sc[grp * 16 + row];
-  wave_lds_sync();
-  const int rr = (int)rt * 16 + row;
-  const int64_t qi = rr / a.share, hq = (int64_t)h * a.share + rr % a.share;
+  for (int grp = 0; grp < G; ++grp) {
+    if (F32) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        start[grp][s] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < QS; ++k) start[grp][s] = mfma16(center, qf[grp][s][k], start[grp][s]);
+      }
+    } else {
+      const float q0 = -CENTER * qsum[grp];
+      start[grp][0] = (f32x4){q0, q0, q0, q0};
+    }
+  }
+  int row = col;                                           // the lane's row in the softmax
+  const int sl = DIRECT ? g : lane % LPR;
+  if (!DIRECT) {
+    wave_lds_sync();
+    row = lane / LPR;
+#pragma unroll
+    for (int grp = 0; grp < G; ++grp) qsum[grp] = sc[grp * 16 + row];
+    wave_lds_sync();
+  }
+  const int qi = (int)((uint32_t)(row0 + row) / (uint32_t)a.share);
+  const int64_t hq = (int64_t)h * a.share + (row0 + row - qi * a.share);
   const int vis = row < tile_rows ? seen(qi) : 0;
-  const int pos = (int)(len - ql + qi);
+  const int pos = len - ql + qi;
   const T *edge = nullptr;
   if (a.edge)
     edge = (const T *)a.edge + b * a.edge_stride[0] + hq * a.edge_stride[1] +
            qi * a.edge_stride[2];
   const T *table = a.table ? (const T *)a.table + hq * a.table_len : nullptr;
   const uint8_t *mask = a.mask ? a.mask + b * a.mask_stride[0] + qi * a.mask_stride[1] : nullptr;
+
+  // a score from the product without CENTER, for the token of parameters w
+  auto scaled = [&](float dot, uint32_t w, int grp) -> float {
+    const float s = scale_of(w);
+    const float c = F32 ? fmaf(7.5f, s, min_of(w)) : min_of(w);
+    return fmaf(s, dot, c * qsum[grp]);
+  };
+  auto finish = [&](float z, int j) -> float {             // bias, scale, mask of key j
+    bool on = j < vis;
+    if (edge || table || mask) {
+      if (on) {
+        if (edge) z += to_f32(edge[(int64_t)j * a.edge_stride[3]]);
+        if (table) {
+          int64_t at = a.table_len - 1 - (int64_t)(pos - j);
+          at = at < 0 ? 0 : (at >= a.table_len ? a.table_len - 1 : at);
+          z += to_f32(table[at]);
+        }
+        if (mask) on = mask[(int64_t)j * a.mask_stride[2]] != 0;
+      }
+    }
+    return on ? z * a.inv_temperature : NEG;
+  };
 
   // ---- running state ----
   float ref = NEG, l = 0.f, csum[G];
@@ -183,212 +322,215 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[grp][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
-  const bf16 cen = (bf16)(-23.5f);
-  const bf16x8 center = {cen, cen, cen, cen, cen, cen, cen, cen};
-
-  u32x2 kw[NSUB][2][G];
-  u32x4 vw[NSUB][G];
-  constexpr int NP = TT / 64;                              // tokens whose parameters a lane fetches
-  uint32_t kpw[G][NP], vpw[G][NP];
-  auto fetch = [&](int t) {
+  auto rebase = [&](float most) {                          // a larger maximum for the lane's row
 #pragma unroll
-    for (int s = 0; s < NSUB; ++s) {
-      int sub = t * NSUB + s;
-      sub = sub < sub_last ? sub : sub_last;               // (past the end: the last ones again)
-      const int64_t tok = (int64_t)sub * 32;
+    for (int o = DIRECT ? 32 : LPR / 2; o > (DIRECT ? 8 : 0); o >>= 1)
+      most = fmaxf(most, __shfl_xor(most, o, 64));
+    const float to = fmaxf(ref, most);
+    const float alpha = ref == to ? 1.f : __builtin_amdgcn_exp2f((ref - to) * LOG2E);
+    ref = to;
+    l *= alpha;
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-        for (int grp = 0; grp < G; ++grp)
-          kw[s][blk][grp] = *reinterpret_cast<const u32x2 *>(
-              kc + (tok + 8 * (col >> 2) + 4 * blk + (col & 3)) * (DP / 8) + grp * 8 + 2 * g);
-#pragma unroll
-      for (int grp = 0; grp < G; ++grp)
-        vw[s][grp] = *reinterpret_cast<const u32x4 *>(vc + (tok / 8 + g) * DP + grp * 64 + 4 * col);
+    for (int grp = 0; grp < G; ++grp) csum[grp] *= alpha;
+    float ac = alpha;
+    if (!DIRECT) {
+      if (sl == 0) al[row] = alpha;
+      wave_lds_sync();
+      ac = al[col < R ? col : R - 1];
     }
-    int64_t tok = (int64_t)t * TT + NP * lane;
-    const int64_t most = (int64_t)sub_last * 32 + 32 - NP;
-    tok = tok < most ? tok : most;
+#pragma unroll
+    for (int grp = 0; grp < G; ++grp)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[grp][i][e] *= ac;
+  };
+  // weight p of a token with V parameters w: parts of p s_v, its share of the per-row sum
+  auto weigh = [&](float p, bool off, uint32_t w, int grp, bf16 (&part)[PS]) {
+    const float pv = off ? 0.f : p * scale_of(w);
+    const float sum = split<PS>(pv, part);
+    // F32: the 23.5 comes off inside the product
+    csum[grp] += (off ? 0.f : p * min_of(w)) + fmaf(7.5f, pv, F32 ? 0.f : -23.5f * sum);
+  };
+  // O^T += V^T P^T of 32 tokens: channel 64 grp + 4 row + i of operand A's row
+  auto products = [&](int s, int grp, const bf16x8 (&pb)[PS]) {
+    if (F32) {
+      f32x4 from = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < PS; ++k) from = mfma16(center, pb[k], from);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bf16x8 v8 = codes16(vw[s][grp][i]);
+        f32x4 o = from;
+#pragma unroll
+        for (int k = 0; k < PS; ++k) o = mfma16(v8, pb[k], o);
+        acc[grp][i] += o;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bf16x8 v8 = codes16(vw[s][grp][i]);
+#pragma unroll
+        for (int k = 0; k < PS; ++k) acc[grp][i] = mfma16(v8, pb[k], acc[grp][i]);
+      }
+    }
+  };
+
+  auto tile = [&](int t, auto more) {
+    constexpr bool MORE = decltype(more)::value;           // another tile follows
+    float x[TPL];
+    uint32_t vpr[G][OWN_PAR ? TPL : 1], kpr[G][OWN_PAR ? TPL : 1];
 #pragma unroll
     for (int grp = 0; grp < G; ++grp)
 #pragma unroll
       for (int e = 0; e < NP; ++e) {
-        kpw[grp][e] = kp[grp * a.S + tok + e];
-        vpw[grp][e] = vp[grp * a.S + tok + e];
-      }
-  };
-
-  int t = t_begin + wave;
-  if (t < t_end) fetch(t);
-  for (; t < t_end; t += 4) {
-    // ---- scores of the tile: S^T = K Q^T, rows of 32 tokens as V wants them ----
-#pragma unroll
-    for (int s = 0; s < NSUB; ++s)
-#pragma unroll
-      for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-        for (int grp = 0; grp < G; ++grp) {
-          f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int st = 0; st < 2; ++st) {
-            const bf16x8 k8 = codes16(kw[s][blk][grp][st]);
-#pragma unroll
-            for (int k = 0; k < QS; ++k) x = mfma16(k8, qf[grp][st][k], x);
-          }
-          if (col < R)
-            *reinterpret_cast<f32x4 *>(sc + (grp * R + col) * SROW + s * 32 + 8 * g + 4 * blk) = x;
-        }
-    uint32_t kpr[G][TPL], vpr[G][TPL];
-    if (R > 1) {
-#pragma unroll
-      for (int grp = 0; grp < G; ++grp)
-#pragma unroll
-        for (int e = 0; e < NP; ++e) {
+        if (OWN_PAR) {
+          kpr[grp][e] = kpw[grp][e];
+          vpr[grp][e] = vpw[grp][e];
+        } else {
           parl[grp * TT + NP * lane + e] = kpw[grp][e];
           parl[(G + grp) * TT + NP * lane + e] = vpw[grp][e];
         }
-    }
-    u32x4 vnow[NSUB][G];
+      }
+    if (DIRECT) wave_lds_sync();
+    // ---- scores: S^T = K Q^T, rows of 32 tokens as V wants them ----
 #pragma unroll
     for (int s = 0; s < NSUB; ++s)
 #pragma unroll
-      for (int grp = 0; grp < G; ++grp) vnow[s][grp] = vw[s][grp];
-    if (R == 1) {
+      for (int blk = 0; blk < 2; ++blk) {
+        if (DIRECT)
 #pragma unroll
-      for (int grp = 0; grp < G; ++grp)
-#pragma unroll
-        for (int e = 0; e < TPL; ++e) {
-          kpr[grp][e] = kpw[grp][e < NP ? e : 0];
-          vpr[grp][e] = vpw[grp][e < NP ? e : 0];
-        }
-    }
-    if (t + 4 < t_end) fetch(t + 4);
-    wave_lds_sync();
-
-    // ---- softmax: lane (row, sl), tokens v LPR VW + sl VW + e of the tile ----
-    float x[TPL];
-    float most = NEG;
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-      for (int e = 0; e < VW; ++e) {
-        const int n = v * VW + e, tok = v * LPR * VW + sl * VW + e, j = t * TT + tok;
-        float z = 0.f;
+          for (int e = 0; e < 4; ++e) x[(s * 2 + blk) * 4 + e] = 0.f;
 #pragma unroll
         for (int grp = 0; grp < G; ++grp) {
-          if (R > 1) {
-            kpr[grp][n] = parl[grp * TT + tok];
-            vpr[grp][n] = parl[(G + grp) * TT + tok];
+          f32x4 d = start[grp][0];
+          if (F32) {
+            f32x4 d2 = start[grp][F32 ? 1 : 0];
+            const bf16x8 k0 = codes16(kw[s][blk][grp][0]), k1 = codes16(kw[s][blk][grp][1]);
+#pragma unroll
+            for (int k = 0; k < QS; ++k) {
+              d = mfma16(k0, qf[grp][0][k], d);
+              d2 = mfma16(k1, qf[grp][1][k], d2);
+            }
+            d += d2;
+          } else {
+            d = mfma16(codes16(kw[s][blk][grp][0]), qf[grp][0][0], d);
+            d = mfma16(codes16(kw[s][blk][grp][1]), qf[grp][1][0], d);
           }
-          const float dot = fmaf(-16.f, qs[grp], sc[(grp * R + row) * SROW + tok]);
-          z += fmaf(scale_of(kpr[grp][n]), dot, min_of(kpr[grp][n]) * qs[grp]);
-        }
-        bool on = j < vis;
-        if (on) {
-          if (edge) z += to_f32(edge[(int64_t)j * a.edge_stride[3]]);
-          if (table) {
-            int64_t at = a.table_len - 1 - (pos - j);
-            at = at < 0 ? 0 : (at >= a.table_len ? a.table_len - 1 : at);
-            z += to_f32(table[at]);
+          if (DIRECT) {
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(parl + grp * TT + s * 32 + 8 * g +
+                                                             4 * blk);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[(s * 2 + blk) * 4 + e] += scaled(d[e], w[e], grp);
+          } else if (col < R) {
+            *reinterpret_cast<f32x4 *>(sc + (grp * R + col) * SROW + s * 32 + 8 * g + 4 * blk) = d;
           }
-          if (mask) on = mask[(int64_t)j * a.mask_stride[2]] != 0;
         }
-        x[n] = on ? z * a.inv_temperature : NEG;
+      }
+    if (MORE) fetch_k(t + 4);
+    float most = NEG;
+    if (DIRECT) {
+#pragma unroll
+      for (int n = 0; n < TPL; ++n) {
+        x[n] = finish(x[n], t * TT + (n >> 3) * 32 + 8 * g + (n & 7));
         most = fmaxf(most, x[n]);
       }
-    if (__any(most > ref + STEP || (ref == NEG && most > NEG))) {
-#pragma unroll
-      for (int o = LPR / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
-      const float to = fmaxf(ref, most);
-      const float alpha = ref == to ? 1.f : __builtin_amdgcn_exp2f((ref - to) * LOG2E);
-      ref = to;
-      l *= alpha;
-#pragma unroll
-      for (int grp = 0; grp < G; ++grp) csum[grp] *= alpha;
-      if (sl == 0) al[row] = alpha;
+    } else {
       wave_lds_sync();
-      const float ac = al[col < R ? col : R - 1];
 #pragma unroll
-      for (int grp = 0; grp < G; ++grp)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[grp][i][e] *= ac;
-    }
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      float p[VW];
-#pragma unroll
-      for (int e = 0; e < VW; ++e) {
-        const float z = x[v * VW + e];
-        p[e] = z == NEG ? 0.f : __builtin_amdgcn_exp2f((z - ref) * LOG2E);
-        l += p[e];
-      }
-#pragma unroll
-      for (int grp = 0; grp < G; ++grp) {
-        bf16 part[PS][VW];
+      for (int v = 0; v < NV; ++v)
 #pragma unroll
         for (int e = 0; e < VW; ++e) {
-          const uint32_t w = vpr[grp][v * VW + e];
-          const bool off = x[v * VW + e] == NEG;
-          const float pv = off ? 0.f : p[e] * scale_of(w);
-          float rest = pv, sum = 0.f;
+          const int n = v * VW + e, tok = v * LPR * VW + sl * VW + e;
+          float z = 0.f;
+#pragma unroll
+          for (int grp = 0; grp < G; ++grp)
+            z += scaled(sc[(grp * R + row) * SROW + tok],
+                        OWN_PAR ? kpr[grp][n] : parl[grp * TT + tok], grp);
+          x[n] = finish(z, t * TT + tok);
+          most = fmaxf(most, x[n]);
+        }
+    }
+    if (__any(most > ref + STEP || (ref == NEG && most > NEG))) rebase(most);
+    // ---- weights and the second product ----
+    if (DIRECT) {
+#pragma unroll
+      for (int s = 0; s < NSUB; ++s) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float z = x[s * 8 + e];
+          p[e] = z == NEG ? 0.f : __builtin_amdgcn_exp2f((z - ref) * LOG2E);
+          l += p[e];
+        }
+#pragma unroll
+        for (int grp = 0; grp < G; ++grp) {
+          bf16x8 pb[PS];
+#pragma unroll
+          for (int blk = 0; blk < 2; ++blk) {
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(parl + (G + grp) * TT + s * 32 +
+                                                             8 * g + 4 * blk);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              bf16 part[PS];
+              weigh(p[blk * 4 + e], x[s * 8 + blk * 4 + e] == NEG, w[e], grp, part);
+#pragma unroll
+              for (int k = 0; k < PS; ++k) pb[k][blk * 4 + e] = part[k];
+            }
+          }
+          products(s, grp, pb);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        float p[VW];
+#pragma unroll
+        for (int e = 0; e < VW; ++e) {
+          const float z = x[v * VW + e];
+          p[e] = z == NEG ? 0.f : __builtin_amdgcn_exp2f((z - ref) * LOG2E);
+          l += p[e];
+        }
+#pragma unroll
+        for (int grp = 0; grp < G; ++grp) {
+          const int tok = v * LPR * VW + sl * VW;
+          bf16 part[VW][PS];
+#pragma unroll
+          for (int e = 0; e < VW; ++e)
+            weigh(p[e], x[v * VW + e] == NEG,
+                  OWN_PAR ? vpr[grp][v * VW + e] : parl[(G + grp) * TT + tok + e], grp, part[e]);
 #pragma unroll
           for (int k = 0; k < PS; ++k) {
-            part[k][e] = (bf16)rest;
-            sum += (float)part[k][e];
-            rest -= (float)part[k][e];
+            bf16 *to = pr + ((grp * PS + k) * R + row) * PROW + tok;
+#pragma unroll
+            for (int e = 0; e < VW; ++e) to[e] = part[e][k];
           }
-          // F32: the 23.5 comes off inside the product
-          csum[grp] += (off ? 0.f : p[e] * min_of(w)) + fmaf(7.5f, pv, F32 ? 0.f : -23.5f * sum);
-        }
-#pragma unroll
-        for (int k = 0; k < PS; ++k) {
-          bf16 *to = pr + ((grp * PS + k) * R + row) * PROW + v * LPR * VW + sl * VW;
-#pragma unroll
-          for (int e = 0; e < VW; ++e) to[e] = part[k][e];
         }
       }
+      wave_lds_sync();
+#pragma unroll
+      for (int s = 0; s < NSUB; ++s)
+#pragma unroll
+        for (int grp = 0; grp < G; ++grp) {
+          bf16x8 pb[PS];
+#pragma unroll
+          for (int k = 0; k < PS; ++k)
+            pb[k] = *reinterpret_cast<const bf16x8 *>(
+                pr + ((grp * PS + k) * R + (col < R ? col : R - 1)) * PROW + s * 32 + 8 * g);
+          products(s, grp, pb);
+        }
     }
+    if (MORE) fetch_v(t + 4);
     wave_lds_sync();
-
-    // ---- O^T += V^T P^T: channel 64 grp + 4 row + i of operand A's row ----
-#pragma unroll
-    for (int s = 0; s < NSUB; ++s)
-#pragma unroll
-      for (int grp = 0; grp < G; ++grp) {
-        bf16x8 pb[PS];
-#pragma unroll
-        for (int k = 0; k < PS; ++k)
-          pb[k] = *reinterpret_cast<const bf16x8 *>(
-              pr + ((grp * PS + k) * R + (col < R ? col : R - 1)) * PROW + s * 32 + 8 * g);
-        if (F32) {
-          f32x4 start = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int k = 0; k < PS; ++k) start = mfma16(center, pb[k], start);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bf16x8 v8 = codes16(vnow[s][grp][i]);
-            f32x4 o = start;
-#pragma unroll
-            for (int k = 0; k < PS; ++k) o = mfma16(v8, pb[k], o);
-            acc[grp][i] += o;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bf16x8 v8 = codes16(vnow[s][grp][i]);
-#pragma unroll
-            for (int k = 0; k < PS; ++k) acc[grp][i] = mfma16(v8, pb[k], acc[grp][i]);
-          }
-        }
-      }
-    wave_lds_sync();
+  };
+  if (t < t_end) {
+    for (; t + 4 < t_end; t += 4) tile(t, std::true_type{});
+    tile(t, std::false_type{});
   }
 
   // ---- join the four waves: each row's sum over its lanes, then the waves through LDS ----
 #pragma unroll
-  for (int o = LPR / 2; o > 0; o >>= 1) {
+  for (int o = DIRECT ? 32 : LPR / 2; o > (DIRECT ? 8 : 0); o >>= 1) {
     l += __shfl_xor(l, o, 64);
 #pragma unroll
     for (int grp = 0; grp < G; ++grp) csum[grp] += __shfl_xor(csum[grp], o, 64);
@@ -400,10 +542,9 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a) {
 #pragma unroll
     for (int grp = 0; grp < G; ++grp)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          jo[(wave * R + col) * DP + 64 * grp + 16 * g + 4 * e + i] = acc[grp][i][e];
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<f32x4 *>(jo + (wave * R + col) * DP + 64 * grp + 16 * g + 4 * e) =
+            (f32x4){acc[grp][0][e], acc[grp][1][e], acc[grp][2][e], acc[grp][3][e]};
   }
   if (sl == 0) {
     float *m = jm + (wave * R + row) * (2 + G);
@@ -413,7 +554,7 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a) {
     for (int grp = 0; grp < G; ++grp) m[2 + grp] = csum[grp];
   }
   __syncthreads();
-  const int64_t first_row = (b * a.H + h) * (a.Lq * a.share) + (int64_t)rt * 16;
+  const int64_t first_row = ((int64_t)b * a.H + h) * ((int64_t)Lq * a.share) + row0;
   for (int idx = threadIdx.x; idx < R * DP; idx += 256) {
     const int orow = idx / DP, c = idx % DP;
     if (orow >= tile_rows) continue;
@@ -429,13 +570,13 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a) {
       o += f * (jo[(w * R + orow) * DP + c] + m[2 + c / 64]);
     }
     if (a.splits == 1) {
-      const int orr = (int)rt * 16 + orow;
-      const int64_t i = orr / a.share, oh = (int64_t)h * a.share + orr % a.share;
+      const int i = (int)((uint32_t)(row0 + orow) / (uint32_t)a.share);
+      const int64_t oh = (int64_t)h * a.share + (row0 + orow - i * a.share);
       if (c < a.d)
         ((T *)a.out)[b * a.o_stride[0] + oh * a.o_stride[1] + i * a.o_stride[2] + c] =
             from_f32<T>(sum == 0.f ? 0.f : o / sum);
     } else {
-      const int64_t at = (first_row + orow) * a.splits + split;
+      const int64_t at = (first_row + orow) * a.splits + split_no;
       a.part_o[at * DP + c] = o;
       if (c == 0) {
         a.part_ml[at * 2] = mx;
@@ -475,8 +616,7 @@ void launch(const Kv4Attn &a, hipStream_t s) {
   const int64_t rows = a.Lq * a.share;
   const dim3 grid((unsigned)(a.B * a.H * a.row_tiles * a.splits)), block(256);
 #define GO(R) hipLaunchKernelGGL((kv4_attn_kernel<T, DP, R>), grid, block, 0, s, a)
-  if (rows > 8) GO(16);
-  else if (rows > 4) GO(8);
+  if (rows > 4) GO(16);
   else if (rows > 2) GO(4);
   else if (rows > 1) GO(2);
   else GO(1);

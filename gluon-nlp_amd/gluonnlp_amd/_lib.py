@@ -225,20 +225,19 @@ PROTOTYPES = {
                                                POINTER(T5BlockFolded), c_int, c_void_p, c_void_p,
                                                POINTER(T5Cfg), c_int64, c_int64, c_void_p, c_int,
                                                c_void_p, c_void_p, c_size_t, c_void_p]),
-    'gnlp_kv4_write': (c_int, [POINTER(Kv4Cache), c_void_p, c_void_p, c_int, c_int64,
-                               POINTER(c_int64), POINTER(c_int64), c_void_p, c_int, c_void_p,
-                               c_int, c_void_p]),
-    'gnlp_kv4_read': (c_int, [POINTER(Kv4Cache), c_void_p, c_void_p, c_int, c_int64,
-                              POINTER(c_int64), POINTER(c_int64), c_void_p, c_int, c_void_p,
-                              c_int, c_void_p]),
-    'gnlp_kv4_attn_workspace_bytes': (c_size_t, [POINTER(Kv4Cache), POINTER(Kv4AttnDesc)]),
-    'gnlp_kv4_attn': (c_int, [c_void_p, c_void_p, POINTER(Kv4Cache), POINTER(Kv4AttnDesc), c_int,
-                              c_void_p, c_size_t, c_void_p]),
-    'gnlp_beam_select_workspace_bytes': (c_size_t, [POINTER(BeamDesc)]),
+    # (descriptors, stride triples and state lists arrive packed: bytes, arrays or byref())
+    'gnlp_kv4_write': (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_void_p, c_void_p,
+                               c_void_p, c_int, c_void_p, c_int, c_void_p]),
+    'gnlp_kv4_read': (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_void_p, c_void_p,
+                              c_void_p, c_int, c_void_p, c_int, c_void_p]),
+    'gnlp_kv4_attn_workspace_bytes': (c_size_t, [c_void_p, c_void_p]),
+    'gnlp_kv4_attn': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t,
+                              c_void_p]),
+    'gnlp_beam_select_workspace_bytes': (c_size_t, [c_void_p]),
     'gnlp_beam_select': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
-                                 c_void_p, POINTER(BeamDesc), c_void_p, c_size_t, c_void_p]),
-    'gnlp_reorder_states': (c_int, [POINTER(State), c_int, c_int64, c_int64, c_void_p, c_int,
-                                    c_void_p, c_int, c_void_p]),
+                                 c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    'gnlp_reorder_states': (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int, c_void_p,
+                                    c_int, c_void_p]),
 }
 
 _lib = None

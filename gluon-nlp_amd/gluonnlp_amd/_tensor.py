@@ -95,14 +95,28 @@ def stream(dev):
     return torch.cuda.current_stream(dev).cuda_stream
 
 
-def launch(dev, fn, *args):
-    """Call a C entry point whose last argument is the stream, on torch's current stream of ``dev``
-    and with ``dev`` as the current device; a non-zero status raises."""
-    if dev.index is None or torch.cuda.current_device() == dev.index:
-        rc = fn(*args, stream(dev))
+_get_device = getattr(torch._C, '_cuda_getDevice', None)
+
+
+def device_index(first, *rest):
+    """Index of the device that all tensors (None: skipped) live on; ``require_device``'s errors."""
+    i = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != i:
+            i = -1
+    if i < 0:
+        return require_device(first, *rest).index
+    return i
+
+
+def launch(index, fn, *args):
+    """Call a C entry point whose last argument is the stream, on torch's current stream of device
+    ``index`` and with that as the current device; a non-zero status raises."""
+    if _get_device() == index:
+        rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, stream(dev))
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
     if rc:
         _lib.check(rc)
 

@@ -2,7 +2,9 @@
 ``gluonnlp/attention_cell.py`` (reference src/gluonnlp/attention_cell.py:19-22), computed by the
 gfx950 HIP kernels behind the C ABI (include/gluonnlp_amd.h)."""
 import ctypes
+import functools
 import math
+import struct
 from typing import Optional
 
 import torch
@@ -317,6 +319,25 @@ def _expand_keys(x, lead, slots):
     return torch.broadcast_to(x, lead + (Lm,)), Lm
 
 
+_KV4_DESC = struct.Struct('4q3q3qPqPqP4qPqP3qqd')     # gnlp_kv4_attn_desc
+
+
+@functools.lru_cache(maxsize=4096)
+def _kv4_workspace_of(B, Hc, slots, d, Lq, share, keys):
+    c = _lib.Kv4Cache()
+    c.B, c.H, c.slots, c.d = B, Hc, slots, d
+    a = _lib.Kv4AttnDesc()
+    a.Lq, a.share, a.keys = Lq, share, keys
+    return _lib.load().gnlp_kv4_attn_workspace_bytes(ctypes.byref(c), ctypes.byref(a))
+
+
+def _kv4_workspace(B, Hc, slots, d, Lq, share, keys, Lm, reach):
+    """Workspace of one call; a function of its sizes alone."""
+    if not 0 < keys < slots:
+        keys = slots
+    return _kv4_workspace_of(B, Hc, slots, d, Lq, share, min(keys, Lm) if reach else keys)
+
+
 def multi_head_dot_attn_cached(query, cache, layer=0, *, causal: bool = True, edge_scores=None,
                                edge_table=None, mask=None, query_length=None, scaled: bool = True,
                                query_head_units: Optional[int] = None, layout=None):
@@ -337,51 +358,53 @@ def multi_head_dot_attn_cached(query, cache, layer=0, *, causal: bool = True, ed
 
     Returns context_vec (B, Lq, H * d) / (Lq, B, H * d).  There is no gradient: a query that asks
     for one is refused."""
-    q = _inner_contig(T.as_tensor(query))
+    q = query if type(query) is torch.Tensor else T.as_tensor(query)
     layout = cache.layout if layout is None else layout
-    if layout not in _LAYOUT_PERM:
+    p = _LAYOUT_PERM.get(layout)
+    if p is None:
         raise NotImplementedError('layout="{}" is not supported! '
                                   'We only support layout = "NKT", "NTK", and "TNK".'
                                   .format(layout))
     e, table, m = T.as_tensor(edge_scores), T.as_tensor(edge_table), T.as_tensor(mask)
-    dev = T.require_device(cache.length, q, e, table, m)
-    if q.dim() != 4:
-        raise ValueError('query {} is not 4-dimensional'.format(tuple(q.shape)))
-    B, H, Lq = _bht_shape(q, layout)
-    d = q.shape[-1]
+    dev = T.device_index(cache.length, q, e, table, m)
+    shape = q.shape
+    if len(shape) != 4:
+        raise ValueError('query {} is not 4-dimensional'.format(tuple(shape)))
+    B, H, Lq, d = shape[p[0]], shape[p[1]], shape[p[2]], shape[3]
     if B != cache.batch_size or d != cache.head_units or H % cache.num_heads or H == 0:
-        raise ValueError('query {} (layout {}) does not match {}'.format(tuple(q.shape), layout,
+        raise ValueError('query {} (layout {}) does not match {}'.format(tuple(shape), layout,
                                                                         cache))
     if wants_grad(q, e, table):
         raise NotImplementedError('attention over a 4-bit cache has no gradient: decode under '
                                   'torch.no_grad()')
-    a = _lib.Kv4AttnDesc()
-    a.Lq, a.share, a.causal, a.keys = Lq, H // cache.num_heads, bool(causal), cache._bound
-    a.q_stride[:] = _bht_strides(q, layout)
+    st = q.stride()
+    if st[3] != 1 and d != 1:
+        q = q.contiguous()
+        st = q.stride()
     if layout == 'TNK':
-        ctx = torch.empty((Lq, B, H * d), dtype=q.dtype, device=dev)
-        a.o_stride[:] = (H * d, d, B * H * d)
+        ctx, os = q.new_empty((Lq, B, H * d)), (H * d, d, B * H * d)
     else:
-        ctx = torch.empty((B, Lq, H * d), dtype=q.dtype, device=dev)
-        a.o_stride[:] = (Lq * H * d, d, H * d)
-    a.length, a.length_dtype = cache.length.data_ptr(), _lib.I32
+        ctx, os = q.new_empty((B, Lq, H * d)), (Lq * H * d, d, H * d)
+    qlp, qlc = 0, 0
     if query_length is not None:
-        ql = cache._lengths(query_length, 'query_length')
-        a.q_length = ql.data_ptr()
-        a.q_length_dtype = _lib.I64 if ql.dtype == torch.int64 else _lib.I32
+        query_length = cache._lengths(query_length, 'query_length')
+        qlp = query_length.data_ptr()
+        qlc = _lib.I64 if query_length.dtype == torch.int64 else _lib.I32
     slots = Lm = cache._slots
+    ep, es, tp, tl, mp, ms = 0, (0, 0, 0, 0), 0, 0, 0, (0, 0, 0)
     if e is not None:
         if table is not None:
             raise ValueError('edge_scores and edge_table exclude each other')
         if e.dtype != q.dtype:
             e = e.to(q.dtype)
         e, Lm = _expand_keys(e, (B, H, Lq), slots)
-        a.edge_scores, a.edge_stride[:] = e.data_ptr(), e.stride()
+        ep, es = e.data_ptr(), e.stride()
     elif table is not None:
         if table.dim() != 2 or table.shape[0] != H or table.shape[1] < 1:
             raise ValueError('edge_table {} != (heads = {}, R >= 1)'.format(tuple(table.shape), H))
-        table = table.to(q.dtype).contiguous()
-        a.edge_table, a.table_len = table.data_ptr(), table.shape[1]
+        if table.dtype != q.dtype or not table.is_contiguous():
+            table = table.to(q.dtype).contiguous()
+        tp, tl = table.data_ptr(), table.shape[1]
     if m is not None:
         if m.dtype != torch.bool:
             m = m != 0
@@ -389,17 +412,18 @@ def multi_head_dot_attn_cached(query, cache, layer=0, *, causal: bool = True, ed
         if e is not None and Lm != Lmm and slots not in (Lm, Lmm):
             raise ValueError('edge_scores reach {} keys, mask {}'.format(Lm, Lmm))
         Lm = min(Lm, Lmm)
-        a.mask, a.mask_stride[:] = m.data_ptr(), m.stride()
-    a.Lm = Lm
-    if scaled:
-        a.temperature = math.sqrt(d if query_head_units is None else query_head_units)
-    lib = _lib.load()
-    desc = ctypes.byref(cache.layer_desc(layer))
-    nws = lib.gnlp_kv4_attn_workspace_bytes(desc, ctypes.byref(a))
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
-    T.launch(dev, lib.gnlp_kv4_attn, ctx.data_ptr(), q.data_ptr(), desc, ctypes.byref(a),
-             T.code(q), T.ptr(ws), nws)
-    return T.like_caller(ctx, query)
+        mp, ms = m.data_ptr(), m.stride()
+    t = math.sqrt(d if query_head_units is None else query_head_units) if scaled else 0.0
+    share = H // cache.num_heads
+    keys = (cache._bound + 255) // 256 * 256       # (a hint: rounded so that plans repeat)
+    desc = _KV4_DESC.pack(Lq, share, bool(causal), keys, st[p[0]], st[p[1]], st[p[2]], *os,
+                          cache._length_ptr, _lib.I32, qlp, qlc, ep, *es, tp, tl, mp, *ms, Lm, t)
+    layer = cache.layer_desc(layer)
+    nws = _kv4_workspace(B, cache.num_heads, slots, d, Lq, share, keys, Lm, ep or mp)
+    ws = q.new_empty(nws, dtype=torch.uint8) if nws else None
+    T.launch(dev, _lib.load().gnlp_kv4_attn, ctx.data_ptr(), q.data_ptr(), layer, desc, T.code(q),
+             ws.data_ptr() if nws else None, nws)
+    return ctx if type(query) is torch.Tensor else T.like_caller(ctx, query)
 
 
 class MultiHeadAttentionCell(torch.nn.Module):

@@ -11,17 +11,18 @@ bfloat16, a value is ``code * scale + minimum`` with a code of 0 .. 15; the erro
 most half a scale, (max - min) / 30, plus the roundings of scale and minimum to bfloat16.
 """
 import ctypes
+import struct
 
 import torch
 
 from . import _lib
 from . import _tensor as T
-from .autograd import wants_grad
 
 __all__ = ['QuantKVCache']
 
 _TIME = {'NKT': 2, 'NTK': 1, 'TNK': 0}
 _PERM = {'NKT': (0, 1, 2), 'NTK': (0, 2, 1), 'TNK': (1, 2, 0)}
+_pack3 = struct.Struct('3q').pack
 
 
 class QuantKVCache:
@@ -64,7 +65,7 @@ class QuantKVCache:
         self._v_codes = torch.zeros(lead + (slots // 8, padded), dtype=torch.int32, device=dev)
         self._k_par = torch.zeros(lead + (groups, slots), dtype=torch.int32, device=dev)
         self._v_par = torch.zeros(lead + (groups, slots), dtype=torch.int32, device=dev)
-        self.length = torch.zeros(batch_size, dtype=torch.int32, device=dev)
+        self._length = torch.zeros(batch_size, dtype=torch.int32, device=dev)
         self._bound = 0            # no sequence holds more tokens
         self._desc = []
         for i in range(num_layers):
@@ -73,27 +74,36 @@ class QuantKVCache:
             c.k_codes, c.v_codes = self._k_codes[i].data_ptr(), self._v_codes[i].data_ptr()
             c.k_par, c.v_par = self._k_par[i].data_ptr(), self._v_par[i].data_ptr()
             self._desc.append(c)
+        self._refs = [ctypes.addressof(c) for c in self._desc]
+        self._length_ptr = self._length.data_ptr()
 
     def __repr__(self):
         return '{}(batch_size={}, num_heads={}, head_units={}, max_length={}, num_layers={}, ' \
                'layout="{}")'.format(self.__class__.__name__, self.batch_size, self.num_heads,
                                      self.head_units, self.max_length, self.num_layers, self.layout)
 
+    @property
+    def length(self):
+        """(batch_size,) int32 on the device: the tokens held (written by the calls below only)."""
+        return self._length
+
     def layer_desc(self, layer):
+        """Address of the layer's gnlp_kv4_cache."""
         if not 0 <= layer < self.num_layers:
             raise IndexError('layer {} of {}'.format(layer, self.num_layers))
-        return self._desc[layer]
+        return self._refs[layer]
 
     def _lengths(self, v, name):
         """A (batch_size,) device vector of whole numbers."""
-        v = T.as_tensor(v)
+        if type(v) is not torch.Tensor:
+            v = T.as_tensor(v)
         if v.dtype not in (torch.int32, torch.int64):
             raise TypeError('{} must be int32 or int64, got {}'.format(name, v.dtype))
         if v.dim() != 1 or v.shape[0] != self.batch_size:
             raise ValueError('{} {} != (batch_size,) = ({},)'.format(name, tuple(v.shape),
                                                                      self.batch_size))
-        T.require_device(self.length, v)
-        return v.contiguous()
+        T.device_index(self.length, v)
+        return v if v.is_contiguous() else v.contiguous()
 
     # ---- lengths ----
     def reset(self):
@@ -135,40 +145,43 @@ class QuantKVCache:
         self._bound = min(self._bound + n, self.max_length)
 
     # ---- tokens ----
-    def _strides(self, x):
-        st, p = x.stride(), _PERM[self.layout]
-        return _lib.I64x3(st[p[0]], st[p[1]], st[p[2]])
-
-    def _check_tokens(self, x, name):
-        p = _PERM[self.layout]
-        if x.dim() != 4 or x.shape[p[0]] != self.batch_size or x.shape[p[1]] != self.num_heads \
-                or x.shape[3] != self.head_units:
-            raise ValueError('{} {} does not match {}'.format(name, tuple(x.shape), self))
-        return x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous()
+    def _tokens(self, x, name):
+        """-> (tensor with contiguous channels, its packed (b, h, t) strides)"""
+        if type(x) is not torch.Tensor:
+            x = T.as_tensor(x)
+        p, shape = _PERM[self.layout], x.shape
+        if len(shape) != 4 or shape[p[0]] != self.batch_size or shape[p[1]] != self.num_heads \
+                or shape[3] != self.head_units:
+            raise ValueError('{} {} does not match {}'.format(name, tuple(shape), self))
+        st = x.stride()
+        if st[3] != 1 and shape[3] != 1:
+            x = x.contiguous()
+            st = x.stride()
+        if x.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError('a 4-bit cache has no gradient: decode under torch.no_grad()')
+        return x, _pack3(st[p[0]], st[p[1]], st[p[2]])
 
     def write(self, key, value, layer=0, new_length=None):
         """Store the last tokens counted in: key / value (batch_size, n, num_heads, head_units) in
         the cache's layout go to the last n of the ``length`` tokens of each sequence.  With
         ``new_length`` (batch_size,), sequence b stores its first new_length[b] tokens as its last
         new_length[b] (the others, padding, are not read).  Other tokens keep their values."""
-        k = self._check_tokens(T.as_tensor(key), 'key')
-        v = self._check_tokens(T.as_tensor(value), 'value')
-        dev = T.require_device(self.length, k, v)
-        if wants_grad(k, v):
-            raise NotImplementedError('a 4-bit cache has no gradient: decode under torch.no_grad()')
+        k, ks = self._tokens(key, 'key')
+        v, vs = self._tokens(value, 'value')
+        dev = T.device_index(self.length, k, v)
         if k.dtype != v.dtype or k.shape != v.shape:
             raise ValueError('key and value must share shape and dtype')
         n = k.shape[_TIME[self.layout]]
-        if new_length is None and n > self._bound:
-            raise ValueError('write of {} tokens, {} are counted in: call extend() first'
-                             .format(n, self._bound))
         nl, code = None, 0
         if new_length is not None:
-            nl = self._lengths(new_length, 'new_length')
-            code = _lib.I64 if nl.dtype == torch.int64 else _lib.I32
-        T.launch(dev, _lib.load().gnlp_kv4_write, ctypes.byref(self.layer_desc(layer)),
-                 k.data_ptr(), v.data_ptr(), T.code(k), n, self._strides(k), self._strides(v),
-                 self.length.data_ptr(), _lib.I32, T.ptr(nl), code)
+            new_length = self._lengths(new_length, 'new_length')
+            nl = new_length.data_ptr()
+            code = _lib.I64 if new_length.dtype == torch.int64 else _lib.I32
+        elif n > self._bound:
+            raise ValueError('write of {} tokens, {} are counted in: call extend() first'
+                             .format(n, self._bound))
+        T.launch(dev, _lib.load().gnlp_kv4_write, self.layer_desc(layer), k.data_ptr(),
+                 v.data_ptr(), T.code(k), n, ks, vs, self._length_ptr, _lib.I32, nl, code)
 
     def read(self, n=None, start=None, layer=0, dtype='float32'):
         """The values held: (key, value) of n tokens (default: max_length) from ``start``
@@ -176,19 +189,24 @@ class QuantKVCache:
         n = self.max_length if n is None else int(n)
         if n < 0:
             raise ValueError('n={} is negative'.format(n))
-        dev = T.require_device(self.length)
+        dev = T.device_index(self.length)
         st, code = None, 0
         if start is not None:
-            st = self._lengths(start, 'start')
-            code = _lib.I64 if st.dtype == torch.int64 else _lib.I32
+            start = self._lengths(start, 'start')
+            st = start.data_ptr()
+            code = _lib.I64 if start.dtype == torch.int64 else _lib.I32
         B, H, d = self.batch_size, self.num_heads, self.head_units
-        shape = {'NKT': (B, H, n, d), 'NTK': (B, n, H, d), 'TNK': (n, B, H, d)}[self.layout]
-        dt = T.torch_dtype(dtype)
-        key = torch.empty(shape, dtype=dt, device=dev)
-        value = torch.empty(shape, dtype=dt, device=dev)
-        T.launch(dev, _lib.load().gnlp_kv4_read, ctypes.byref(self.layer_desc(layer)),
-                 key.data_ptr(), value.data_ptr(), T.code(key), n, self._strides(key),
-                 self._strides(value), self.length.data_ptr(), _lib.I32, T.ptr(st), code)
+        if self.layout == 'NTK':
+            shape, strides = (B, n, H, d), _pack3(n * H * d, d, H * d)
+        elif self.layout == 'NKT':
+            shape, strides = (B, H, n, d), _pack3(H * n * d, n * d, d)
+        else:
+            shape, strides = (n, B, H, d), _pack3(H * d, d, B * H * d)
+        key = self.length.new_empty(shape, dtype=T.torch_dtype(dtype))
+        value = torch.empty_like(key)
+        T.launch(dev, _lib.load().gnlp_kv4_read, self.layer_desc(layer), key.data_ptr(),
+                 value.data_ptr(), T.code(key), n, strides, strides, self._length_ptr, _lib.I32, st,
+                 code)
         return key, value
 
     def reorder(self, parents):
@@ -197,7 +215,7 @@ class QuantKVCache:
         tokens held are moved."""
         from .sequence_sampler import check_parents, launch_reorder
         p, N, K = check_parents(parents, self.batch_size)
-        dev = T.require_device(self.length, p)
+        dev = T.device_index(self.length, p)
         if K > 32:
             raise ValueError('beam size {} > 32'.format(K))
         flat = []

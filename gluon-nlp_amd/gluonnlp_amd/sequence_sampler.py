@@ -2,6 +2,8 @@
 that follows it (what the reference's sequence_sampler.py builds from log_softmax, topk and take)."""
 import array
 import ctypes
+import functools
+import struct
 
 import torch
 
@@ -13,6 +15,16 @@ from .kv_cache import QuantKVCache
 __all__ = ['beam_search_select', 'reorder_states']
 
 MAX_BEAMS = 32
+
+
+_BEAM_DESC = struct.Struct('7qPq3d')     # gnlp_beam_desc
+
+
+@functools.lru_cache(maxsize=1024)
+def _select_workspace(N, K, V):
+    d = _lib.BeamDesc()
+    d.N, d.K, d.V = N, K, V
+    return _lib.load().gnlp_beam_select_workspace_bytes(ctypes.byref(d))
 
 
 def beam_search_select(outputs, scores, finished=None, *, eos_id=None, step=1, alpha=0.0,
@@ -37,23 +49,25 @@ def beam_search_select(outputs, scores, finished=None, *, eos_id=None, step=1, a
     of finished beams are not read.  ``step`` may be a device integer tensor of one element (a
     captured step then follows it).  Candidates are compared in 64 bits."""
     x, s, f = T.as_tensor(outputs), T.as_tensor(scores), T.as_tensor(finished)
-    dev = T.require_device(x, s, f)
+    dev = T.device_index(x, s, f)
     if s.dim() != 2 or s.dtype != torch.float32:
         raise ValueError('scores must be (items, beams) float32, got {} {}'.format(
             tuple(s.shape), s.dtype))
     N, K = s.shape
     if not 1 <= K <= MAX_BEAMS:
         raise ValueError('beam size {} is outside [1, {}]'.format(K, MAX_BEAMS))
-    if x.dim() not in (2, 3) or x.shape[:-1] not in ((N, K), (N * K,)) or x.shape[-1] < 1:
-        raise ValueError('outputs {} do not match scores {}'.format(tuple(x.shape), tuple(s.shape)))
+    shape = x.shape
+    if shape[:-1] not in ((N, K), (N * K,)) or shape[-1] < 1:
+        raise ValueError('outputs {} do not match scores {}'.format(tuple(shape), tuple(s.shape)))
     if wants_grad(x, s):
         raise NotImplementedError('the selection has no gradient: search under torch.no_grad()')
-    V = x.shape[-1]
-    if x.stride(-1) != 1 and V > 1 or x.dim() == 3 and x.stride(0) != K * x.stride(1) \
-            or x.stride(-2) < V:
+    V, st = shape[-1], x.stride()
+    if st[-1] != 1 and V > 1 or len(st) == 3 and st[0] != K * st[1] or st[-2] < V:
         x = x.contiguous()
+        st = x.stride()
     if not s.is_contiguous():
         s = s.contiguous()
+    fp = None
     if f is not None:
         if f.shape != s.shape:
             raise ValueError('finished {} does not match scores {}'.format(tuple(f.shape),
@@ -62,28 +76,29 @@ def beam_search_select(outputs, scores, finished=None, *, eos_id=None, step=1, a
             f = f != 0
         if not f.is_contiguous():
             f = f.contiguous()
-    d = _lib.BeamDesc()
-    d.N, d.K, d.V, d.row_stride = N, K, V, x.stride(-2)
-    d.normalize, d.eos = bool(normalize), -1 if eos_id is None else int(eos_id)
-    d.temperature, d.alpha = temperature, alpha
-    d.length_base = K if length_base is None else length_base
+        fp = f.data_ptr()
+    step_ptr, step_code = 0, 0
     if isinstance(step, torch.Tensor):
-        T.require_device(x, step)
+        T.device_index(x, step)
         if step.numel() != 1 or step.dtype not in (torch.int32, torch.int64):
             raise ValueError('step must hold one int32 / int64')
-        d.step_dev = step.data_ptr()
-        d.step_dtype = _lib.I64 if step.dtype == torch.int64 else _lib.I32
-    else:
-        d.step = step
-    lib = _lib.load()
-    out_scores = torch.empty((N, K), dtype=torch.float32, device=dev)
-    parents, tokens = torch.empty((2, N, K), dtype=torch.int32, device=dev).unbind(0)
-    out_finished = torch.empty((N, K), dtype=torch.bool, device=dev)
-    nws = lib.gnlp_beam_select_workspace_bytes(ctypes.byref(d))
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev)
-    T.launch(dev, lib.gnlp_beam_select, out_scores.data_ptr(), parents.data_ptr(),
-             tokens.data_ptr(), out_finished.data_ptr(), x.data_ptr(), T.code(x), s.data_ptr(),
-             T.ptr(f), ctypes.byref(d), ws.data_ptr(), nws)
+        step_ptr = step.data_ptr()
+        step_code = _lib.I64 if step.dtype == torch.int64 else _lib.I32
+        step = 0
+    desc = _BEAM_DESC.pack(N, K, V, st[-2], bool(normalize), -1 if eos_id is None else int(eos_id),
+                           step, step_ptr, step_code, temperature, alpha,
+                           K if length_base is None else length_base)
+    out_scores = torch.empty_like(s)
+    parents = s.new_empty((N, K), dtype=torch.int32)
+    tokens = torch.empty_like(parents)
+    out_finished = s.new_empty((N, K), dtype=torch.bool)
+    nws = _select_workspace(N, K, V)
+    ws = s.new_empty(nws, dtype=torch.uint8)
+    T.launch(dev, _lib.load().gnlp_beam_select, out_scores.data_ptr(), parents.data_ptr(),
+             tokens.data_ptr(), out_finished.data_ptr(), x.data_ptr(), T.code(x), s.data_ptr(), fp,
+             desc, ws.data_ptr(), nws)
+    if type(outputs) is torch.Tensor:
+        return out_scores, parents, tokens, out_finished
     return tuple(T.like_caller(o, outputs) for o in (out_scores, parents, tokens, out_finished))
 
 
@@ -101,10 +116,9 @@ def check_parents(parents, rows):
 def launch_reorder(dev, flat, N, K, parents, length):
     """flat: the fields of one gnlp_state (include/gluonnlp_amd.h) after the other."""
     buf = array.array('q', flat)
-    T.launch(dev, _lib.load().gnlp_reorder_states,
-             ctypes.cast(buf.buffer_info()[0], ctypes.POINTER(_lib.State)), len(flat) // 10, N, K,
+    T.launch(dev, _lib.load().gnlp_reorder_states, buf.buffer_info()[0], len(flat) // 10, N, K,
              parents.data_ptr(), _lib.I64 if parents.dtype == torch.int64 else _lib.I32,
-             T.ptr(length), _lib.I32)
+             None if length is None else length.data_ptr(), _lib.I32)
 
 
 def reorder_states(states, parents, batch_axis=0, out=None):
@@ -121,61 +135,64 @@ def reorder_states(states, parents, batch_axis=0, out=None):
     in_place = out is states
     if in_place and K > MAX_BEAMS:
         raise ValueError('in place: beam size {} > {}'.format(K, MAX_BEAMS))
+    dev = T.device_index(p)
+    rows, grad = N * K, torch.is_grad_enabled()
     flat, sources, caches = [], [], []
-    dev = T.require_device(p)
+
+    def one(s, axis, o):
+        t = s if type(s) is torch.Tensor else T.as_tensor(s)
+        if t.get_device() != dev:
+            T.require_device(p, t)
+        if grad and t.requires_grad:
+            raise NotImplementedError('reordering has no gradient: decode under torch.no_grad()')
+        shape = t.shape
+        if type(axis) is not int or not 0 <= axis < len(shape) or shape[axis] != rows:
+            raise ValueError('state {}: axis {} does not hold {} x {} rows'.format(
+                tuple(shape), axis, N, K))
+        if not t.is_contiguous():
+            if in_place:
+                raise ValueError('in place: the states must be contiguous')
+            t = t.contiguous()
+            sources.append(t)      # (it has to live until the launch)
+        if in_place:
+            d = t
+        elif o is None:
+            d = torch.empty_like(t)
+        else:
+            d = o if type(o) is torch.Tensor else T.as_tensor(o)
+            if d.shape != shape or d.dtype != t.dtype or not d.is_contiguous() or \
+                    d.get_device() != dev:
+                raise ValueError('out {} {} does not fit the state {} {}'.format(
+                    tuple(d.shape), d.dtype, tuple(shape), t.dtype))
+        n = t.numel()
+        if n:
+            step = t.stride(axis)
+            row = step * t.element_size()
+            flat.extend((t.data_ptr(), d.data_ptr(), n // (rows * step), row * rows, row, 1, row,
+                         row, 0, 0))
+        return d if s is t or type(s) is torch.Tensor else T.like_caller(d, s)
 
     def walk(s, axis, o):
+        if isinstance(s, torch.Tensor):
+            return one(s, axis, o)
         if s is None:
             return None
         if isinstance(s, QuantKVCache):
-            if s not in caches:
+            if not any(c is s for c in caches):
                 caches.append(s)
             return s
         if isinstance(s, (list, tuple)):
             n = len(s)
-            axes = axis if isinstance(axis, (list, tuple)) else [axis] * n
-            outs = o if isinstance(o, (list, tuple)) else [o] * n
+            axes = axis if isinstance(axis, (list, tuple)) else (axis,) * n
+            outs = o if isinstance(o, (list, tuple)) else (o,) * n
             if len(axes) != n or len(outs) != n or (o is not None and outs is not o):
                 raise ValueError('batch_axis / out are not nested like the states')
-            return type(s)([walk(*x) for x in zip(s, axes, outs)])
-        t = T.as_tensor(s)
-        T.require_device(p, t)
-        if wants_grad(t):
-            raise NotImplementedError('reordering has no gradient: decode under torch.no_grad()')
-        if not isinstance(axis, int) or not 0 <= axis < t.dim() or t.shape[axis] != N * K:
-            raise ValueError('state {}: axis {} does not hold {} x {} rows'.format(
-                tuple(t.shape), axis, N, K))
-        if in_place:
-            if not t.is_contiguous():
-                raise ValueError('in place: the states must be contiguous')
-            d = t
-        else:
-            t = t.contiguous()
-            if o is None:
-                d = torch.empty_like(t)
-            else:
-                d = T.as_tensor(o)
-                if d.shape != t.shape or d.dtype != t.dtype or not d.is_contiguous():
-                    raise ValueError('out {} {} does not fit the state {} {}'.format(
-                        tuple(d.shape), d.dtype, tuple(t.shape), t.dtype))
-                T.require_device(p, d)
-        row = t.stride(axis) * t.element_size() if t.numel() else 0
-        outer = t.numel() // (N * K * t.stride(axis)) if row else 0
-        flat.extend((t.data_ptr(), d.data_ptr(), outer, row * N * K, row, 1, row, row, 0, 0))
-        sources.append(t)      # (a contiguous copy has to live until the launch)
-        return T.like_caller(d, s)
+            r = [walk(*x) for x in zip(s, axes, outs)]
+            return r if isinstance(s, list) else tuple(r)
+        return one(s, axis, o)
 
     result = walk(states, batch_axis, None if in_place else out)
     if flat:
-        # no destination may be read, or written twice
-        spans = sorted((flat[i + w], flat[i + 2] * flat[i + 3], w)
-                       for i in range(0, len(flat), 10) for w in ((1,) if in_place else (0, 1)))
-        end = last = 0
-        for at, size, w in spans:
-            if size and at < end and (w or last):
-                raise ValueError('states and out overlap')
-            if at + size > end:
-                end, last = at + size, w
         launch_reorder(dev, flat, N, K, p, None)
     for c in caches:
         c.reorder(p)
