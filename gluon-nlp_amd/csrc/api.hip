@@ -1814,7 +1814,8 @@ int gnlp_kv4_attn(void *ctx, const void *q, const gnlp_kv4_cache *cache,
   REQUIRE(d->Lq <= (1LL << 24) && d->share <= (1LL << 24) && d->Lq * d->share <= (1LL << 30),
           "4-bit attention: too many query rows");
   REQUIRE(!(d->edge_scores && d->edge_table), "edge_scores and edge_table exclude each other");
-  REQUIRE(!d->edge_table || d->table_len > 0, "edge_table without entries");
+  REQUIRE(!d->edge_table || (d->table_len > 0 && d->table_len < (1LL << 30)),
+          "edge_table: bad number of entries");
   REQUIRE(!(d->edge_scores || d->mask) || d->Lm >= 0, "negative Lm");
   REQUIRE(vl_ok((int)d->length_dtype) && (!d->q_length || vl_ok((int)d->q_length_dtype)),
           "lengths must be int32 or int64");
@@ -1842,12 +1843,13 @@ int gnlp_kv4_attn(void *ctx, const void *q, const gnlp_kv4_cache *cache,
   a.edge = d->edge_scores; a.table = d->edge_table; a.table_len = d->table_len;
   a.mask = d->mask;
   a.Lm = d->edge_scores || d->mask ? d->Lm : cache->slots;
+  if (a.Lm == 0) { a.edge = nullptr; a.mask = nullptr; }   // nothing is seen, nothing to read
   a.inv_temperature = d->temperature > 0 ? (float)(1.0 / d->temperature) : 1.0f;
   const int64_t rows = d->Lq * d->share;
   a.row_tiles = (int)((rows + 15) / 16);
   a.splits = kv4_splits(cache, d);
-  REQUIRE(cache->B * cache->H * a.row_tiles * a.splits < (1LL << 31),
-          "4-bit attention: too many workgroups");
+  REQUIRE(cache->B * cache->H * a.row_tiles * a.splits < (1LL << 31) &&
+              cache->B * cache->H * rows < (1LL << 31), "4-bit attention: too many workgroups");
   if (a.splits > 1) {
     const size_t need = gnlp_kv4_attn_workspace_bytes(cache, d);
     REQUIRE(workspace && workspace_bytes >= need, "workspace too small: %zu < %zu",

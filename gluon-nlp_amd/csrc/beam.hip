@@ -18,8 +18,8 @@
 //   order-preserving integer, for a bound that K lanes reach; the best bound of the four waves
 //   leaves little more than K values, which a list in LDS ranks by counting.  Where ties overfill
 //   the list (a constant row), K rounds of a block-wide maximum do it.
-//   The merge does the same with the chunks' best candidates and walks down a chunk's list only
-//   while it stays above the bound.
+//   The merge does the same with the chunks' best candidates and reads on only in the lists that
+//   reach its bound, all of them at once.
 // Bound by memory (the logits once) and by the instructions of the pass: 10 a logit, of which the
 // exponential's 4; a workgroup of 8192 logits spreads the 400 or so that it spends on top.
 //
@@ -170,19 +170,12 @@ __global__ void __launch_bounds__(256) beam_chunk_kernel(BeamSelect a) {
   }
   const float least = unordered(max(max(sh_bound[0], sh_bound[1]), max(sh_bound[2], sh_bound[3])));
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const bool in = x[e] >= least && (whole || at(e) < V);
-    const uint64_t on = __ballot(in);
-    if (on) {
-      uint32_t start = 0;
-      if (lane == 0) start = atomicAdd(&sh_n, (uint32_t)__popcll(on));
-      start = __builtin_amdgcn_readfirstlane(start);
-      const uint32_t pos = start + __builtin_amdgcn_mbcnt_hi((uint32_t)(on >> 32),
-                                                             __builtin_amdgcn_mbcnt_lo((uint32_t)on, 0));
-      if (in && pos < CAP)                 // (x + 0: -0 and +0 are one value)
+  for (int e = 0; e < E; ++e)
+    if (x[e] >= least && (whole || at(e) < V)) {
+      const uint32_t pos = atomicAdd(&sh_n, 1u);
+      if (pos < CAP)                       // (x + 0: -0 and +0 are one value)
         list[pos] = ((uint64_t)ordered(x[e] + 0.0f) << 32) | (uint32_t)~at(e);
     }
-  }
   __syncthreads();
   const uint32_t n = sh_n;
   float *ox = a.cand_x + slot * a.K;
@@ -242,27 +235,33 @@ __device__ __forceinline__ bool better(double x, int64_t i, double y, int64_t j)
   return x > y || (x == y && i < j);
 }
 
-__global__ void __launch_bounds__(256) beam_merge_kernel(BeamSelect a) {
-  constexpr int LIST = 1024;
+constexpr int MERGE = 512;                // threads of the merge
+
+__global__ void __launch_bounds__(MERGE) beam_merge_kernel(BeamSelect a) {
+  constexpr int LIST = 1024, WAVES = MERGE / 64;
   __shared__ double lse[BEAM_MAX], sx[LIST];     // lse: the maximum of z taken off
   __shared__ float peak[BEAM_MAX];
   __shared__ int64_t si[LIST];
-  __shared__ uint32_t sh_n, sh_bound[4];
-  __shared__ double bx4[4];
-  __shared__ int64_t bi4[4];
+  __shared__ uint32_t live[LIST], sh_n, sh_live, sh_bound[WAVES];
+  __shared__ double bx4[WAVES];
+  __shared__ int64_t bi4[WAVES];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t item = blockIdx.x;
   const int K = a.K;
   const uint8_t *fin = a.finished ? a.finished + item * K : nullptr;
   const float *prevs = a.scores + item * K;
-  if (tid == 0) sh_n = 0;
+  const int64_t first = item * K * a.chunks;     // of the item's lists
+  // list c = beam * chunks + chunk holds up to K candidates, best first; from K chunks on: a
+  // finished beam, its own only candidate
+  const uint32_t own = K * a.chunks, lists = own + K;
+  if (tid == 0) { sh_n = 0; sh_live = 0; }
   // ---- logsumexp of each beam from its chunks ----
-  for (int k = wave; k < K; k += 4) {
+  for (int k = wave; k < K; k += WAVES) {
     double out = 0;
     float m = 0.f;
     if (a.normalize && !(fin && fin[k])) {
-      const float *st = a.stats + (item * K + k) * a.chunks * 2;
+      const float *st = a.stats + (first + k * a.chunks) * 2;
       m = NEG;
       for (uint32_t c = lane; c < a.chunks; c += 64) m = fmaxf(m, st[2 * c]);
       m = all_max(m);
@@ -280,7 +279,6 @@ __global__ void __launch_bounds__(256) beam_merge_kernel(BeamSelect a) {
       peak[k] = m;
     }
   }
-  __syncthreads();
   double lp_prev = a.lp_prev, lp_new = a.lp_new;
   if (a.step) {
     const double s = (double)load_len(a.step, a.step_dtype, 0);
@@ -288,15 +286,14 @@ __global__ void __launch_bounds__(256) beam_merge_kernel(BeamSelect a) {
     lp_new = pow((a.length_base + s) / (a.length_base + 1.0), a.alpha);
   }
   const double per_lp = 1.0 / lp_new;
+  __syncthreads();
   const int64_t none = 0x7fffffffffffffffLL, KV = (int64_t)K * a.V;
-  // candidate j of list c (c = beam * chunks + chunk; from K chunks on: finished beams, of one
-  // candidate) -> score and index (index `none`: there is no such candidate)
-  const uint32_t lists = K * a.chunks + K;
+  // candidate j of list c -> score and index (index `none`: there is no such candidate)
   auto get = [&](uint32_t c, int j, double &x, int64_t &i) {
     x = -__builtin_inf();
     i = none;
-    const bool self = c >= K * a.chunks;
-    const uint32_t k = self ? c - K * a.chunks : c / a.chunks;
+    const bool self = c >= own;
+    const uint32_t k = self ? c - own : c / a.chunks;
     const bool done = fin && fin[k];
     const float prev = prevs[k];
     const bool dead = !(prev > -1e15f);
@@ -306,11 +303,11 @@ __global__ void __launch_bounds__(256) beam_merge_kernel(BeamSelect a) {
         if (!dead) x = (double)prev;
       }
     } else if (!done) {
-      const int64_t at = (item * K * a.chunks + c) * K + j;
+      const int64_t at = (first + c) * K + j;
       const int32_t v = a.cand_i[at];
+      const float z = a.cand_x[at];
       if (v >= 0) {
         i = (int64_t)k * a.V + v;
-        const float z = a.cand_x[at];
         if (z > NEG && !dead)
           x = ((double)prev * lp_prev +
                (((double)z - (double)peak[k]) * a.inv_temperature - lse[k])) * per_lp;
@@ -320,7 +317,7 @@ __global__ void __launch_bounds__(256) beam_merge_kernel(BeamSelect a) {
   // ---- a bound that K lists' best candidates reach ----
   double mx = -__builtin_inf();
   bool any = false;
-  for (uint32_t c = tid; c < lists; c += 256) {
+  for (uint32_t c = tid; c < lists; c += MERGE) {
     double x;
     int64_t i;
     get(c, 0, x, i);
@@ -330,15 +327,31 @@ __global__ void __launch_bounds__(256) beam_merge_kernel(BeamSelect a) {
   const uint32_t bound = wave_bound<8>(any ? (uint32_t)(ordered(mx) >> 32) : 0u, K);
   if (lane == 0) sh_bound[wave] = bound;
   __syncthreads();
-  const uint32_t least = max(max(sh_bound[0], sh_bound[1]), max(sh_bound[2], sh_bound[3]));
-  for (uint32_t c = tid; c < lists; c += 256)
-    for (int j = 0; j < K; ++j) {                // (best first)
+  uint32_t least = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) least = max(least, sh_bound[w]);
+  // ---- the lists whose best candidate reaches it, then all of their candidates at once ----
+  for (uint32_t c = tid; c < lists; c += MERGE) {
+    double x;
+    int64_t i;
+    get(c, 0, x, i);
+    if (i != none && (uint32_t)(ordered(x) >> 32) >= least) {
+      const uint32_t pos = atomicAdd(&sh_live, 1u);
+      if (pos < LIST) live[pos] = c;
+    }
+  }
+  __syncthreads();
+  const uint32_t nlive = sh_live;
+  if (nlive <= LIST)
+    for (uint32_t q = tid; q < nlive * (uint32_t)K; q += MERGE) {
+      const uint32_t l = q / (uint32_t)K;
       double x;
       int64_t i;
-      get(c, j, x, i);
-      if (i == none || (uint32_t)(ordered(x) >> 32) < least) break;
-      const uint32_t pos = atomicAdd(&sh_n, 1u);
-      if (pos < LIST) { sx[pos] = x; si[pos] = i; }
+      get(live[l], (int)(q - l * K), x, i);
+      if (i != none && (uint32_t)(ordered(x) >> 32) >= least) {
+        const uint32_t pos = atomicAdd(&sh_n, 1u);
+        if (pos < LIST) { sx[pos] = x; si[pos] = i; }
+      }
     }
   __syncthreads();
   const uint32_t found = sh_n;
@@ -351,22 +364,24 @@ __global__ void __launch_bounds__(256) beam_merge_kernel(BeamSelect a) {
     a.out_tokens[to] = (int32_t)v;
     a.out_finished[to] = was || (a.has_eos && v == a.eos);
   };
-  if (found <= LIST) {
-    for (uint32_t c = tid; c < found; c += 256) {
+  if (nlive <= LIST && found <= LIST) {
+    for (uint32_t c = tid; c < found; c += MERGE) {
       const double x = sx[c];
       const int64_t i = si[c];
       int rank = 0;
+#pragma unroll 4
       for (uint32_t o = 0; o < found; ++o) rank += better(sx[o], si[o], x, i);
       if (rank < K) put(rank, x, i);
     }
     return;
   }
+  // ties overfill a list: K times the best of what is left
   double tx = __builtin_inf();
   int64_t ti = -1;
   for (int r = 0; r < K; ++r) {
     double bx = -__builtin_inf();
     int64_t bi = none;
-    for (uint32_t c = tid; c < lists; c += 256)
+    for (uint32_t c = tid; c < lists; c += MERGE)
       for (int j = 0; j < K; ++j) {
         double x;
         int64_t i;
@@ -386,7 +401,7 @@ __global__ void __launch_bounds__(256) beam_merge_kernel(BeamSelect a) {
     tx = bx4[0];
     ti = bi4[0];
 #pragma unroll
-    for (int w = 1; w < 4; ++w)
+    for (int w = 1; w < WAVES; ++w)
       if (better(bx4[w], bi4[w], tx, ti)) { tx = bx4[w]; ti = bi4[w]; }
     if (tid == 0) put(r, tx, ti);
   }
@@ -400,97 +415,125 @@ template <> struct Piece<16> { typedef f32x4 type; };
 template <> struct Piece<4> { typedef float type; };
 template <> struct Piece<1> { typedef uint8_t type; };
 
-// bytes of a segment that the row's length covers
-__device__ __forceinline__ int64_t live_bytes(const Reorder &a, const ReorderEntry &e, int64_t src) {
-  if (!a.length || e.slots_per_unit == 0) return e.seg_bytes;
-  int64_t n = load_len(a.length, a.length_dtype, src);
-  n = n < 0 ? 0 : n;
-  const int64_t used = (n + e.slots_per_unit - 1) / e.slots_per_unit * e.unit_bytes;
-  return used < e.seg_bytes ? used : e.seg_bytes;
+// pieces of a segment that the row's length covers
+template <int VB>
+__device__ __forceinline__ uint32_t live_pieces(const Reorder &a, const ReorderEntry &e,
+                                                int64_t row) {
+  const uint32_t all = (uint32_t)(e.seg_bytes / VB);
+  if (!a.length || e.slots_per_unit == 0) return all;
+  int64_t n = load_len(a.length, a.length_dtype, row);
+  n = n < 0 ? 0 : (n > (1LL << 30) ? 1LL << 30 : n);
+  const uint32_t units = ((uint32_t)n + (uint32_t)e.slots_per_unit - 1) / (uint32_t)e.slots_per_unit;
+  const int64_t used = ((int64_t)units * e.unit_bytes + VB - 1) / VB;
+  return used < all ? (uint32_t)used : all;
 }
 __device__ __forceinline__ int parent_of(const Reorder &a, int64_t row) {
   const int64_t p = load_len(a.parents, a.parents_dtype, row);
   return (int)(p < 0 ? 0 : (p >= a.K ? a.K - 1 : p));
 }
 
-// KM = 0: source and destination apart; a thread = UN pieces of one row, or of one piece column over
-// rows where a row's segment is short.
-// KM > 0: in place; a thread = one piece of all K <= KM rows of an item.
-template <int VB, int KM>
-__device__ __forceinline__ void reorder_piece(const Reorder &a, const ReorderEntry &e, int64_t block) {
+// Source and destination apart: a thread moves REORDER_UNROLL pieces of one row, or, where a row's
+// segment is short (flat), of a run of pieces over rows.
+template <int VB>
+__device__ __forceinline__ void reorder_apart(const Reorder &a, const ReorderEntry &e,
+                                              uint32_t block) {
   typedef typename Piece<VB>::type P;
-  constexpr int UN = KM ? 1 : REORDER_UNROLL;
-  const int64_t rows = KM ? a.N : a.N * a.K, pieces = e.seg_bytes / VB;
-  const int64_t span = e.flat ? rows * pieces : pieces, nb = (span + 256 * UN - 1) / (256 * UN);
-  const int64_t first = (block % nb) * (256 * UN) + threadIdx.x;
-  block /= nb;
-  int64_t row = 0;
+  constexpr int UN = REORDER_UNROLL;
+  const uint32_t rows = (uint32_t)(a.N * a.K), pieces = (uint32_t)(e.seg_bytes / VB);
+  const uint32_t nb = (uint32_t)e.nb;
+  uint32_t rest = block / nb;
+  const uint32_t first = (block - rest * nb) * (256 * UN) + threadIdx.x;
+  P v[UN];
   if (!e.flat) {
-    row = block % rows;
-    block /= rows;
-  }
-  const int64_t seg = block % e.nseg, outer = block / e.nseg;
-  const int64_t off = outer * e.outer_stride + seg * e.seg_stride;
-  const char *src = (const char *)e.src + off;
-  char *dst = (char *)e.dst + off;
-  if (KM == 0) {
-    P v[UN];
-    int64_t to[UN];
-#pragma unroll
-    for (int u = 0; u < UN; ++u) {
-      const int64_t at = first + u * 256;
-      int64_t r = row, p = at;
-      if (e.flat) {
-        r = (uint32_t)at / (uint32_t)pieces;
-        p = at - r * pieces;
-      }
-      to[u] = -1;
-      if (at < span) {
-        const int64_t from = r / a.K * a.K + parent_of(a, r);
-        if (p * VB < live_bytes(a, e, from)) {
-          v[u] = *reinterpret_cast<const P *>(src + from * e.row_stride + p * VB);
-          to[u] = r * e.row_stride + p * VB;
-        }
-      }
-    }
+    const uint32_t next = rest / rows, row = rest - next * rows;
+    const uint32_t outer = next / (uint32_t)e.nseg, seg = next - outer * (uint32_t)e.nseg;
+    const int64_t off = outer * e.outer_stride + seg * e.seg_stride;
+    const uint32_t from = row / (uint32_t)a.K * (uint32_t)a.K + parent_of(a, row);
+    const uint32_t live = live_pieces<VB>(a, e, from);
+    const P *src = (const P *)((const char *)e.src + off + from * e.row_stride);
+    P *dst = (P *)((char *)e.dst + off + row * e.row_stride);
 #pragma unroll
     for (int u = 0; u < UN; ++u)
-      if (to[u] >= 0) *reinterpret_cast<P *>(dst + to[u]) = v[u];
-  } else {
-    int64_t r = row, p = first;
-    if (first >= span) return;
-    if (e.flat) {
-      r = (uint32_t)first / (uint32_t)pieces;
-      p = first - r * pieces;
-    }
-    P v[KM ? KM : 1];
-    const int64_t r0 = r * a.K;
+      if (first + u * 256 < live) v[u] = src[first + u * 256];
 #pragma unroll
-    for (int k = 0; k < KM; ++k)
-      if (k < a.K) {
-        const int f = parent_of(a, r0 + k);
-        if (f != k && p * VB < live_bytes(a, e, r0 + f))
-          v[k] = *reinterpret_cast<const P *>(src + (r0 + f) * e.row_stride + p * VB);
-      }
-#pragma unroll
-    for (int k = 0; k < KM; ++k)
-      if (k < a.K) {
-        const int f = parent_of(a, r0 + k);
-        if (f != k && p * VB < live_bytes(a, e, r0 + f))
-          *reinterpret_cast<P *>(dst + (r0 + k) * e.row_stride + p * VB) = v[k];
-      }
+    for (int u = 0; u < UN; ++u)
+      if (first + u * 256 < live) dst[first + u * 256] = v[u];
+    return;
   }
+  const uint32_t outer = rest / (uint32_t)e.nseg, seg = rest - outer * (uint32_t)e.nseg;
+  const int64_t off = outer * e.outer_stride + seg * e.seg_stride;
+  int64_t to[UN];
+#pragma unroll
+  for (int u = 0; u < UN; ++u) {
+    const uint32_t at = first + u * 256, row = at / pieces, p = at - row * pieces;
+    to[u] = -1;
+    if (row < rows) {
+      const uint32_t from = row / (uint32_t)a.K * (uint32_t)a.K + parent_of(a, row);
+      if (p < live_pieces<VB>(a, e, from)) {
+        v[u] = *(const P *)((const char *)e.src + off + from * e.row_stride + (int64_t)p * VB);
+        to[u] = off + row * e.row_stride + (int64_t)p * VB;
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < UN; ++u)
+    if (to[u] >= 0) *(P *)((char *)e.dst + to[u]) = v[u];
 }
 
+// In place: a thread holds one piece of all K <= KM rows of an item before it writes any.
+template <int VB, int KM>
+__device__ __forceinline__ void reorder_in_place(const Reorder &a, const ReorderEntry &e,
+                                                 uint32_t block) {
+  typedef typename Piece<VB>::type P;
+  const uint32_t items = (uint32_t)a.N, pieces = (uint32_t)(e.seg_bytes / VB);
+  const uint32_t nb = (uint32_t)e.nb;
+  uint32_t rest = block / nb;
+  uint32_t p = (block - rest * nb) * 256 + threadIdx.x, item = 0;
+  if (e.flat) {
+    item = p / pieces;
+    p -= item * pieces;
+  } else {
+    const uint32_t next = rest / items;
+    item = rest - next * items;
+    rest = next;
+  }
+  if (item >= items || p >= pieces) return;
+  const uint32_t outer = rest / (uint32_t)e.nseg, seg = rest - outer * (uint32_t)e.nseg;
+  const int64_t r0 = (int64_t)item * a.K;
+  char *at = (char *)e.dst + outer * e.outer_stride + seg * e.seg_stride + r0 * e.row_stride +
+             (int64_t)p * VB;
+  P v[KM];
+  uint32_t moves = 0;
+#pragma unroll
+  for (int k = 0; k < KM; ++k)
+    if (k < a.K) {
+      const int f = parent_of(a, r0 + k);
+      if (f != k && p < live_pieces<VB>(a, e, r0 + f)) {
+        v[k] = *(const P *)(at + f * e.row_stride);
+        moves |= 1u << k;
+      }
+    }
+#pragma unroll
+  for (int k = 0; k < KM; ++k)
+    if ((moves >> k) & 1) *(P *)(at + k * e.row_stride) = v[k];
+}
+
+// KM = 0: source and destination apart
 template <int KM>
 __global__ void __launch_bounds__(256) reorder_kernel(Reorder a) {
-  int64_t block = blockIdx.x;
+  uint32_t block = blockIdx.x;
   int i = 0;
-  while (i + 1 < a.n && block >= a.e[i].blocks) block -= a.e[i++].blocks;
+  while (i + 1 < a.n && block >= (uint32_t)a.e[i].blocks) block -= (uint32_t)a.e[i++].blocks;
   const ReorderEntry &e = a.e[i];
-  if (e.piece == 16) reorder_piece<16, KM>(a, e, block);
-  else if (e.piece == 4) reorder_piece<4, KM>(a, e, block);
-  else reorder_piece<1, KM>(a, e, block);
+  if (KM == 0) {
+    if (e.piece == 16) reorder_apart<16>(a, e, block);
+    else if (e.piece == 4) reorder_apart<4>(a, e, block);
+    else reorder_apart<1>(a, e, block);
+  } else {
+    if (e.piece == 16) reorder_in_place<16, KM ? KM : 1>(a, e, block);
+    else if (e.piece == 4) reorder_in_place<4, KM ? KM : 1>(a, e, block);
+    else reorder_in_place<1, KM ? KM : 1>(a, e, block);
+  }
 }
 
 }  // namespace
@@ -529,7 +572,7 @@ void launch_beam_select(BeamSelect a, int64_t items, int dtype, void *ws, hipStr
     else GO(float, 16);
   }
 #undef GO
-  hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)items), block, 0, s, a);
+  hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)items), dim3(MERGE), 0, s, a);
 }
 
 // The caller has filled everything but piece and blocks.
@@ -546,7 +589,9 @@ bool launch_reorder(Reorder a, bool in_place, hipStream_t s) {
     const int64_t un = in_place ? 1 : REORDER_UNROLL;
     e.flat = pieces < 256 * un && rows * pieces < (1LL << 31);
     const int64_t span = e.flat ? rows * pieces : pieces;
-    e.blocks = (span + 256 * un - 1) / (256 * un) * (e.flat ? 1 : rows) * e.nseg * e.outer;
+    e.nb = (span + 256 * un - 1) / (256 * un);
+    e.blocks = e.nb * (e.flat ? 1 : rows) * e.nseg * e.outer;
+    if (pieces >= (1LL << 31) || e.blocks > 0x7fffffffLL) return false;
     total += e.blocks;
   }
   if (total > 0x7fffffffLL) return false;

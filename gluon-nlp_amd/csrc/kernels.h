@@ -332,6 +332,7 @@ struct Kv4Attn {
   int row_tiles, splits;
   float *part_o, *part_ml;            // splits > 1: (row, split, DP) and (row, split, 2) in float
 };
+constexpr int KV4_MAX_SPLITS = 64;    // (a wave of the join holds one each)
 int kv4_attn_plan(int64_t B, int64_t H, int64_t rows, int64_t keys, int64_t d);   // splits
 void launch_kv4_attn(const Kv4Attn &a, int dtype, hipStream_t s);
 
@@ -365,7 +366,7 @@ struct ReorderEntry {
   int64_t row_stride;                 // bytes
   int64_t nseg, seg_stride, seg_bytes;   // a row = nseg segments
   int64_t slots_per_unit, unit_bytes; // segments that hold tokens: slots share a unit (0: all copied)
-  int64_t blocks;
+  int64_t nb, blocks;                 // workgroups of a row's (flat: of all rows') segment, in all
   int piece;                          // bytes a thread moves at once
   int flat;                           // short segments: a block runs over rows too
 };

@@ -61,10 +61,15 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t w, int r) {
 }
 
 struct Unit {      // what a wave works on
-  int64_t b, h, slot0, first, end;   // slot0: the block's first slot; [first, end): the call's slots
-  int grp, which;                    // which: 0 = K, 1 = V
+  int b, h, grp, which;              // which: 0 = K, 1 = V
+  int slot0, first, end;             // slot0: the block's first slot; [first, end): the call's slots
   bool on;
 };
+
+// a length within what 32-bit arithmetic on slots (below 2^30, as L is) takes
+__device__ __forceinline__ int bounded(int64_t n) {
+  return n > (1 << 30) ? 1 << 30 : (n < -(1 << 30) ? -(1 << 30) : (int)n);
+}
 
 // grid: x = (block of slots, head, group), four waves a workgroup; y = sequence; z = K or V.  Heads
 // run fastest: neighbouring waves read neighbouring rows of an (N, T, H, d) tensor.
@@ -72,28 +77,29 @@ __device__ __forceinline__ Unit unit_of(const Kv4Io &a) {
   Unit u;
   const uint32_t w = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t per = (uint32_t)a.H << a.g_shift, blk = w / per, hg = w - blk * per;
+  const int L = (int)a.L;
   u.b = blockIdx.y;
   u.which = blockIdx.z;
-  u.h = hg >> a.g_shift;
+  u.h = (int)(hg >> a.g_shift);
   u.grp = (int)(hg & ((1u << a.g_shift) - 1));
   if (a.write) {                     // the last new_length slots of the sequence
-    const int64_t len = a.length ? load_len(a.length, a.length_dtype, u.b) : a.L;
-    int64_t n = a.count ? load_len(a.count, a.count_dtype, u.b) : a.L;
-    n = n < 0 ? 0 : (n > a.L ? a.L : n);
-    u.first = len - n;
-    u.end = len;
+    u.end = a.length ? bounded(load_len(a.length, a.length_dtype, u.b)) : L;
+    int n = a.count ? bounded(load_len(a.count, a.count_dtype, u.b)) : L;
+    n = n < 0 ? 0 : (n > L ? L : n);
+    u.first = u.end - n;
   } else {
-    u.first = a.count ? load_len(a.count, a.count_dtype, u.b) : 0;
-    u.end = u.first + a.L;
+    u.first = a.count ? bounded(load_len(a.count, a.count_dtype, u.b)) : 0;
+    u.end = u.first > 0x7fffffff - L ? 0x7fffffff : u.first + L;
   }
   // blocks of 8 slots, counted from the first slot's (also below slot 0, where nothing is held)
-  u.slot0 = ((u.first >> 3) + blk) << 3;
-  u.on = blk < a.nblk && u.slot0 < u.end && u.end < (1LL << 40) && u.first > -(1LL << 40);
+  u.on = blk < a.nblk && blk <= (uint32_t)((0x7ffffff0 - u.first) >> 3);
+  u.slot0 = (int)((u.first & ~7) + (u.on ? 8 * blk : 0));
+  u.on = u.on && u.slot0 < u.end;
   return u;
 }
 
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(float (&x)[8], const T *p, int64_t c0, int64_t d) {
+__device__ __forceinline__ void load8(float (&x)[8], const T *p, int c0, int d) {
   if (VEC) {
     if (c0 < d) {
       if (sizeof(T) == 2) {
@@ -119,36 +125,38 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(Kv4Io a) {
   const int lane = threadIdx.x & 63;
   const Unit u = unit_of(a);
   if (!u.on) return;
-  const int r = lane >> 3, c = lane & 7;
-  const int64_t slot = u.slot0 + tok_of(r);
-  const bool live = slot >= u.first && slot < u.end && slot >= 0 && slot < a.S;
-  if (__ballot(live) == 0) return;
-  const int64_t c0 = u.grp * 64 + 8 * c;
-  const int64_t *st = u.which ? a.v_stride : a.k_stride;
-  const T *src = (const T *)(u.which ? a.v : a.k);
+  const int r = lane >> 3, c = lane & 7, S = (int)a.S, d = (int)a.d;
+  const int slot = u.slot0 + tok_of(r);
+  const bool live = slot >= u.first && slot < u.end && slot >= 0 && slot < S;
+  const uint64_t on = __ballot(live);
+  if (on == 0) return;
+  const int c0 = u.grp * 64 + 8 * c;
+  const int64_t head = (int64_t)u.b * a.H + u.h;
   uint32_t *codes = (uint32_t *)(u.which ? a.v_codes : a.k_codes);
   uint32_t *par = (uint32_t *)(u.which ? a.v_par : a.k_par);
-  const int64_t head = u.b * a.H + u.h;
-  uint32_t *vword = codes + ((head * (a.S >> 3) + (u.slot0 >> 3)) * a.DP + c0 + r);
+  const T *src = (const T *)(u.which ? a.v : a.k) +
+                 (u.which ? u.b * a.v_stride[0] + u.h * a.v_stride[1]
+                          : u.b * a.k_stride[0] + u.h * a.k_stride[1]);
+  const int64_t step = u.which ? a.v_stride[2] : a.k_stride[2];
 
-  // nibbles of the block that this call stores (the others of the words are kept)
-  uint32_t keep = 0;
-  if (u.which) {
-    const uint64_t on = __ballot(live);
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (live) load8<T, VEC>(x, src + (slot - u.first) * step, c0, d);
+  // a block that this call stores in part: nibbles of the other tokens are kept
+  uint32_t *word_at = u.which ? codes + (head * (S >> 3) + (u.slot0 >> 3)) * a.DP + c0 + r
+                              : codes + (((head * S + slot) * a.DP + c0) >> 3);
+  uint32_t keep = 0xffffffffu, old = 0;
+  if (u.which && on != ~0ull) {
+    keep = 0;
 #pragma unroll
     for (int t = 0; t < 8; ++t)
       if ((on >> (8 * t)) & 1) keep |= 0xfu << (4 * t);
+    old = *word_at;
   }
-  uint32_t old = 0;
-  if (u.which && keep != 0xffffffffu) old = *vword;
 
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (live)
-    load8<T, VEC>(x, src + u.b * st[0] + u.h * st[1] + (slot - u.first) * st[2], c0, a.d);
   float lo = __builtin_inff(), hi = -__builtin_inff(), odd = 0.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e)
-    if (c0 + e < a.d) {
+    if (VEC ? c0 < d : c0 + e < d) {
       lo = fminf(lo, x[e]);
       hi = fmaxf(hi, x[e]);
       odd = fmaf(x[e], 0.f, odd);             // NaN where a value is not finite
@@ -157,38 +165,41 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(Kv4Io a) {
   hi = max8(hi);
   const uint64_t odds = __ballot(!(odd == 0.f));
   const bf16 sb = (bf16)((hi - lo) * (float)(1.0 / 15.0)), mb = (bf16)lo;
-  float s = (float)sb, m = (float)mb;
-  const float largest = 3.4028234663852886e38f;
+  float s = (float)sb;
+  const float m = (float)mb, largest = 3.4028234663852886e38f;
   const bool bad = ((odds >> (lane & 56)) & 0xff) != 0 || !(s <= largest) || !(fabsf(m) <= largest);
-  uint32_t word;
-  if (bad) {
-    word = 0x7fc07fc0u;
-  } else {
-    if (s < 1.1754943508222875e-38f) s = 0.f;
-    word = (uint32_t)__builtin_bit_cast(uint16_t, (bf16)s) |
-           ((uint32_t)__builtin_bit_cast(uint16_t, mb) << 16);
-  }
-  uint32_t n[8];
+  s = s < 1.1754943508222875e-38f ? 0.f : s;
+  uint32_t word = (uint32_t)__builtin_bit_cast(uint16_t, (bf16)s) |
+                  ((uint32_t)__builtin_bit_cast(uint16_t, mb) << 16);
+  if (bad) { word = 0x7fc07fc0u; s = 0.f; }
+  // Codes: (x - m) times the hardware's reciprocal of s, off by less than 1e-5 of a code, and the
+  // true quotient where that is near a half (one value in a thousand of bf16 tensors, where exact
+  // halves occur) or the reciprocal is not a normal number.  Adding 1.5 2^23 rounds to a whole
+  // number in the low bits; what the high bits add up to in the packed word comes off at the end.
+  constexpr float ROUND = 12582912.f;
+  constexpr uint32_t HIGH = 0x4b400000u;
+  const bool plain = s > 1e-36f && s < 1e36f;
+  const float inv = plain ? __builtin_amdgcn_rcpf(s) : 0.f;
+  uint32_t w = 0, high = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float q = (bad || s == 0.f || c0 + e >= a.d) ? 0.f : rintf((x[e] - m) / s);
-    n[e] = (uint32_t)(int)fminf(fmaxf(q, 0.f), 15.f);
+    const float t = x[e] - m;
+    float y = __builtin_amdgcn_fmed3f(t * inv, 0.f, 15.f);
+    float n = y + ROUND;
+    if (fabsf(y - (n - ROUND)) > 0.4999f || (!plain && s > 0.f))
+      n = fminf(fmaxf(t / s, 0.f), 15.f) + ROUND;
+    const int at = u.which ? 4 * e : 4 * ((e >> 1) + 4 * (e & 1));
+    w += __builtin_bit_cast(uint32_t, n) << at;
+    high += HIGH << at;
   }
-  if (u.which == 0) {
-    if (live) {
-      uint32_t w = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w |= n[e] << (4 * ((e >> 1) + 4 * (e & 1)));
-      codes[((head * a.S + slot) * a.DP + c0) >> 3] = w;
-    }
-  } else {
-    uint32_t w = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w |= n[e] << (4 * e);
+  w -= high;
+  if (u.which) {
     w = transpose8(w, r);
-    *vword = (old & ~keep) | (w & keep);
+    *word_at = (old & ~keep) | (w & keep);
+  } else if (live) {
+    *word_at = w;
   }
-  if (live && c == 0) par[((head << a.g_shift) + u.grp) * a.S + slot] = word;
+  if (live && c == 0) par[((head << a.g_shift) + u.grp) * S + slot] = word;
 }
 
 template <typename T, bool VEC>
@@ -196,23 +207,23 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4Io a) {
   const int lane = threadIdx.x & 63;
   const Unit u = unit_of(a);
   if (!u.on) return;
-  const int r = lane >> 3, c = lane & 7;
-  const int64_t slot = u.slot0 + tok_of(r);
+  const int r = lane >> 3, c = lane & 7, S = (int)a.S, d = (int)a.d;
+  const int slot = u.slot0 + tok_of(r);
   const bool wanted = slot >= u.first && slot < u.end;
-  int64_t len = a.length ? load_len(a.length, a.length_dtype, u.b) : a.S;
-  len = len > a.S ? a.S : len;
+  int len = a.length ? bounded(load_len(a.length, a.length_dtype, u.b)) : S;
+  len = len > S ? S : len;
   const bool held = slot >= 0 && slot < len;
-  const int64_t c0 = u.grp * 64 + 8 * c;
-  const int64_t head = u.b * a.H + u.h;
+  const int c0 = u.grp * 64 + 8 * c;
+  const int64_t head = (int64_t)u.b * a.H + u.h;
   const uint32_t *codes = (const uint32_t *)(u.which ? a.v_codes : a.k_codes);
   const uint32_t *par = (const uint32_t *)(u.which ? a.v_par : a.k_par);
   uint32_t w = 0, word = 0;
-  if (held) word = par[((head << a.g_shift) + u.grp) * a.S + slot];
+  if (held) word = par[((head << a.g_shift) + u.grp) * S + slot];
   if (u.which == 0) {
-    if (held) w = codes[((head * a.S + slot) * a.DP + c0) >> 3];
+    if (held) w = codes[((head * S + slot) * a.DP + c0) >> 3];
   } else {
-    if (u.slot0 >= 0 && u.slot0 < a.S)
-      w = codes[(head * (a.S >> 3) + (u.slot0 >> 3)) * a.DP + c0 + r];
+    if (u.slot0 >= 0 && u.slot0 < S)
+      w = codes[(head * (S >> 3) + (u.slot0 >> 3)) * a.DP + c0 + r];
     w = transpose8(w, r);
   }
   if (!wanted) return;
@@ -224,10 +235,12 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4Io a) {
     const int at = u.which ? e : (e >> 1) + 4 * (e & 1);
     x[e] = held ? fmaf((float)((w >> (4 * at)) & 15), s, m) : 0.f;
   }
-  const int64_t *st = u.which ? a.v_stride : a.k_stride;
-  T *out = (T *)(u.which ? a.v : a.k) + u.b * st[0] + u.h * st[1] + (slot - u.first) * st[2];
+  T *out = (T *)(u.which ? a.v : a.k) +
+           (u.which ? u.b * a.v_stride[0] + u.h * a.v_stride[1]
+                    : u.b * a.k_stride[0] + u.h * a.k_stride[1]) +
+           (slot - u.first) * (u.which ? a.v_stride[2] : a.k_stride[2]);
   if (VEC) {
-    if (c0 < a.d) {
+    if (c0 < d) {
       if (sizeof(T) == 2) {
         bf16x8 v;
 #pragma unroll
@@ -241,7 +254,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4Io a) {
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (c0 + e < a.d) out[c0 + e] = from_f32<T>(x[e]);
+      if (c0 + e < d) out[c0 + e] = from_f32<T>(x[e]);
   }
 }
 

@@ -33,8 +33,6 @@
 // one's products are: a code is dequantised out of the register that it was loaded into.
 //
 // Bound by memory: 72 bytes a token and cached head at head dim 64 (256 in bf16).
-#include <type_traits>
-
 #include "common.h"
 #include "kernels.h"
 
@@ -89,8 +87,16 @@ __device__ __forceinline__ float split(float x, bf16 (&part)[PS]) {
   return sum;
 }
 
-template <typename T, int DP, int R>
-__global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a) {
+// Waves a SIMD that the registers are cut for: as many as nothing spills with.
+constexpr int waves_of(bool f32, int DP, int R, bool bias) {
+  if (R <= 4) return f32 ? (DP == 64 ? 3 : 2) : (DP == 64 ? 4 : 3);
+  return f32 ? (DP == 64 || !bias ? 2 : 1) : (DP == 64 || !bias ? 3 : 2);
+}
+
+// BIAS: edge_scores, edge_table or mask given
+template <typename T, int DP, int R, bool BIAS>
+__global__ void __launch_bounds__(256, waves_of(sizeof(T) == 4, DP, R, BIAS))
+kv4_attn_kernel(Kv4Attn a) {
   constexpr int G = DP / 64;             // groups of a token
   constexpr int TT = 128 / G;            // tokens of a tile
   constexpr int NSUB = TT / 32;
@@ -115,7 +121,8 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a) {
   constexpr int P_BYTES = DIRECT ? 0 : G * PS * R * PROW * 2;
   constexpr int PAR_BYTES = OWN_PAR ? 0 : 2 * G * TT * 4;
   constexpr int WAVE_BYTES = (S_BYTES + P_BYTES + PAR_BYTES + 2 * 16 * 4 + 15) / 16 * 16;
-  constexpr int OUT_BYTES = 4 * R * (DP + 2 + G) * 4;
+  constexpr int OROW = DP + 4;
+  constexpr int OUT_BYTES = 4 * R * (OROW + 2 + G) * 4;
   __shared__ __attribute__((aligned(16)))
       unsigned char smem[4 * WAVE_BYTES > OUT_BYTES ? 4 * WAVE_BYTES : OUT_BYTES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -156,7 +163,9 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a) {
     t_begin = (int)split_no * per;
     t_end = t_begin + per < ntiles ? t_begin + per : ntiles;
   }
-  const int sub_last = top > 0 ? (top - 1) / 32 : 0;       // last 32 tokens that are read
+  // last 32 tokens that this workgroup reads (requests past its end go there again)
+  int sub_last = top > 0 ? (top - 1) / 32 : 0;
+  if (t_end * NSUB - 1 < sub_last) sub_last = t_end > 0 ? t_end * NSUB - 1 : 0;
 
   const int64_t head = (int64_t)b * a.H + h;
   const char *kc = (const char *)a.k_codes + head * a.S * KROW;
@@ -173,7 +182,7 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a) {
 #pragma unroll
     for (int s = 0; s < NSUB; ++s) {
       int sub = t * NSUB + s;
-      sub = sub < sub_last ? sub : sub_last;               // (past the end: the last ones again)
+      sub = sub < sub_last ? sub : sub_last;
       const char *base = kc + (int64_t)sub * 32 * KROW;
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk)
@@ -285,11 +294,12 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a) {
   const int vis = row < tile_rows ? seen(qi) : 0;
   const int pos = len - ql + qi;
   const T *edge = nullptr;
-  if (a.edge)
+  const int table_last = (int)a.table_len - 1;
+  if (BIAS && a.edge)
     edge = (const T *)a.edge + b * a.edge_stride[0] + hq * a.edge_stride[1] +
            qi * a.edge_stride[2];
-  const T *table = a.table ? (const T *)a.table + hq * a.table_len : nullptr;
-  const uint8_t *mask = a.mask ? a.mask + b * a.mask_stride[0] + qi * a.mask_stride[1] : nullptr;
+  const T *table = BIAS && a.table ? (const T *)a.table + hq * a.table_len : nullptr;
+  const uint8_t *mask = BIAS && a.mask ? a.mask + b * a.mask_stride[0] + qi * a.mask_stride[1] : nullptr;
 
   // a score from the product without CENTER, for the token of parameters w
   auto scaled = [&](float dot, uint32_t w, int grp) -> float {
@@ -297,18 +307,18 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a) {
     const float c = F32 ? fmaf(7.5f, s, min_of(w)) : min_of(w);
     return fmaf(s, dot, c * qsum[grp]);
   };
+  const int seen_last = vis > 0 ? vis - 1 : 0;             // (loads stay on keys that exist)
   auto finish = [&](float z, int j) -> float {             // bias, scale, mask of key j
     bool on = j < vis;
-    if (edge || table || mask) {
-      if (on) {
-        if (edge) z += to_f32(edge[(int64_t)j * a.edge_stride[3]]);
-        if (table) {
-          int64_t at = a.table_len - 1 - (int64_t)(pos - j);
-          at = at < 0 ? 0 : (at >= a.table_len ? a.table_len - 1 : at);
-          z += to_f32(table[at]);
-        }
-        if (mask) on = mask[(int64_t)j * a.mask_stride[2]] != 0;
+    if (BIAS) {
+      const int jj = j < seen_last ? j : seen_last;
+      if (edge) z += to_f32(edge[(int64_t)jj * a.edge_stride[3]]);
+      if (table) {
+        int at = table_last - pos + jj;
+        at = at < 0 ? 0 : (at > table_last ? table_last : at);
+        z += to_f32(table[at]);
       }
+      if (mask) on = on && mask[(int64_t)jj * a.mask_stride[2]] != 0;
     }
     return on ? z * a.inv_temperature : NEG;
   };
@@ -376,8 +386,7 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a) {
     }
   };
 
-  auto tile = [&](int t, auto more) {
-    constexpr bool MORE = decltype(more)::value;           // another tile follows
+  for (; t < t_end; t += 4) {
     float x[TPL];
     uint32_t vpr[G][OWN_PAR ? TPL : 1], kpr[G][OWN_PAR ? TPL : 1];
 #pragma unroll
@@ -427,7 +436,7 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a) {
           }
         }
       }
-    if (MORE) fetch_k(t + 4);
+    fetch_k(t + 4);
     float most = NEG;
     if (DIRECT) {
 #pragma unroll
@@ -520,12 +529,8 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a) {
           products(s, grp, pb);
         }
     }
-    if (MORE) fetch_v(t + 4);
+    fetch_v(t + 4);
     wave_lds_sync();
-  };
-  if (t < t_end) {
-    for (; t + 4 < t_end; t += 4) tile(t, std::true_type{});
-    tile(t, std::false_type{});
   }
 
   // ---- join the four waves: each row's sum over its lanes, then the waves through LDS ----
@@ -536,14 +541,14 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a) {
     for (int grp = 0; grp < G; ++grp) csum[grp] += __shfl_xor(csum[grp], o, 64);
   }
   __syncthreads();
-  float *jo = (float *)smem;                       // (4, R, DP)
-  float *jm = jo + 4 * R * DP;                     // (4, R, 2 + G): ref, l, csum
+  float *jo = (float *)smem;                       // (4, R, OROW)
+  float *jm = jo + 4 * R * OROW;                    // (4, R, 2 + G): ref, l, csum
   if (col < R) {
 #pragma unroll
     for (int grp = 0; grp < G; ++grp)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        *reinterpret_cast<f32x4 *>(jo + (wave * R + col) * DP + 64 * grp + 16 * g + 4 * e) =
+        *reinterpret_cast<f32x4 *>(jo + (wave * R + col) * OROW + 64 * grp + 16 * g + 4 * e) =
             (f32x4){acc[grp][0][e], acc[grp][1][e], acc[grp][2][e], acc[grp][3][e]};
   }
   if (sl == 0) {
@@ -567,7 +572,7 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a) {
       const float *m = jm + (w * R + orow) * (2 + G);
       const float f = m[0] == mx ? 1.f : __builtin_amdgcn_exp2f((m[0] - mx) * LOG2E);
       sum += f * m[1];
-      o += f * (jo[(w * R + orow) * DP + c] + m[2 + c / 64]);
+      o += f * (jo[(w * R + orow) * OROW + c] + m[2 + c / 64]);
     }
     if (a.splits == 1) {
       const int i = (int)((uint32_t)(row0 + orow) / (uint32_t)a.share);
@@ -586,45 +591,80 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4Attn a) {
   }
 }
 
-// The splits of a row, in order: O = sum_s exp(m_s - M) O_s / sum_s exp(m_s - M) l_s.
+// The splits of a row: O = sum_s exp(m_s - M) O_s / sum_s exp(m_s - M) l_s.  A workgroup takes one
+// row: 256 threads = DP / 4 channel quads x groups of splits, added up in a fixed order.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Attn a) {
   constexpr float LOG2E = 1.4426950408889634f;
-  const int64_t rows = a.B * a.H * a.Lq * a.share;
-  const int64_t row = (int64_t)blockIdx.x * (256 / DP) + threadIdx.x / DP;
-  const int c = threadIdx.x % DP;
-  if (row >= rows || c >= a.d) return;
+  constexpr int Q = DP / 4, GROUPS = 256 / Q;
+  __shared__ float f[KV4_MAX_SPLITS];
+  __shared__ f32x4 part[GROUPS][Q];
+  __shared__ float total;
+  const int64_t row = blockIdx.x;
   const float *ml = a.part_ml + row * a.splits * 2;
-  const float *po = a.part_o + row * a.splits * DP + c;
-  float mx = -__builtin_inff();
-  for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, ml[2 * s]);
-  float sum = 0.f, o = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = ml[2 * s] == mx ? 1.f : __builtin_amdgcn_exp2f((ml[2 * s] - mx) * LOG2E);
-    sum += f * ml[2 * s + 1];
-    o += f * po[(int64_t)s * DP];
+  const f32x4 *po = (const f32x4 *)(a.part_o + row * a.splits * DP);
+  const int q = threadIdx.x % Q, grp = threadIdx.x / Q;
+  f32x4 v[KV4_MAX_SPLITS / GROUPS];
+#pragma unroll
+  for (int k = 0; k < KV4_MAX_SPLITS / GROUPS; ++k) {
+    const int s = grp + k * GROUPS;
+    v[k] = s < a.splits ? po[(int64_t)s * Q + q] : (f32x4){0.f, 0.f, 0.f, 0.f};
   }
-  const int64_t per = a.Lq * a.share, bh = row / per, rr = row - bh * per;
-  const int64_t b = bh / a.H, h = bh - b * a.H, i = rr / a.share;
-  const int64_t hq = h * a.share + rr - i * a.share;
+  if (threadIdx.x < 64) {
+    const int s = threadIdx.x;
+    const float m = s < a.splits ? ml[2 * s] : -__builtin_inff();
+    const float l = s < a.splits ? ml[2 * s + 1] : 0.f;
+    const float mx = wave_max(m);
+    const float w = m == mx ? 1.f : __builtin_amdgcn_exp2f((m - mx) * LOG2E);
+    f[s] = w;
+    const float sum = wave_sum(w * l);
+    if (s == 0) total = sum;
+  }
+  __syncthreads();
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < KV4_MAX_SPLITS / GROUPS; ++k) {
+    const int s = grp + k * GROUPS;
+    if (s < a.splits) {
+      const float w = f[s];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(w, v[k][e], o[e]);
+    }
+  }
+  part[grp][q] = o;
+  __syncthreads();
+  const int c = threadIdx.x;
+  if (c >= a.d) return;
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < GROUPS; ++k) sum += part[k][c / 4][c % 4];
+  const uint32_t per = (uint32_t)(a.Lq * a.share);
+  const uint32_t bh = (uint32_t)row / per, rr = (uint32_t)row - bh * per;
+  const uint32_t b = bh / (uint32_t)a.H, h = bh - b * (uint32_t)a.H, i = rr / (uint32_t)a.share;
+  const int64_t hq = (int64_t)h * a.share + (rr - i * (uint32_t)a.share);
   ((T *)a.out)[b * a.o_stride[0] + hq * a.o_stride[1] + i * a.o_stride[2] + c] =
-      from_f32<T>(sum == 0.f ? 0.f : o / sum);
+      from_f32<T>(total == 0.f ? 0.f : sum / total);
 }
 
-template <typename T, int DP>
-void launch(const Kv4Attn &a, hipStream_t s) {
+template <typename T, int DP, bool BIAS>
+void launch_rows(const Kv4Attn &a, hipStream_t s) {
   const int64_t rows = a.Lq * a.share;
   const dim3 grid((unsigned)(a.B * a.H * a.row_tiles * a.splits)), block(256);
-#define GO(R) hipLaunchKernelGGL((kv4_attn_kernel<T, DP, R>), grid, block, 0, s, a)
+#define GO(R) hipLaunchKernelGGL((kv4_attn_kernel<T, DP, R, BIAS>), grid, block, 0, s, a)
   if (rows > 4) GO(16);
   else if (rows > 2) GO(4);
   else if (rows > 1) GO(2);
   else GO(1);
 #undef GO
+}
+
+template <typename T, int DP>
+void launch(const Kv4Attn &a, hipStream_t s) {
+  if (a.edge || a.table || a.mask) launch_rows<T, DP, true>(a, s);
+  else launch_rows<T, DP, false>(a, s);
   if (a.splits > 1) {
-    const int64_t all = a.B * a.H * rows, per = 256 / DP;
-    hipLaunchKernelGGL((kv4_join_kernel<T, DP>), dim3((unsigned)((all + per - 1) / per)), block, 0,
-                       s, a);
+    const int64_t all = a.B * a.H * a.Lq * a.share;
+    hipLaunchKernelGGL((kv4_join_kernel<T, DP>), dim3((unsigned)all), dim3(256), 0, s, a);
   }
 }
 
@@ -635,7 +675,7 @@ int kv4_attn_plan(int64_t B, int64_t H, int64_t rows, int64_t keys, int64_t d) {
   const int64_t wgs = B * H * ((rows + 15) / 16), most = (keys + 4 * tile - 1) / (4 * tile);
   int64_t n = (1024 + wgs - 1) / wgs;
   n = n > most ? most : n;
-  return (int)(n < 1 ? 1 : (n > 64 ? 64 : n));
+  return (int)(n < 1 ? 1 : (n > KV4_MAX_SPLITS ? KV4_MAX_SPLITS : n));
 }
 
 void launch_kv4_attn(const Kv4Attn &a, int dtype, hipStream_t s) {
