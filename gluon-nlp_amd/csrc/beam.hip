@@ -83,6 +83,26 @@ __device__ __forceinline__ float all_sum(float x) {
   return lane63(x);
 }
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_or_zero(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ double all_sum(double x) {
+  x += dpp_or_zero<0x111, 0xf>(x);
+  x += dpp_or_zero<0x112, 0xf>(x);
+  x += dpp_or_zero<0x114, 0xf>(x);
+  x += dpp_or_zero<0x118, 0xf>(x);
+  x += dpp_or_zero<0x142, 0xa>(x);
+  x += dpp_or_zero<0x143, 0xc>(x);
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, 63);
+  const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 63);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+
 // a bound, of the high bits of the keys down to LOW, that at least K of the wave's 64 keys reach (0
 // if fewer than K are above 0)
 template <int LOW>
@@ -100,9 +120,15 @@ __device__ __forceinline__ bool better(float x, uint32_t i, float y, uint32_t j)
   return x > y || (x == y && i < j);
 }
 
+// p[i] by way of its aligned word: a scalar load, the same in all lanes
+__device__ __forceinline__ bool flag_at(const uint8_t *p, int64_t i) {
+  const uintptr_t at = (uintptr_t)(p + i);
+  return (*reinterpret_cast<const uint32_t *>(at & ~(uintptr_t)3) >> (8 * (at & 3))) & 0xff;
+}
+
 // E: values of a thread
 template <typename T, bool VEC, int E>
-__global__ void __launch_bounds__(256) beam_chunk_kernel(BeamSelect a) {
+__global__ void __launch_bounds__(256, E == 32 && !VEC ? 4 : 8) beam_chunk_kernel(BeamSelect a) {
   __shared__ uint64_t list[CAP];           // ordered value above, complement of the index below
   __shared__ uint32_t sh_n, sh_bound[4];
   __shared__ float sh_m[4], sh_s[4];
@@ -110,7 +136,7 @@ __global__ void __launch_bounds__(256) beam_chunk_kernel(BeamSelect a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t row = blockIdx.y;
   const uint32_t chunk = blockIdx.x, base = chunk * (256 * E), V = (uint32_t)a.V;
-  if (a.finished && a.finished[row]) return;
+  if (a.finished && flag_at(a.finished, row)) return;
   const bool dead = !(a.scores[row] > -1e15f);
   const T *src = (const T *)a.outputs + row * a.row_stride;
   if (tid == 0) sh_n = 0;
@@ -120,17 +146,16 @@ __global__ void __launch_bounds__(256) beam_chunk_kernel(BeamSelect a) {
   auto at = [&](int e) -> uint32_t { return base + (e / PER) * (256 * PER) + tid * PER + e % PER; };
   float x[E];
   const bool whole = base + 256 * E <= V;
+  if (VEC && whole) {
+    typename VecOf<T>::type w[E / PER];
 #pragma unroll
-  for (int v = 0; v < E / PER; ++v) {
-    const uint32_t i = at(v * PER);
-    if (VEC) {
-      typename VecOf<T>::type w;
-      if (whole || i < V) w = *reinterpret_cast<const typename VecOf<T>::type *>(src + i);
+    for (int v = 0; v < E / PER; ++v)
+      w[v] = *reinterpret_cast<const typename VecOf<T>::type *>(src + at(v * PER));
 #pragma unroll
-      for (int e = 0; e < PER; ++e) x[v * PER + e] = whole || i < V ? to_f32((T)w[e]) : NEG;
-    } else {
-      x[v] = whole || i < V ? to_f32(src[i]) : NEG;
-    }
+    for (int e = 0; e < E; ++e) x[e] = to_f32((T)w[e / PER][e % PER]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = at(e) < V ? to_f32(src[at(e)]) : NEG;
   }
   float most = NEG;
 #pragma unroll
@@ -256,21 +281,36 @@ __global__ void __launch_bounds__(MERGE) beam_merge_kernel(BeamSelect a) {
   // finished beam, its own only candidate
   const uint32_t own = K * a.chunks, lists = own + K;
   if (tid == 0) { sh_n = 0; sh_live = 0; }
+  // the lists' best candidates, requested before anything waits
+  constexpr int AHEAD = 2;
+  int32_t hv[AHEAD];
+  float hz[AHEAD];
+#pragma unroll
+  for (int r = 0; r < AHEAD; ++r) {
+    const uint32_t c = tid + r * MERGE;
+    hv[r] = -1;
+    hz[r] = NEG;
+    if (c < own) {
+      hv[r] = a.cand_i[(first + c) * K];
+      hz[r] = a.cand_x[(first + c) * K];
+    }
+  }
   // ---- logsumexp of each beam from its chunks ----
   for (int k = wave; k < K; k += WAVES) {
     double out = 0;
     float m = 0.f;
     if (a.normalize && !(fin && fin[k])) {
       const float *st = a.stats + (first + k * a.chunks) * 2;
-      m = NEG;
-      for (uint32_t c = lane; c < a.chunks; c += 64) m = fmaxf(m, st[2 * c]);
+      const uint32_t c0 = lane;
+      const float m0 = c0 < a.chunks ? st[2 * c0] : NEG, t0 = c0 < a.chunks ? st[2 * c0 + 1] : 0.f;
+      m = m0;
+      for (uint32_t c = lane + 64; c < a.chunks; c += 64) m = fmaxf(m, st[2 * c]);
       m = all_max(m);
-      double t = 0;
-      for (uint32_t c = lane; c < a.chunks; c += 64)
+      double t = m0 > NEG ? (double)(t0 * __builtin_amdgcn_exp2f((m0 - m) * a.exp_scale)) : 0.0;
+      for (uint32_t c = lane + 64; c < a.chunks; c += 64)
         if (st[2 * c] > NEG)
-          t += (double)st[2 * c + 1] * exp(((double)st[2 * c] - (double)m) * a.inv_temperature);
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+          t += (double)(st[2 * c + 1] * __builtin_amdgcn_exp2f((st[2 * c] - m) * a.exp_scale));
+      t = all_sum(t);
       if (m > NEG) out = log(t);
       else m = 0.f;
     }
@@ -287,9 +327,10 @@ __global__ void __launch_bounds__(MERGE) beam_merge_kernel(BeamSelect a) {
   }
   const double per_lp = 1.0 / lp_new;
   __syncthreads();
-  const int64_t none = 0x7fffffffffffffffLL, KV = (int64_t)K * a.V;
-  // candidate j of list c -> score and index (index `none`: there is no such candidate)
-  auto get = [&](uint32_t c, int j, double &x, int64_t &i) {
+  // an index: beam above, token below (finished beams: K above, beam below), in the order of k V + v
+  const int64_t none = 0x7fffffffffffffffLL;
+  // candidate (token v, logit z) of list c -> score and index (index `none`: there is none)
+  auto rate = [&](uint32_t c, int32_t v, float z, double &x, int64_t &i) {
     x = -__builtin_inf();
     i = none;
     const bool self = c >= own;
@@ -298,26 +339,41 @@ __global__ void __launch_bounds__(MERGE) beam_merge_kernel(BeamSelect a) {
     const float prev = prevs[k];
     const bool dead = !(prev > -1e15f);
     if (self) {
-      if (done && j == 0) {
-        i = KV + k;
+      if (done) {
+        i = ((int64_t)K << 32) | k;
         if (!dead) x = (double)prev;
       }
-    } else if (!done) {
-      const int64_t at = (first + c) * K + j;
-      const int32_t v = a.cand_i[at];
-      const float z = a.cand_x[at];
-      if (v >= 0) {
-        i = (int64_t)k * a.V + v;
-        if (z > NEG && !dead)
-          x = ((double)prev * lp_prev +
-               (((double)z - (double)peak[k]) * a.inv_temperature - lse[k])) * per_lp;
-      }
+    } else if (!done && v >= 0) {
+      i = ((int64_t)k << 32) | (uint32_t)v;
+      if (z > NEG && !dead)
+        x = ((double)prev * lp_prev +
+             (((double)z - (double)peak[k]) * a.inv_temperature - lse[k])) * per_lp;
     }
   };
+  auto get = [&](uint32_t c, int j, double &x, int64_t &i) {
+    int32_t v = -1;
+    float z = NEG;
+    if (c < own) {
+      v = a.cand_i[(first + c) * K + j];
+      z = a.cand_x[(first + c) * K + j];
+    }
+    rate(c, v, z, x, i);
+    if (c >= own && j > 0) i = none;
+  };
   // ---- a bound that K lists' best candidates reach ----
-  double mx = -__builtin_inf();
-  bool any = false;
-  for (uint32_t c = tid; c < lists; c += MERGE) {
+  double mx = -__builtin_inf(), hx[AHEAD];
+  bool any = false, has[AHEAD];
+#pragma unroll
+  for (int r = 0; r < AHEAD; ++r) {
+    const uint32_t c = tid + r * MERGE;
+    int64_t i = none;
+    hx[r] = -__builtin_inf();
+    if (c < lists) rate(c, hv[r], hz[r], hx[r], i);
+    has[r] = i != none;
+    any |= has[r];
+    mx = fmax(mx, hx[r]);
+  }
+  for (uint32_t c = tid + AHEAD * MERGE; c < lists; c += MERGE) {
     double x;
     int64_t i;
     get(c, 0, x, i);
@@ -331,14 +387,19 @@ __global__ void __launch_bounds__(MERGE) beam_merge_kernel(BeamSelect a) {
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) least = max(least, sh_bound[w]);
   // ---- the lists whose best candidate reaches it, then all of their candidates at once ----
-  for (uint32_t c = tid; c < lists; c += MERGE) {
-    double x;
-    int64_t i;
-    get(c, 0, x, i);
-    if (i != none && (uint32_t)(ordered(x) >> 32) >= least) {
+  auto keep = [&](uint32_t c, double x, bool is) {
+    if (is && (uint32_t)(ordered(x) >> 32) >= least) {
       const uint32_t pos = atomicAdd(&sh_live, 1u);
       if (pos < LIST) live[pos] = c;
     }
+  };
+#pragma unroll
+  for (int r = 0; r < AHEAD; ++r) keep(tid + r * MERGE, hx[r], has[r]);
+  for (uint32_t c = tid + AHEAD * MERGE; c < lists; c += MERGE) {
+    double x;
+    int64_t i;
+    get(c, 0, x, i);
+    keep(c, x, i != none);
   }
   __syncthreads();
   const uint32_t nlive = sh_live;
@@ -357,11 +418,11 @@ __global__ void __launch_bounds__(MERGE) beam_merge_kernel(BeamSelect a) {
   const uint32_t found = sh_n;
   auto put = [&](int rank, double x, int64_t i) {
     const int64_t to = item * K + rank;
-    const bool was = i >= KV;
-    const int64_t k = was ? i - KV : i / a.V, v = was ? -1 : i - k * a.V;
+    const bool was = (i >> 32) == K;
+    const int32_t k = was ? (int32_t)i : (int32_t)(i >> 32), v = was ? -1 : (int32_t)i;
     a.out_scores[to] = (float)x;
-    a.out_parents[to] = (int32_t)k;
-    a.out_tokens[to] = (int32_t)v;
+    a.out_parents[to] = k;
+    a.out_tokens[to] = v;
     a.out_finished[to] = was || (a.has_eos && v == a.eos);
   };
   if (nlive <= LIST && found <= LIST) {
@@ -538,20 +599,21 @@ __global__ void __launch_bounds__(256) reorder_kernel(Reorder a) {
 
 }  // namespace
 
-// Values of a thread: 32 where that still gives every CU a few workgroups, 16 otherwise
-// (256 rows of 32128 float32 logits: MEASURED; 4 rows: MEASURED).
-static int chunk_values(int64_t rows, int64_t V) {
-  return rows * ((V + 8191) / 8192) >= 1024 ? 32 : 16;
+// Values of a thread: 64 bytes, 32 of bfloat16 where that still gives every CU a few workgroups.
+// (128 rows of 250112 bfloat16 logits: 24 us, 27 with 16; 512 rows of 32128 float32: 17 us with 16
+// and with 32; 4 rows of 32128: 5.2 us with 16, 6.3 with 32.)
+static int chunk_values(int64_t rows, int64_t V, int dtype) {
+  return dtype == GNLP_BF16 && rows * ((V + 8191) / 8192) >= 1024 ? 32 : 16;
 }
 
-size_t beam_workspace_bytes(int64_t rows, int64_t V, int K) {
-  const int64_t ch = 256 * chunk_values(rows, V), slots = rows * ((V + ch - 1) / ch);
+size_t beam_workspace_bytes(int64_t rows, int64_t V, int K) {     // for either dtype
+  const int64_t ch = 256 * chunk_values(rows, V, GNLP_F32), slots = rows * ((V + ch - 1) / ch);
   return (size_t)slots * (8 + 8 * (size_t)K);
 }
 
 void launch_beam_select(BeamSelect a, int64_t items, int dtype, void *ws, hipStream_t s) {
   const int64_t rows = items * a.K;
-  const int values = chunk_values(rows, a.V);
+  const int values = chunk_values(rows, a.V, dtype);
   a.chunks = (uint32_t)((a.V + 256 * values - 1) / (256 * values));
   a.stats = (float *)ws;
   a.cand_x = a.stats + rows * a.chunks * 2;
@@ -568,8 +630,7 @@ void launch_beam_select(BeamSelect a, int64_t items, int dtype, void *ws, hipStr
     if (values == 32) GO(bf16, 32);
     else GO(bf16, 16);
   } else {
-    if (values == 32) GO(float, 32);
-    else GO(float, 16);
+    GO(float, 16);
   }
 #undef GO
   hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)items), dim3(MERGE), 0, s, a);

@@ -22,6 +22,8 @@
 // Both kernels: a wave = one (batch, head, group, block of 8 slots) of K or V; lane 8 r + c holds
 // channels 8 c .. 8 c + 7 of token tok(r).  V goes through an 8 x 8 nibble transpose over the r
 // lanes in three exchange steps.  Bound by memory: 2 or 4 bytes a value in (out), 0.5625 out (in).
+// For long writes and reads a wave takes four consecutive blocks and requests all their values
+// before it waits: with one block (1 KB of bf16) a wave there are too few requests in flight.
 #include "common.h"
 #include "kernels.h"
 
@@ -60,7 +62,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t w, int r) {
                  : (w & 0x0f0f0f0fu) | ((p & 0x0f0f0f0fu) << 4);
 }
 
-struct Unit {      // what a wave works on
+struct Unit {      // what a wave works on: the blocks of 8 slots from slot0 on
   int b, h, grp, which;              // which: 0 = K, 1 = V
   int slot0, first, end;             // slot0: the block's first slot; [first, end): the call's slots
   bool on;
@@ -73,6 +75,7 @@ __device__ __forceinline__ int bounded(int64_t n) {
 
 // grid: x = (block of slots, head, group), four waves a workgroup; y = sequence; z = K or V.  Heads
 // run fastest: neighbouring waves read neighbouring rows of an (N, T, H, d) tensor.
+template <int UN>
 __device__ __forceinline__ Unit unit_of(const Kv4Io &a) {
   Unit u;
   const uint32_t w = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -92,176 +95,200 @@ __device__ __forceinline__ Unit unit_of(const Kv4Io &a) {
     u.end = u.first > 0x7fffffff - L ? 0x7fffffff : u.first + L;
   }
   // blocks of 8 slots, counted from the first slot's (also below slot 0, where nothing is held)
-  u.on = blk < a.nblk && blk <= (uint32_t)((0x7ffffff0 - u.first) >> 3);
-  u.slot0 = (int)((u.first & ~7) + (u.on ? 8 * blk : 0));
-  u.on = u.on && u.slot0 < u.end;
+  u.on = blk * UN < a.nblk;
+  const int64_t slot0 = (int64_t)(u.first & ~7) + 8 * UN * (int64_t)blk;
+  u.on = u.on && slot0 < u.end;
+  u.slot0 = u.on ? (int)slot0 : 0;
   return u;
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(float (&x)[8], const T *p, int c0, int d) {
-  if (VEC) {
-    if (c0 < d) {
-      if (sizeof(T) == 2) {
-        const bf16x8 v = *reinterpret_cast<const bf16x8 *>(p + c0);
+// 8 channels of a token, as they were loaded (0 where nothing was)
+template <typename T, bool VEC> struct Values {
+  typedef typename VecOf<T>::type V;
+  static constexpr int N = VecOf<T>::N;
+  V v[8 / N];
+  __device__ __forceinline__ void load(bool live, const T *p, int c0, int d) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = (float)v[e];
+    for (int i = 0; i < 8 / N; ++i) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[i][e] = (T)0.f;
+      if (VEC) {
+        if (live && c0 < d) v[i] = *reinterpret_cast<const V *>(p + c0 + i * N);
       } else {
-        const f32x4 v = *reinterpret_cast<const f32x4 *>(p + c0);
-        const f32x4 w = *reinterpret_cast<const f32x4 *>(p + c0 + 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { x[e] = v[e]; x[4 + e] = w[e]; }
+        for (int e = 0; e < N; ++e)
+          if (live && c0 + i * N + e < d) v[i][e] = p[c0 + i * N + e];
       }
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (c0 + e < d) x[e] = to_f32(p[c0 + e]);
   }
-}
+  __device__ __forceinline__ float get(int e) const { return to_f32((T)v[e / N][e % N]); }
+};
 
-template <typename T, bool VEC>
+template <typename T, bool VEC, int UN>
 __global__ void __launch_bounds__(256) kv4_write_kernel(Kv4Io a) {
   const int lane = threadIdx.x & 63;
-  const Unit u = unit_of(a);
+  const Unit u = unit_of<UN>(a);
   if (!u.on) return;
   const int r = lane >> 3, c = lane & 7, S = (int)a.S, d = (int)a.d;
-  const int slot = u.slot0 + tok_of(r);
-  const bool live = slot >= u.first && slot < u.end && slot >= 0 && slot < S;
-  const uint64_t on = __ballot(live);
-  if (on == 0) return;
   const int c0 = u.grp * 64 + 8 * c;
   const int64_t head = (int64_t)u.b * a.H + u.h;
   uint32_t *codes = (uint32_t *)(u.which ? a.v_codes : a.k_codes);
-  uint32_t *par = (uint32_t *)(u.which ? a.v_par : a.k_par);
+  uint32_t *par = (uint32_t *)(u.which ? a.v_par : a.k_par) + ((head << a.g_shift) + u.grp) * S;
   const T *src = (const T *)(u.which ? a.v : a.k) +
                  (u.which ? u.b * a.v_stride[0] + u.h * a.v_stride[1]
                           : u.b * a.k_stride[0] + u.h * a.k_stride[1]);
   const int64_t step = u.which ? a.v_stride[2] : a.k_stride[2];
-
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (live) load8<T, VEC>(x, src + (slot - u.first) * step, c0, d);
-  // a block that this call stores in part: nibbles of the other tokens are kept
-  uint32_t *word_at = u.which ? codes + (head * (S >> 3) + (u.slot0 >> 3)) * a.DP + c0 + r
-                              : codes + (((head * S + slot) * a.DP + c0) >> 3);
-  uint32_t keep = 0xffffffffu, old = 0;
-  if (u.which && on != ~0ull) {
-    keep = 0;
+  Values<T, VEC> in[UN];
 #pragma unroll
-    for (int t = 0; t < 8; ++t)
-      if ((on >> (8 * t)) & 1) keep |= 0xfu << (4 * t);
-    old = *word_at;
+  for (int k = 0; k < UN; ++k) {
+    const int slot = u.slot0 + 8 * k + tok_of(r);
+    in[k].load(slot >= u.first && slot < u.end && slot >= 0 && slot < S,
+               src + (slot - u.first) * step, c0, d);
   }
-
-  float lo = __builtin_inff(), hi = -__builtin_inff(), odd = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (VEC ? c0 < d : c0 + e < d) {
-      lo = fminf(lo, x[e]);
-      hi = fmaxf(hi, x[e]);
+  for (int k = 0; k < UN; ++k) {
+    const int block = u.slot0 + 8 * k, slot = block + tok_of(r);
+    const bool live = slot >= u.first && slot < u.end && slot >= 0 && slot < S;
+    const uint64_t on = __ballot(live);
+    if (on == 0) continue;
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = in[k].get(e);
+    // a block that this call stores in part: nibbles of the other tokens are kept
+    uint32_t *word_at = u.which ? codes + (head * (S >> 3) + (block >> 3)) * a.DP + c0 + r
+                                : codes + (((head * S + slot) * a.DP + c0) >> 3);
+    uint32_t keep = 0xffffffffu, old = 0;
+    if (u.which && on != ~0ull) {
+      keep = 0;
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+        if ((on >> (8 * t)) & 1) keep |= 0xfu << (4 * t);
+      old = *word_at;
+    }
+
+    float lo = x[0], hi = x[0], odd = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (VEC || c0 + e < d) {
+        lo = fminf(lo, x[e]);
+        hi = fmaxf(hi, x[e]);
+      }
       odd = fmaf(x[e], 0.f, odd);             // NaN where a value is not finite
     }
-  lo = min8(lo);
-  hi = max8(hi);
-  const uint64_t odds = __ballot(!(odd == 0.f));
-  const bf16 sb = (bf16)((hi - lo) * (float)(1.0 / 15.0)), mb = (bf16)lo;
-  float s = (float)sb;
-  const float m = (float)mb, largest = 3.4028234663852886e38f;
-  const bool bad = ((odds >> (lane & 56)) & 0xff) != 0 || !(s <= largest) || !(fabsf(m) <= largest);
-  s = s < 1.1754943508222875e-38f ? 0.f : s;
-  uint32_t word = (uint32_t)__builtin_bit_cast(uint16_t, (bf16)s) |
-                  ((uint32_t)__builtin_bit_cast(uint16_t, mb) << 16);
-  if (bad) { word = 0x7fc07fc0u; s = 0.f; }
-  // Codes: (x - m) times the hardware's reciprocal of s, off by less than 1e-5 of a code, and the
-  // true quotient where that is near a half (one value in a thousand of bf16 tensors, where exact
-  // halves occur) or the reciprocal is not a normal number.  Adding 1.5 2^23 rounds to a whole
-  // number in the low bits; what the high bits add up to in the packed word comes off at the end.
-  constexpr float ROUND = 12582912.f;
-  constexpr uint32_t HIGH = 0x4b400000u;
-  const bool plain = s > 1e-36f && s < 1e36f;
-  const float inv = plain ? __builtin_amdgcn_rcpf(s) : 0.f;
-  uint32_t w = 0, high = 0;
+    if (c0 >= d) { lo = __builtin_inff(); hi = -__builtin_inff(); }   // (no channel of the head)
+    lo = min8(lo);
+    hi = max8(hi);
+    const uint64_t odds = __ballot(!(odd == 0.f));
+    const bf16 sb = (bf16)((hi - lo) * (float)(1.0 / 15.0)), mb = (bf16)lo;
+    float s = (float)sb;
+    const float m = (float)mb, largest = 3.4028234663852886e38f;
+    const bool bad = ((odds >> (lane & 56)) & 0xff) != 0 || !(s <= largest) ||
+                     !(fabsf(m) <= largest);
+    s = s < 1.1754943508222875e-38f ? 0.f : s;
+    uint32_t word = (uint32_t)__builtin_bit_cast(uint16_t, (bf16)s) |
+                    ((uint32_t)__builtin_bit_cast(uint16_t, mb) << 16);
+    if (bad) { word = 0x7fc07fc0u; s = 0.f; }
+    // The quotient (x - m) / s, rounded as a division rounds it: the residual of an approximate
+    // quotient is exact in one fma, another corrects it (exact halves, which a few in a hundred
+    // bf16 values are, stay exact).  Outside the range where reciprocal and residual are normal
+    // numbers: the division.  Adding 1.5 2^23 rounds to a whole number in the low bits; what the
+    // high bits add up to in the packed word comes off at the end.
+    constexpr float ROUND = 12582912.f;
+    constexpr uint32_t HIGH = 0x4b400000u;
+    float inv = __builtin_amdgcn_rcpf(s);
+    inv = fmaf(fmaf(-s, inv, 1.f), inv, inv);
+    const bool flat = s == 0.f, plain = s > 1e-30f && s < 1e30f;
+    if (flat) { inv = 0.f; }
+    const bool exact = __any(!flat && !plain);
+    uint32_t w = 0, high = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float t = x[e] - m;
-    float y = __builtin_amdgcn_fmed3f(t * inv, 0.f, 15.f);
-    float n = y + ROUND;
-    if (fabsf(y - (n - ROUND)) > 0.4999f || (!plain && s > 0.f))
-      n = fminf(fmaxf(t / s, 0.f), 15.f) + ROUND;
-    const int at = u.which ? 4 * e : 4 * ((e >> 1) + 4 * (e & 1));
-    w += __builtin_bit_cast(uint32_t, n) << at;
-    high += HIGH << at;
+    for (int e = 0; e < 8; ++e) {
+      const float t = x[e] - m;
+      float y = t * inv;
+      y = fmaf(fmaf(-y, s, t), inv, y);
+      if (exact && !flat && !plain) y = t / s;
+      const float n = __builtin_amdgcn_fmed3f(y, 0.f, 15.f) + ROUND;
+      const int at = u.which ? 4 * e : 4 * ((e >> 1) + 4 * (e & 1));
+      w += __builtin_bit_cast(uint32_t, n) << at;
+      high += HIGH << at;
+    }
+    w -= high;
+    if (u.which) {
+      w = transpose8(w, r);
+      *word_at = (old & ~keep) | (w & keep);
+    } else if (live) {
+      *word_at = w;
+    }
+    if (live && c == 0) par[slot] = word;
   }
-  w -= high;
-  if (u.which) {
-    w = transpose8(w, r);
-    *word_at = (old & ~keep) | (w & keep);
-  } else if (live) {
-    *word_at = w;
-  }
-  if (live && c == 0) par[((head << a.g_shift) + u.grp) * S + slot] = word;
 }
 
-template <typename T, bool VEC>
+template <typename T, bool VEC, int UN>
 __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4Io a) {
   const int lane = threadIdx.x & 63;
-  const Unit u = unit_of(a);
+  const Unit u = unit_of<UN>(a);
   if (!u.on) return;
   const int r = lane >> 3, c = lane & 7, S = (int)a.S, d = (int)a.d;
-  const int slot = u.slot0 + tok_of(r);
-  const bool wanted = slot >= u.first && slot < u.end;
   int len = a.length ? bounded(load_len(a.length, a.length_dtype, u.b)) : S;
   len = len > S ? S : len;
-  const bool held = slot >= 0 && slot < len;
   const int c0 = u.grp * 64 + 8 * c;
   const int64_t head = (int64_t)u.b * a.H + u.h;
   const uint32_t *codes = (const uint32_t *)(u.which ? a.v_codes : a.k_codes);
-  const uint32_t *par = (const uint32_t *)(u.which ? a.v_par : a.k_par);
-  uint32_t w = 0, word = 0;
-  if (held) word = par[((head << a.g_shift) + u.grp) * S + slot];
-  if (u.which == 0) {
-    if (held) w = codes[((head * S + slot) * a.DP + c0) >> 3];
-  } else {
-    if (u.slot0 >= 0 && u.slot0 < S)
-      w = codes[(head * (S >> 3) + (u.slot0 >> 3)) * a.DP + c0 + r];
-    w = transpose8(w, r);
-  }
-  if (!wanted) return;
-  const float s = __builtin_bit_cast(float, word << 16);
-  const float m = __builtin_bit_cast(float, word & 0xffff0000u);
-  float x[8];
+  const uint32_t *par =
+      (const uint32_t *)(u.which ? a.v_par : a.k_par) + ((head << a.g_shift) + u.grp) * S;
+  uint32_t w[UN], word[UN];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int at = u.which ? e : (e >> 1) + 4 * (e & 1);
-    x[e] = held ? fmaf((float)((w >> (4 * at)) & 15), s, m) : 0.f;
+  for (int k = 0; k < UN; ++k) {
+    const int block = u.slot0 + 8 * k, slot = block + tok_of(r);
+    w[k] = word[k] = 0;
+    if (slot >= 0 && slot < len) word[k] = par[slot];
+    if (block >= 0 && block < len)
+      w[k] = codes[u.which ? (head * (S >> 3) + (block >> 3)) * a.DP + c0 + r
+                           : ((head * S + slot) * a.DP + c0) >> 3];
   }
-  T *out = (T *)(u.which ? a.v : a.k) +
-           (u.which ? u.b * a.v_stride[0] + u.h * a.v_stride[1]
-                    : u.b * a.k_stride[0] + u.h * a.k_stride[1]) +
-           (slot - u.first) * (u.which ? a.v_stride[2] : a.k_stride[2]);
-  if (VEC) {
-    if (c0 < d) {
-      if (sizeof(T) == 2) {
-        bf16x8 v;
+  T *out0 = (T *)(u.which ? a.v : a.k) +
+            (u.which ? u.b * a.v_stride[0] + u.h * a.v_stride[1]
+                     : u.b * a.k_stride[0] + u.h * a.k_stride[1]);
+  const int64_t step = u.which ? a.v_stride[2] : a.k_stride[2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (bf16)x[e];
-        *reinterpret_cast<bf16x8 *>(out + c0) = v;
-      } else {
-        *reinterpret_cast<f32x4 *>(out + c0) = (f32x4){x[0], x[1], x[2], x[3]};
-        *reinterpret_cast<f32x4 *>(out + c0 + 4) = (f32x4){x[4], x[5], x[6], x[7]};
-      }
+  for (int k = 0; k < UN; ++k) {
+    const int slot = u.slot0 + 8 * k + tok_of(r);
+    if (u.which) w[k] = transpose8(w[k], r);
+    if (slot < u.first || slot >= u.end) continue;
+    const bool held = slot >= 0 && slot < len;
+    const float s = __builtin_bit_cast(float, word[k] << 16);
+    const float m = __builtin_bit_cast(float, word[k] & 0xffff0000u);
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int at = u.which ? 4 * e : 4 * ((e >> 1) + 4 * (e & 1));
+      x[e] = held ? fmaf((float)((w[k] >> at) & 15), s, m) : 0.f;
     }
-  } else {
+    T *out = out0 + (slot - u.first) * step;
+    if (VEC) {
+      if (c0 < d) {
+        typedef typename VecOf<T>::type V;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (c0 + e < d) out[c0 + e] = from_f32<T>(x[e]);
+        for (int i = 0; i < 8 / VecOf<T>::N; ++i) {
+          V v;
+#pragma unroll
+          for (int e = 0; e < VecOf<T>::N; ++e) v[e] = from_f32<T>(x[i * VecOf<T>::N + e]);
+          *reinterpret_cast<V *>(out + c0 + i * VecOf<T>::N) = v;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c0 + e < d) out[c0 + e] = from_f32<T>(x[e]);
+    }
   }
 }
 
 }  // namespace
 
 void launch_kv4_io(const Kv4Io &a, int dtype, hipStream_t s) {
-  const int64_t waves = ((int64_t)a.nblk * a.H) << a.g_shift;
+  const int un = a.nblk >= 8 ? 4 : 1;
+  const int64_t waves = ((int64_t)((a.nblk + un - 1) / un) * a.H) << a.g_shift;
   const dim3 grid((unsigned)((waves + 3) / 4), (unsigned)a.B, 2), block(256);
   // 16-byte accesses need whole 8-channel pieces at 16-byte aligned places
   auto aligned = [&](const void *p, const int64_t *st) {
@@ -269,19 +296,25 @@ void launch_kv4_io(const Kv4Io &a, int dtype, hipStream_t s) {
     return ((uintptr_t)p & 15) == 0 && st[0] % per == 0 && st[1] % per == 0 && st[2] % per == 0;
   };
   const bool vec = a.d % 8 == 0 && aligned(a.k, a.k_stride) && aligned(a.v, a.v_stride);
+#define GO3(KERNEL, T, VEC) \
+  do { \
+    if (un == 4) hipLaunchKernelGGL((KERNEL<T, VEC, 4>), grid, block, 0, s, a); \
+    else hipLaunchKernelGGL((KERNEL<T, VEC, 1>), grid, block, 0, s, a); \
+  } while (0)
 #define GO(KERNEL) \
   do { \
     if (dtype == GNLP_BF16) { \
-      if (vec) hipLaunchKernelGGL((KERNEL<bf16, true>), grid, block, 0, s, a); \
-      else hipLaunchKernelGGL((KERNEL<bf16, false>), grid, block, 0, s, a); \
+      if (vec) GO3(KERNEL, bf16, true); \
+      else GO3(KERNEL, bf16, false); \
     } else { \
-      if (vec) hipLaunchKernelGGL((KERNEL<float, true>), grid, block, 0, s, a); \
-      else hipLaunchKernelGGL((KERNEL<float, false>), grid, block, 0, s, a); \
+      if (vec) GO3(KERNEL, float, true); \
+      else GO3(KERNEL, float, false); \
     } \
   } while (0)
   if (a.write) GO(kv4_write_kernel);
   else GO(kv4_read_kernel);
 #undef GO
+#undef GO3
 }
 
 }  // namespace gnlp
