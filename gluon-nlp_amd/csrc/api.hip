@@ -1848,6 +1848,8 @@ int gnlp_kv4_attn(void *ctx, const void *q, const gnlp_kv4_cache *cache,
   const int64_t rows = d->Lq * d->share;
   a.row_tiles = (int)((rows + 15) / 16);
   a.splits = kv4_splits(cache, d);
+  const int64_t round = 4 * (cache->d > 64 ? 64 : 128);      // tokens that four waves take at once
+  a.ahead = a.splits == 1 && d->keys >= round && cache->slots >= round;
   REQUIRE(cache->B * cache->H * a.row_tiles * a.splits < (1LL << 31) &&
               cache->B * cache->H * rows < (1LL << 31), "4-bit attention: too many workgroups");
   if (a.splits > 1) {

@@ -330,6 +330,7 @@ struct Kv4Attn {
   int64_t Lm;                         // keys that edge and mask reach (S when neither is given)
   float inv_temperature;
   int row_tiles, splits;
+  int ahead;                          // the first tiles are requested before the lengths are known
   float *part_o, *part_ml;            // splits > 1: (row, split, DP) and (row, split, 2) in float
 };
 constexpr int KV4_MAX_SPLITS = 64;    // (a wave of the join holds one each)

@@ -200,14 +200,23 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(Kv4Io a) {
     const bool flat = s == 0.f, plain = s > 1e-30f && s < 1e30f;
     if (flat) { inv = 0.f; }
     const bool exact = __any(!flat && !plain);
-    uint32_t w = 0, high = 0;
+    float y[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float t = x[e] - m;
-      float y = t * inv;
-      y = fmaf(fmaf(-y, s, t), inv, y);
-      if (exact && !flat && !plain) y = t / s;
-      const float n = __builtin_amdgcn_fmed3f(y, 0.f, 15.f) + ROUND;
+      y[e] = t * inv;
+      y[e] = fmaf(fmaf(-y[e], s, t), inv, y[e]);
+    }
+    if (exact) {
+      asm volatile("");                       // (a branch: not to be computed ahead)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (!flat && !plain) y[e] = (x[e] - m) / s;
+    }
+    uint32_t w = 0, high = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float n = __builtin_amdgcn_fmed3f(y[e], 0.f, 15.f) + ROUND;
       const int at = u.which ? 4 * e : 4 * ((e >> 1) + 4 * (e & 1));
       w += __builtin_bit_cast(uint32_t, n) << at;
       high += HIGH << at;

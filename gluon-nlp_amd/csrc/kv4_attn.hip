@@ -11,11 +11,11 @@
 // 16 .. 32); the 16 comes off in the epilogue, q . n = q . (16 + n) - 16 sum(q).
 //
 // Roundings: bf16 queries are exact operands, float32 ones are split into three bf16 parts; p s_v
-// is split into two (bf16 tensors: 16 bits) or three parts (float32: all 24 bits).  What the parts
-// lose multiplies n - 7.5, not n: the rest of p s_v goes into the per-row sum with 7.5.  For float32
-// the 23.5 = 16 + 7.5 is also taken off inside the matrix products (a product with a constant
-// operand starts the accumulators, every 32 channels or tokens): sums over a long context would
-// otherwise grow to 23.5 sum(p s_v) and lose the digits of a result that averages out.
+// is split into two (bf16 tensors: 16 bits, what they lose times 16 + n is 3e-5 of a result, a bf16
+// rounding 2e-3) or three parts (float32: all 24 bits).  For float32 23.5 = 16 + 7.5 is taken off
+// inside the matrix products (a product with a constant operand starts the accumulators, every 32
+// channels or tokens): sums over a long context would otherwise grow to 23.5 sum(p s_v) and lose the
+// digits of a result that averages out.
 //
 // Work: a wave takes tiles of TT = 128 (head dim 64) or 64 tokens, 8 KB of codes, on its own, with
 // its own running maximum; four waves of a workgroup and, for few heads, several workgroups
@@ -74,23 +74,21 @@ __device__ __forceinline__ V load_at(const void *base, uint32_t off) {
   return *reinterpret_cast<const V *>((const char *)base + off);
 }
 
-// x = sum of its PS bf16 parts (the last one rounded), returns that sum
-template <int PS>
-__device__ __forceinline__ float split(float x, bf16 (&part)[PS]) {
-  float rest = x, sum = 0.f;
+// x = the sum of its bf16 parts, the last one rounded
+template <int N>
+__device__ __forceinline__ void split(float x, bf16 (&part)[N]) {
 #pragma unroll
-  for (int k = 0; k < PS; ++k) {
-    part[k] = (bf16)rest;
-    sum += (float)part[k];
-    rest -= (float)part[k];
+  for (int k = 0; k < N; ++k) {
+    part[k] = (bf16)x;
+    x -= (float)part[k];
   }
-  return sum;
 }
 
 // Waves a SIMD that the registers are cut for: as many as nothing spills with.
 constexpr int waves_of(bool f32, int DP, int R, bool bias) {
-  if (R <= 4) return f32 ? (DP == 64 ? 3 : 2) : (DP == 64 ? 4 : 3);
-  return f32 ? (DP == 64 || !bias ? 2 : 1) : (DP == 64 || !bias ? 3 : 2);
+  if (R <= 4) return (f32 ? (DP == 64 ? 3 : 2) : (DP == 64 ? 4 : 3)) -
+                     (DP == 64 && (bias || (f32 && R == 4)) ? 1 : 0);
+  return f32 ? (bias ? 1 : 2) : (bias ? 2 : 3);
 }
 
 // BIAS: edge_scores, edge_table or mask given
@@ -112,7 +110,9 @@ kv4_attn_kernel(Kv4Attn a) {
   constexpr bool OWN_PAR = R == 1;       // ... which are the ones that it evaluates
   constexpr int SROW = TT + 4, PROW = TT + 8;
   constexpr float NEG = -__builtin_inff();
-  constexpr float STEP = 8.0f, LOG2E = 1.4426950408889634f;
+  constexpr float LOG2E = 1.4426950408889634f;
+  // scores in units of log2 where no bias of the type's lowest number can overflow them
+  constexpr float STEP = BIAS ? 8.0f : 8.0f * LOG2E, UNIT = BIAS ? LOG2E : 1.f;
   constexpr float CENTER = F32 ? 23.5f : 16.f;    // taken off a code inside the first product
   constexpr int KROW = DP / 2, VROW = DP * 4;     // bytes of a token's K, of 8 tokens' V
 
@@ -143,6 +143,57 @@ kv4_attn_kernel(Kv4Attn a) {
   const int Lq = (int)a.Lq, S = (int)a.S, row0 = (int)rt * 16;
   const int rows = Lq * a.share - row0;                    // of this tile: row = query * share + r
   const int tile_rows = rows < 16 ? rows : 16;
+  const int64_t head = (int64_t)b * a.H + h;
+  const char *kc = (const char *)a.k_codes + head * a.S * KROW;
+  const char *vc = (const char *)a.v_codes + head * a.S * KROW;
+  const uint32_t *kp = (const uint32_t *)a.k_par + head * G * a.S;
+  const uint32_t *vp = (const uint32_t *)a.v_par + head * G * a.S;
+
+  u32x2 kw[NSUB][2][G];
+  u32x4 vw[NSUB][G];
+  uint32_t kpw[G][NP], vpw[G][NP];
+  const uint32_t k_off = (8 * (col >> 2) + (col & 3)) * KROW + 8 * g;
+  const uint32_t v_off = g * VROW + 16 * col;
+  // tile t, 32 tokens at a time, none beyond the `most`th
+  auto fetch_k = [&](int t, int most) {
+#pragma unroll
+    for (int s = 0; s < NSUB; ++s) {
+      int sub = t * NSUB + s;
+      sub = sub < most ? sub : most;
+      const char *base = kc + (int64_t)sub * 32 * KROW;
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+        for (int grp = 0; grp < G; ++grp)
+          kw[s][blk][grp] = load_at<u32x2>(base + blk * 4 * KROW + grp * 32, k_off);
+    }
+    const uint32_t tok = (uint32_t)t * TT + NP * lane, end = S - NP;
+    const uint32_t off = (tok < end ? tok : end) * 4;
+#pragma unroll
+    for (int grp = 0; grp < G; ++grp)
+#pragma unroll
+      for (int e = 0; e < NP; ++e) {
+        kpw[grp][e] = load_at<uint32_t>(kp + grp * a.S + e, off);
+        vpw[grp][e] = load_at<uint32_t>(vp + grp * a.S + e, off);
+      }
+  };
+  auto fetch_v = [&](int t, int most) {
+#pragma unroll
+    for (int s = 0; s < NSUB; ++s) {
+      int sub = t * NSUB + s;
+      sub = sub < most ? sub : most;
+      const char *base = vc + (int64_t)sub * 4 * VROW;
+#pragma unroll
+      for (int grp = 0; grp < G; ++grp) vw[s][grp] = load_at<u32x4>(base + grp * 256, v_off);
+    }
+  };
+  // the first tile does not depend on the length where no split does; where sequences are expected
+  // to reach it, it is requested before the length is known
+  if (a.ahead) {
+    fetch_k(wave, S / 32 - 1);
+    fetch_v(wave, S / 32 - 1);
+  }
+
   int64_t len64 = load_len(a.length, a.length_dtype, b);
   const int len = len64 < 0 ? 0 : (len64 > S ? S : (int)len64);
   int64_t ql64 = a.q_length ? load_len(a.q_length, a.q_length_dtype, b) : Lq;
@@ -167,53 +218,10 @@ kv4_attn_kernel(Kv4Attn a) {
   int sub_last = top > 0 ? (top - 1) / 32 : 0;
   if (t_end * NSUB - 1 < sub_last) sub_last = t_end > 0 ? t_end * NSUB - 1 : 0;
 
-  const int64_t head = (int64_t)b * a.H + h;
-  const char *kc = (const char *)a.k_codes + head * a.S * KROW;
-  const char *vc = (const char *)a.v_codes + head * a.S * KROW;
-  const uint32_t *kp = (const uint32_t *)a.k_par + head * G * a.S;
-  const uint32_t *vp = (const uint32_t *)a.v_par + head * G * a.S;
-
-  u32x2 kw[NSUB][2][G];
-  u32x4 vw[NSUB][G];
-  uint32_t kpw[G][NP], vpw[G][NP];
-  const uint32_t k_off = (8 * (col >> 2) + (col & 3)) * KROW + 8 * g;
-  const uint32_t v_off = g * VROW + 16 * col;
-  auto fetch_k = [&](int t) {
-#pragma unroll
-    for (int s = 0; s < NSUB; ++s) {
-      int sub = t * NSUB + s;
-      sub = sub < sub_last ? sub : sub_last;
-      const char *base = kc + (int64_t)sub * 32 * KROW;
-#pragma unroll
-      for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-        for (int grp = 0; grp < G; ++grp)
-          kw[s][blk][grp] = load_at<u32x2>(base + blk * 4 * KROW + grp * 32, k_off);
-    }
-    const uint32_t tok = (uint32_t)t * TT + NP * lane, most = S - NP;
-    const uint32_t off = (tok < most ? tok : most) * 4;
-#pragma unroll
-    for (int grp = 0; grp < G; ++grp)
-#pragma unroll
-      for (int e = 0; e < NP; ++e) {
-        kpw[grp][e] = load_at<uint32_t>(kp + grp * a.S + e, off);
-        vpw[grp][e] = load_at<uint32_t>(vp + grp * a.S + e, off);
-      }
-  };
-  auto fetch_v = [&](int t) {
-#pragma unroll
-    for (int s = 0; s < NSUB; ++s) {
-      int sub = t * NSUB + s;
-      sub = sub < sub_last ? sub : sub_last;
-      const char *base = vc + (int64_t)sub * 4 * VROW;
-#pragma unroll
-      for (int grp = 0; grp < G; ++grp) vw[s][grp] = load_at<u32x4>(base + grp * 256, v_off);
-    }
-  };
   int t = t_begin + wave;
-  if (t < t_end) {
-    fetch_k(t);
-    fetch_v(t);
+  if (!a.ahead && t < t_end) {
+    fetch_k(t, sub_last);
+    fetch_v(t, sub_last);
   }
 
   // ---- queries: operand B of K Q^T, channel 64 grp + 16 g + 8 s + j of row col ----
@@ -254,7 +262,7 @@ kv4_attn_kernel(Kv4Attn a) {
         for (int j = 0; j < 8; ++j) {
           qsum[grp] += x[j];
           bf16 part[QS];
-          split<QS>(x[j], part);
+          split(x[j], part);
 #pragma unroll
           for (int k = 0; k < QS; ++k) qf[grp][s][k][j] = part[k];
         }
@@ -307,20 +315,24 @@ kv4_attn_kernel(Kv4Attn a) {
     const float c = F32 ? fmaf(7.5f, s, min_of(w)) : min_of(w);
     return fmaf(s, dot, c * qsum[grp]);
   };
+  const float scale = BIAS ? a.inv_temperature : a.inv_temperature * LOG2E;
   const int seen_last = vis > 0 ? vis - 1 : 0;             // (loads stay on keys that exist)
-  auto finish = [&](float z, int j) -> float {             // bias, scale, mask of key j
-    bool on = j < vis;
-    if (BIAS) {
-      const int jj = j < seen_last ? j : seen_last;
-      if (edge) z += to_f32(edge[(int64_t)jj * a.edge_stride[3]]);
-      if (table) {
-        int at = table_last - pos + jj;
-        at = at < 0 ? 0 : (at > table_last ? table_last : at);
-        z += to_f32(table[at]);
-      }
-      if (mask) on = on && mask[(int64_t)jj * a.mask_stride[2]] != 0;
+  // the bias of key j, -inf where the mask is off; key j's score with it
+  auto bias_of = [&](int j) -> float {
+    float z = 0.f;
+    const int jj = j < seen_last ? j : seen_last;
+    if (edge) z = to_f32(edge[(int64_t)jj * a.edge_stride[3]]);
+    if (table) {
+      int at = table_last - pos + jj;
+      at = at < 0 ? 0 : (at > table_last ? table_last : at);
+      z = to_f32(table[at]);
     }
-    return on ? z * a.inv_temperature : NEG;
+    if (mask) z = mask[(int64_t)jj * a.mask_stride[2]] != 0 ? z : NEG;
+    return z;
+  };
+  auto finish = [&](float z, float bias, int j) -> float {
+    if (BIAS) z = bias == NEG ? NEG : z + bias;
+    return j < vis ? z * scale : NEG;
   };
 
   // ---- running state ----
@@ -337,7 +349,7 @@ kv4_attn_kernel(Kv4Attn a) {
     for (int o = DIRECT ? 32 : LPR / 2; o > (DIRECT ? 8 : 0); o >>= 1)
       most = fmaxf(most, __shfl_xor(most, o, 64));
     const float to = fmaxf(ref, most);
-    const float alpha = ref == to ? 1.f : __builtin_amdgcn_exp2f((ref - to) * LOG2E);
+    const float alpha = ref == to ? 1.f : __builtin_amdgcn_exp2f((ref - to) * UNIT);
     ref = to;
     l *= alpha;
 #pragma unroll
@@ -357,10 +369,11 @@ kv4_attn_kernel(Kv4Attn a) {
   };
   // weight p of a token with V parameters w: parts of p s_v, its share of the per-row sum
   auto weigh = [&](float p, bool off, uint32_t w, int grp, bf16 (&part)[PS]) {
-    const float pv = off ? 0.f : p * scale_of(w);
-    const float sum = split<PS>(pv, part);
-    // F32: the 23.5 comes off inside the product
-    csum[grp] += (off ? 0.f : p * min_of(w)) + fmaf(7.5f, pv, F32 ? 0.f : -23.5f * sum);
+    const float pv = off ? 0.f : p * scale_of(w), pm = off ? 0.f : min_of(w);
+    split(pv, part);
+    // (the product takes 16 + n, or, F32, n - 7.5)
+    csum[grp] = fmaf(p, pm, csum[grp]);
+    csum[grp] = fmaf(F32 ? 7.5f : -16.f, pv, csum[grp]);
   };
   // O^T += V^T P^T of 32 tokens: channel 64 grp + 4 row + i of operand A's row
   auto products = [&](int s, int grp, const bf16x8 (&pb)[PS]) {
@@ -401,6 +414,13 @@ kv4_attn_kernel(Kv4Attn a) {
           parl[(G + grp) * TT + NP * lane + e] = vpw[grp][e];
         }
       }
+    float bias[TPL];
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < VW; ++e)
+        bias[v * VW + e] =
+            BIAS && !DIRECT ? bias_of(t * TT + v * LPR * VW + sl * VW + e) : 0.f;
     if (DIRECT) wave_lds_sync();
     // ---- scores: S^T = K Q^T, rows of 32 tokens as V wants them ----
 #pragma unroll
@@ -436,12 +456,13 @@ kv4_attn_kernel(Kv4Attn a) {
           }
         }
       }
-    fetch_k(t + 4);
+    fetch_k(t + 4, sub_last);
     float most = NEG;
     if (DIRECT) {
 #pragma unroll
       for (int n = 0; n < TPL; ++n) {
-        x[n] = finish(x[n], t * TT + (n >> 3) * 32 + 8 * g + (n & 7));
+        const int j = t * TT + (n >> 3) * 32 + 8 * g + (n & 7);
+        x[n] = finish(x[n], BIAS ? bias_of(j) : 0.f, j);
         most = fmaxf(most, x[n]);
       }
     } else {
@@ -456,7 +477,7 @@ kv4_attn_kernel(Kv4Attn a) {
           for (int grp = 0; grp < G; ++grp)
             z += scaled(sc[(grp * R + row) * SROW + tok],
                         OWN_PAR ? kpr[grp][n] : parl[grp * TT + tok], grp);
-          x[n] = finish(z, t * TT + tok);
+          x[n] = finish(z, bias[n], t * TT + tok);
           most = fmaxf(most, x[n]);
         }
     }
@@ -469,7 +490,7 @@ kv4_attn_kernel(Kv4Attn a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float z = x[s * 8 + e];
-          p[e] = z == NEG ? 0.f : __builtin_amdgcn_exp2f((z - ref) * LOG2E);
+          p[e] = z == NEG ? 0.f : __builtin_amdgcn_exp2f((z - ref) * UNIT);
           l += p[e];
         }
 #pragma unroll
@@ -497,7 +518,7 @@ kv4_attn_kernel(Kv4Attn a) {
 #pragma unroll
         for (int e = 0; e < VW; ++e) {
           const float z = x[v * VW + e];
-          p[e] = z == NEG ? 0.f : __builtin_amdgcn_exp2f((z - ref) * LOG2E);
+          p[e] = z == NEG ? 0.f : __builtin_amdgcn_exp2f((z - ref) * UNIT);
           l += p[e];
         }
 #pragma unroll
@@ -529,7 +550,7 @@ kv4_attn_kernel(Kv4Attn a) {
           products(s, grp, pb);
         }
     }
-    fetch_v(t + 4);
+    fetch_v(t + 4, sub_last);
     wave_lds_sync();
   }
 
@@ -570,7 +591,7 @@ kv4_attn_kernel(Kv4Attn a) {
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const float *m = jm + (w * R + orow) * (2 + G);
-      const float f = m[0] == mx ? 1.f : __builtin_amdgcn_exp2f((m[0] - mx) * LOG2E);
+      const float f = m[0] == mx ? 1.f : __builtin_amdgcn_exp2f((m[0] - mx) * UNIT);
       sum += f * m[1];
       o += f * (jo[(w * R + orow) * OROW + c] + m[2 + c / 64]);
     }
@@ -584,18 +605,17 @@ kv4_attn_kernel(Kv4Attn a) {
       const int64_t at = (first_row + orow) * a.splits + split_no;
       a.part_o[at * DP + c] = o;
       if (c == 0) {
-        a.part_ml[at * 2] = mx;
+        a.part_ml[at * 2] = mx * UNIT;             // in units of log2
         a.part_ml[at * 2 + 1] = sum;
       }
     }
   }
 }
 
-// The splits of a row: O = sum_s exp(m_s - M) O_s / sum_s exp(m_s - M) l_s.  A workgroup takes one
+// The splits of a row: O = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.  A workgroup takes one
 // row: 256 threads = DP / 4 channel quads x groups of splits, added up in a fixed order.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Attn a) {
-  constexpr float LOG2E = 1.4426950408889634f;
   constexpr int Q = DP / 4, GROUPS = 256 / Q;
   __shared__ float f[KV4_MAX_SPLITS];
   __shared__ f32x4 part[GROUPS][Q];
@@ -615,7 +635,7 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Attn a) {
     const float m = s < a.splits ? ml[2 * s] : -__builtin_inff();
     const float l = s < a.splits ? ml[2 * s + 1] : 0.f;
     const float mx = wave_max(m);
-    const float w = m == mx ? 1.f : __builtin_amdgcn_exp2f((m - mx) * LOG2E);
+    const float w = m == mx ? 1.f : __builtin_amdgcn_exp2f(m - mx);
     f[s] = w;
     const float sum = wave_sum(w * l);
     if (s == 0) total = sum;

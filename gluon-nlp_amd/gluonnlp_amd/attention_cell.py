@@ -366,7 +366,7 @@ def multi_head_dot_attn_cached(query, cache, layer=0, *, causal: bool = True, ed
                                   'We only support layout = "NKT", "NTK", and "TNK".'
                                   .format(layout))
     e, table, m = T.as_tensor(edge_scores), T.as_tensor(edge_table), T.as_tensor(mask)
-    dev = T.device_index(cache.length, q, e, table, m)
+    dev = T.device_index(q, cache.length, e, table, m)
     shape = q.shape
     if len(shape) != 4:
         raise ValueError('query {} is not 4-dimensional'.format(tuple(shape)))
@@ -374,7 +374,7 @@ def multi_head_dot_attn_cached(query, cache, layer=0, *, causal: bool = True, ed
     if B != cache.batch_size or d != cache.head_units or H % cache.num_heads or H == 0:
         raise ValueError('query {} (layout {}) does not match {}'.format(tuple(shape), layout,
                                                                         cache))
-    if wants_grad(q, e, table):
+    if (q.requires_grad or e is not None or table is not None) and wants_grad(q, e, table):
         raise NotImplementedError('attention over a 4-bit cache has no gradient: decode under '
                                   'torch.no_grad()')
     st = q.stride()

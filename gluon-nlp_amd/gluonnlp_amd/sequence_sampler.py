@@ -9,7 +9,6 @@ import torch
 
 from . import _lib
 from . import _tensor as T
-from .autograd import wants_grad
 from .kv_cache import QuantKVCache
 
 __all__ = ['beam_search_select', 'reorder_states']
@@ -59,7 +58,7 @@ def beam_search_select(outputs, scores, finished=None, *, eos_id=None, step=1, a
     shape = x.shape
     if shape[:-1] not in ((N, K), (N * K,)) or shape[-1] < 1:
         raise ValueError('outputs {} do not match scores {}'.format(tuple(shape), tuple(s.shape)))
-    if wants_grad(x, s):
+    if (x.requires_grad or s.requires_grad) and torch.is_grad_enabled():
         raise NotImplementedError('the selection has no gradient: search under torch.no_grad()')
     V, st = shape[-1], x.stride()
     if st[-1] != 1 and V > 1 or len(st) == 3 and st[0] != K * st[1] or st[-2] < V:
@@ -89,8 +88,7 @@ def beam_search_select(outputs, scores, finished=None, *, eos_id=None, step=1, a
                            step, step_ptr, step_code, temperature, alpha,
                            K if length_base is None else length_base)
     out_scores = torch.empty_like(s)
-    parents = s.new_empty((N, K), dtype=torch.int32)
-    tokens = torch.empty_like(parents)
+    parents, tokens = s.new_empty((2, N, K), dtype=torch.int32).unbind(0)
     out_finished = s.new_empty((N, K), dtype=torch.bool)
     nws = _select_workspace(N, K, V)
     ws = s.new_empty(nws, dtype=torch.uint8)
@@ -138,39 +136,48 @@ def reorder_states(states, parents, batch_axis=0, out=None):
     dev = T.device_index(p)
     rows, grad = N * K, torch.is_grad_enabled()
     flat, sources, caches = [], [], []
+    last = (None, None, None)              # (shape, dtype, axis) of the state before, and its rows
+    tail = None
 
     def one(s, axis, o):
+        nonlocal last, tail
         t = s if type(s) is torch.Tensor else T.as_tensor(s)
         if t.get_device() != dev:
             T.require_device(p, t)
         if grad and t.requires_grad:
             raise NotImplementedError('reordering has no gradient: decode under torch.no_grad()')
-        shape = t.shape
-        if type(axis) is not int or not 0 <= axis < len(shape) or shape[axis] != rows:
-            raise ValueError('state {}: axis {} does not hold {} x {} rows'.format(
-                tuple(shape), axis, N, K))
+        shape, dtype = t.shape, t.dtype
+        if last[0] != shape or last[1] is not dtype or last[2] is not axis:
+            if type(axis) is not int or not 0 <= axis < len(shape) or shape[axis] != rows:
+                raise ValueError('state {}: axis {} does not hold {} x {} rows'.format(
+                    tuple(shape), axis, N, K))
+            last, tail, n = (shape, dtype, axis), None, t.numel()
+            if n:
+                outer = 1
+                for i in range(axis):
+                    outer *= shape[i]
+                row = n // (outer * rows) * t.element_size()
+                tail = (outer, row * rows, row, 1, row, row, 0, 0)
         if not t.is_contiguous():
             if in_place:
                 raise ValueError('in place: the states must be contiguous')
             t = t.contiguous()
-            sources.append(t)      # (it has to live until the launch)
+            sources.append(t)              # (it has to live until the launch)
         if in_place:
             d = t
         elif o is None:
             d = torch.empty_like(t)
         else:
             d = o if type(o) is torch.Tensor else T.as_tensor(o)
-            if d.shape != shape or d.dtype != t.dtype or not d.is_contiguous() or \
+            if d.shape != shape or d.dtype is not dtype or not d.is_contiguous() or \
                     d.get_device() != dev:
                 raise ValueError('out {} {} does not fit the state {} {}'.format(
-                    tuple(d.shape), d.dtype, tuple(shape), t.dtype))
-        n = t.numel()
-        if n:
-            step = t.stride(axis)
-            row = step * t.element_size()
-            flat.extend((t.data_ptr(), d.data_ptr(), n // (rows * step), row * rows, row, 1, row,
-                         row, 0, 0))
-        return d if s is t or type(s) is torch.Tensor else T.like_caller(d, s)
+                    tuple(d.shape), d.dtype, tuple(shape), dtype))
+        if tail is not None:
+            flat.append(t.data_ptr())
+            flat.append(d.data_ptr())
+            flat.extend(tail)
+        return d if type(s) is torch.Tensor else T.like_caller(d, s)
 
     def walk(s, axis, o):
         if isinstance(s, torch.Tensor):
@@ -187,7 +194,8 @@ def reorder_states(states, parents, batch_axis=0, out=None):
             outs = o if isinstance(o, (list, tuple)) else (o,) * n
             if len(axes) != n or len(outs) != n or (o is not None and outs is not o):
                 raise ValueError('batch_axis / out are not nested like the states')
-            r = [walk(*x) for x in zip(s, axes, outs)]
+            r = [one(x, ax, ox) if type(x) is torch.Tensor else walk(x, ax, ox)
+                 for x, ax, ox in zip(s, axes, outs)]
             return r if isinstance(s, list) else tuple(r)
         return one(s, axis, o)
 
