@@ -18,7 +18,7 @@ import torch
 from . import _lib
 from . import _tensor as T
 
-__all__ = ['QuantKVCache']
+__all__ = ['QuantKVCache', 'QuantDecoderStates']
 
 _TIME = {'NKT': 2, 'NTK': 1, 'TNK': 0}
 _PERM = {'NKT': (0, 1, 2), 'NTK': (0, 2, 1), 'TNK': (1, 2, 0)}
@@ -232,3 +232,58 @@ class QuantKVCache:
         # (a launch of its own: the one above reads the lengths)
         at = self.length.data_ptr()
         launch_reorder(dev, [at, at, 1, 4 * B, 4, 1, 4, 4, 0, 0], N, K, p, None)
+
+
+class QuantDecoderStates:
+    """States of ``T5Decoder.incremental_decode`` / ``TransformerDecoder.incremental_decode`` with
+    keys and values in 4 bits (made by the decoders' ``init_quant_states``): ``self_cache`` grows by
+    a token a step; ``memory_cache`` holds the memory's projections, written once, one sequence an
+    item -- the beams of an item (consecutive rows) attend over it as the queries of one call.
+    ``bias_table``: T5's position bias by distance.  Projections and table are those of the weights
+    at the time the states were made.  A step does not change its shapes: it can be captured in a
+    graph and replayed."""
+
+    def __init__(self, self_cache, memory_cache, bias_table=None):
+        if self_cache.batch_size % memory_cache.batch_size:
+            raise ValueError('{} rows do not share {} memories evenly'.format(
+                self_cache.batch_size, memory_cache.batch_size))
+        self.self_cache, self.memory_cache, self.bias_table = self_cache, memory_cache, bias_table
+
+    @property
+    def length(self):
+        return self.self_cache.length
+
+    def reorder(self, parents):
+        """Beam search: row n K + k goes on from row n K + parents[n, k].  The memory stays: the
+        beams of an item share it."""
+        if self.memory_cache.batch_size not in (parents.shape[0], self.self_cache.batch_size):
+            raise ValueError('{} items, the states hold {} memories'.format(
+                parents.shape[0], self.memory_cache.batch_size))
+        if self.memory_cache.batch_size != parents.shape[0]:
+            self.memory_cache.reorder(parents)
+        self.self_cache.reorder(parents)
+
+    def memory_queries(self, q):
+        """(rows, 1, H, d) or (1, rows, H, d) -> (memories, beams, H, d)."""
+        return q.reshape(self.memory_cache.batch_size, -1, q.shape[2], q.shape[3])
+
+
+def quant_decoder_states(mem, mem_valid_length, projections, num_heads, head_units, max_length,
+                         beam_size, layout, bias_table=None):
+    """The states of a decoder; ``projections``: per layer the Dense layers of the memory's keys and
+    values.  mem: (items, Lm, C) / (Lm, items, C)."""
+    m = T.as_tensor(mem)
+    axis = 1 if layout == 'NT' else 0
+    items, Lm = m.shape[1 - axis], m.shape[axis]
+    kv = 'NTK' if layout == 'NT' else 'TNK'
+    n = len(projections)
+    with torch.no_grad():
+        memory = QuantKVCache(items, num_heads, head_units, Lm, n, m.device, kv)
+        memory.set_length(Lm)
+        for i, (key, value) in enumerate(projections):
+            memory.write(*(T.as_tensor(p(m)).reshape(m.shape[0], m.shape[1], num_heads, head_units)
+                           for p in (key, value)), layer=i)
+        if mem_valid_length is not None:
+            memory.set_length(T.as_tensor(mem_valid_length))
+        rows = QuantKVCache(items * beam_size, num_heads, head_units, max_length, n, m.device, kv)
+    return QuantDecoderStates(rows, memory, bias_table)

@@ -11,7 +11,9 @@ from torch import nn
 from .. import _lib
 from .. import _tensor as T
 from ..attention_cell import (MultiHeadAttentionCell, RelAttentionScoreCell, gen_mem_attn_mask,
-                              gen_rel_position, gen_self_attn_mask, mask_predicate)
+                              gen_rel_position, gen_self_attn_mask, mask_predicate,
+                              multi_head_dot_attn_cached)
+from ..kv_cache import QuantDecoderStates, quant_decoder_states
 from ..layers import Dense, Embedding, PositionwiseFFN, RMSNorm, ffn_params_struct, memory_kv
 
 __all__ = ['T5Block', 'T5Encoder', 'T5Decoder', 'T5Model']
@@ -192,6 +194,23 @@ class T5Block(nn.Module):
         x = self._cross_and_ffn(x, mem_states, step_mem_attn_mask,
                                 states=(past_key_value[0], self_key))
         return T.like_caller(T.as_tensor(x), step_hidden_states), (self_key, self_value)
+
+    def decode_cached(self, x, states, i):
+        """One target position with ``QuantDecoderStates``, as layer i; x (B, 1, d_model) /
+        (1, B, d_model) -> the same."""
+        out = self.self_attn_layer_norm(x)
+        q = self.transpose_for_scores(self.self_attn_q(out))
+        states.self_cache.write(self.transpose_for_scores(self.self_attn_k(out)),
+                                self.transpose_for_scores(self.self_attn_v(out)), i)
+        out = multi_head_dot_attn_cached(q, states.self_cache, i, edge_table=states.bias_table,
+                                         scaled=False)
+        x = T.as_tensor(self.self_attn_proj(out, other=x, combine='add'))
+        out = self.cross_attn_layer_norm(x)
+        q = states.memory_queries(self.transpose_for_scores(self.cross_attn_q(out)))
+        out = multi_head_dot_attn_cached(q, states.memory_cache, i, causal=False, scaled=False,
+                                         layout='NTK')
+        out = out.reshape(x.shape[0], x.shape[1], -1)
+        return self.ffn(self.cross_attn_proj(out, other=x, combine='add'))
 
     def forward(self, hidden_states, self_attn_mask, position_embeddings, mem_states=None,
                 mem_attn_mask=None):
@@ -407,10 +426,30 @@ class T5Decoder(nn.Module):
     def _init_key_values(self, batch_size, ctx, dtype='float32'):
         return list(layer._init_key_value(batch_size, ctx, dtype) for layer in self.layers)
 
+    def init_quant_states(self, mem_states, mem_valid_length, max_length, beam_size=1):
+        """States with keys and values in 4 bits for ``incremental_decode``: room for
+        ``max_length`` target positions of beam_size rows an item; the memory, (items, L_src,
+        d_model) / (L_src, items, d_model), is projected here."""
+        # the bias depends on the distance alone, and not on it from max_distance on
+        R = min(max_length, self.relative_position_encoder._max_distance + 1)
+        table = self.relative_position_encoder.self_attn_bias_table(R)[:, :R].contiguous()
+        return quant_decoder_states(
+            mem_states, mem_valid_length, [(b.cross_attn_k, b.cross_attn_v) for b in self.layers],
+            self._num_heads, self._d_kv, max_length, beam_size, self.layout, table)
+
     def incremental_decode(self, step_hidden_states, position, past_key_values, mem_states,
                            mem_valid_length):
         """models/t5.py:812-893.  ``position`` (B,) is accepted as in the reference, which derives
-        the step's relative positions from the length of the cached keys instead (:863-870)."""
+        the step's relative positions from the length of the cached keys instead (:863-870).
+        With ``past_key_values`` from ``init_quant_states`` the memory arguments are not used (under
+        torch.no_grad(); the states are updated and returned)."""
+        if isinstance(past_key_values, QuantDecoderStates):
+            x = T.as_tensor(step_hidden_states)
+            past_key_values.self_cache.extend(1)
+            for i, layer in enumerate(self.layers):
+                x = T.as_tensor(layer.decode_cached(x, past_key_values, i))
+            return T.like_caller(T.as_tensor(self.final_layer_norm(x)), step_hidden_states), \
+                past_key_values
         past = T.as_tensor(past_key_values[0][0])
         L = past.shape[self._time_axis] + 1
         # last row of the (L, L) bias = relative positions (mem_j - (L - 1)) of the new query =

@@ -11,8 +11,10 @@ from torch import nn
 from .. import _lib
 from .. import _tensor as T
 from ..attention_cell import (MultiHeadAttentionCell, gen_mem_attn_mask, gen_self_attn_mask,
-                              mask_predicate)
+                              mask_predicate,
+                              multi_head_dot_attn_cached)
 from ..autograd import SeqMaskFn, wants_grad
+from ..kv_cache import QuantDecoderStates, quant_decoder_states
 from ..layers import Dense, LayerNorm, PositionwiseFFN, ffn_params_struct, memory_kv
 
 __all__ = ['TransformerEncoderLayer', 'TransformerEncoder', 'run_encoder_stack',
@@ -486,6 +488,33 @@ class TransformerDecoderLayer(nn.Module):
         out = T.as_tensor(self.ffn(out))
         return T.like_caller(out.reshape(-1, out.shape[-1]), data), (new_key, new_value)
 
+    def decode_cached(self, data, states, i):
+        """One target position with ``QuantDecoderStates``, as layer i; data (B, C_in) ->
+        (B, C_out)."""
+        x = T.as_tensor(data)
+        if self._pre_norm:
+            x = self.ln_in(x)
+        x = T.as_tensor(x).unsqueeze(1 if self.layout == 'NT' else 0)
+        qkv = T.as_tensor(self.attn_in_qkv(x))
+        U = self._units
+        q, k, v = (self._heads(qkv[..., n * U:(n + 1) * U]) for n in range(3))
+        states.self_cache.write(k, v, i)
+        out = multi_head_dot_attn_cached(q, states.self_cache, i)
+        out = self.proj_in(out, other=x)
+        if not self._pre_norm:
+            out = self.ln_in(out)
+        x = T.as_tensor(out)
+        if self._pre_norm:
+            x = self.ln_inter(x)
+        q = states.memory_queries(self._heads(T.as_tensor(self.attn_inter_q(x))))
+        out = multi_head_dot_attn_cached(q, states.memory_cache, i, causal=False, layout='NTK')
+        x = T.as_tensor(x)
+        out = self.proj_inter(out.reshape(x.shape[0], x.shape[1], -1), other=x)
+        if not self._pre_norm:
+            out = self.ln_inter(out)
+        out = T.as_tensor(self.ffn(out))
+        return out.reshape(-1, out.shape[-1])
+
 
 class TransformerDecoder(nn.Module):
     """models/transformer.py:738-959."""
@@ -556,8 +585,21 @@ class TransformerDecoder(nn.Module):
         return [(self.layers[0] if self.recurrent else self.layers[i]).init_states(
             batch_size=batch_size, ctx=ctx, dtype=dtype) for i in range(self.num_layers)]
 
+    def init_quant_states(self, mem, mem_valid_length, max_length, beam_size=1):
+        """States with keys and values in 4 bits for ``incremental_decode``: room for
+        ``max_length`` target positions of beam_size rows an item; the memory, (items, L_mem, C) /
+        (L_mem, items, C), is projected here."""
+        layers = [self.layers[0] if self.recurrent else self.layers[i]
+                  for i in range(self.num_layers)]
+        heads = layers[0]._num_heads
+        return quant_decoder_states(
+            mem, mem_valid_length, [(x.attn_inter_k, x.attn_inter_v) for x in layers], heads,
+            self._units // heads, max_length, beam_size, self._layout)
+
     def incremental_decode(self, data, states, mem, mem_valid_length):
         """data (B, C_in), one cache pair per layer -> (out (B, C_out), new caches).
+        With states from ``init_quant_states`` the memory arguments are not used (under
+        torch.no_grad(); the states are updated and returned).
         models/transformer.py:884-959: the memory mask (B, 1, mem_length) is built once.
         The memory's key / value projections are kept in the states between steps
         (layers.memory_kv): they follow optimizer steps and copy_() of the weights, not writes
@@ -565,6 +607,14 @@ class TransformerDecoder(nn.Module):
         out = data
         if self._data_norm:
             out = self.ln_data(out)
+        if isinstance(states, QuantDecoderStates):
+            states.self_cache.extend(1)
+            for i in range(self.num_layers):
+                out = (self.layers[0] if self.recurrent else self.layers[i]).decode_cached(
+                    out, states, i)
+            if self._pre_norm:
+                out = self.ln_final(out)
+            return T.like_caller(T.as_tensor(out), data), states
         time_axis = 0 if self.layout == 'TN' else 1
         step = T.as_tensor(data).unsqueeze(time_axis)
         mem_attn_mask = gen_mem_attn_mask(mem, mem_valid_length, step, None, dtype=self._dtype,

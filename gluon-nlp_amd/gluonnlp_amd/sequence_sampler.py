@@ -9,9 +9,9 @@ import torch
 
 from . import _lib
 from . import _tensor as T
-from .kv_cache import QuantKVCache
+from .kv_cache import QuantDecoderStates, QuantKVCache
 
-__all__ = ['beam_search_select', 'reorder_states']
+__all__ = ['beam_search_select', 'reorder_states', 'BeamSearchSampler']
 
 MAX_BEAMS = 32
 
@@ -123,7 +123,7 @@ def reorder_states(states, parents, batch_axis=0, out=None):
     """Reorder decoding states after a selection: row n K + k along the batch axis of every tensor
     becomes its row n K + parents[n, k] (parents (N, K), values in [0, K); others are clamped).
 
-    states: a tensor, a ``QuantKVCache``, None, or nested lists / tuples of them, as
+    states: a tensor, a ``QuantKVCache``, ``QuantDecoderStates``, None, or nested lists / tuples of them, as
     ``incremental_decode`` returns them; ``batch_axis``: one int, or axes nested like the states
     (a decoder's ``state_batch_axis``).  Returns the same structure: new tensors, or the tensors of
     ``out`` (nested like the states, contiguous, no overlap with the states), or, with
@@ -184,7 +184,7 @@ def reorder_states(states, parents, batch_axis=0, out=None):
             return one(s, axis, o)
         if s is None:
             return None
-        if isinstance(s, QuantKVCache):
+        if isinstance(s, (QuantKVCache, QuantDecoderStates)):
             if not any(c is s for c in caches):
                 caches.append(s)
             return s
@@ -205,3 +205,59 @@ def reorder_states(states, parents, batch_axis=0, out=None):
     for c in caches:
         c.reorder(p)
     return result
+
+
+class BeamSearchSampler:
+    """Beam search with a step decoder (the reference's sequence_sampler.BeamSearchSampler).
+
+    decoder(step_input (N * K,), states) -> (outputs (N * K, V), states): logits (or, with
+    ``from_logits=False``, log-probabilities) of the next token, and the states after the step;
+    the states hold N * K rows along ``state_batch_axis``.  A candidate's score is its
+    log-probability sum over ((length_base + length) / (length_base + 1)) ** alpha."""
+
+    def __init__(self, beam_size, decoder, eos_id, alpha=1.0, length_base=5, max_length=100,
+                 temperature=1.0, from_logits=True, state_batch_axis=0, early_return=True):
+        if not 1 <= beam_size <= MAX_BEAMS:
+            raise ValueError('beam size {} is outside [1, {}]'.format(beam_size, MAX_BEAMS))
+        if max_length < 1:
+            raise ValueError('max_length={} must be positive'.format(max_length))
+        self._beam_size, self._decoder, self._eos_id = beam_size, decoder, eos_id
+        self._alpha, self._length_base, self._max_length = alpha, length_base, max_length
+        self._temperature, self._from_logits = temperature, from_logits
+        self._axis, self._early_return = state_batch_axis, early_return
+
+    def __call__(self, inputs, states):
+        """inputs (N,): the first token of each item.  Returns samples (N, K, T) int32 -- the first
+        token, the tokens found, then -1 --, scores (N, K), best first, and valid_length (N, K)
+        (the first token and the end of sentence counted)."""
+        first = T.as_tensor(inputs)
+        N, K = first.shape[0], self._beam_size
+        T.require_device(first)
+        with torch.no_grad():
+            samples = torch.full((N * K, self._max_length + 1), -1, dtype=torch.int32,
+                                 device=first.device)
+            step_input = first.to(torch.int32).repeat_interleave(K)
+            samples[:, 0] = step_input
+            scores = torch.full((N, K), -float('inf'), dtype=torch.float32, device=first.device)
+            scores[:, 0] = 0.0
+            finished = None
+            pad = torch.full_like(step_input[:1], 0 if self._eos_id is None else self._eos_id)
+            steps = 0
+            for step in range(1, self._max_length + 1):
+                outputs, states = self._decoder(step_input, states)
+                scores, parents, tokens, finished = beam_search_select(
+                    outputs, scores, finished, eos_id=self._eos_id, step=step, alpha=self._alpha,
+                    length_base=self._length_base, temperature=self._temperature,
+                    normalize=self._from_logits)
+                steps = step
+                reorder_states(samples, parents, out=samples)
+                samples[:, step] = tokens.reshape(-1)
+                if step == self._max_length or self._early_return and bool(finished.all()):
+                    break
+                states = reorder_states(states, parents, batch_axis=self._axis)
+                # (a finished beam is decoded on, from the end of sentence; nothing reads it)
+                step_input = torch.where(tokens < 0, pad, tokens).reshape(-1)
+        samples = samples[:, :steps + 1].reshape(N, K, -1)
+        valid_length = (samples >= 0).sum(-1).to(torch.int32)
+        return tuple(T.like_caller(o, inputs) for o in (samples, scores, valid_length))
+
