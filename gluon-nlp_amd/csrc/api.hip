@@ -9,6 +9,7 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 #include <string>
@@ -1777,7 +1778,8 @@ int kv4_splits(const gnlp_kv4_cache *c, const gnlp_kv4_attn_desc *d) {
 }
 bool kv4_desc_sane(const gnlp_kv4_cache *c, const gnlp_kv4_attn_desc *d) {
   return c && d && d->Lq >= 0 && d->share >= 1 && c->B >= 0 && c->H >= 0 && c->slots >= 0 &&
-         d->Lq <= (1LL << 24) && d->share <= (1LL << 24) && c->B <= 65535 && c->H <= 65535 &&
+         d->Lq <= (1LL << 24) && d->share <= (1LL << 24) && d->Lq * d->share <= (1LL << 30) &&
+         c->B <= 65535 && c->H <= 65535 &&
          c->B * c->H * d->Lq * d->share > 0;
 }
 }  // namespace
@@ -1883,14 +1885,29 @@ int gnlp_beam_select(float *out_scores, int32_t *out_parents, int32_t *out_token
           (long long)d->V);
   REQUIRE(d->row_stride >= d->V, "row stride %lld < V", (long long)d->row_stride);
   REQUIRE(d->N * d->K <= 65535, "more than 65535 beams in one call");
-  REQUIRE(d->temperature > 0 && isfinite(d->temperature), "temperature must be positive");
+  REQUIRE(d->temperature >= 1e-30 && d->temperature <= 1e30,
+          "temperature %g outside [1e-30, 1e30]", d->temperature);
   REQUIRE(isfinite(d->alpha) && isfinite(d->length_base) && d->length_base > -1,
           "alpha / length_base out of range");
   REQUIRE(d->step_dev ? vl_ok((int)d->step_dtype) : d->length_base + d->step > 1.0,
           "step: a device int32 / int64, or length_base + step > 1");
+  double lp_prev = 1.0, lp_new = 1.0;
+  if (!d->step_dev) {
+    lp_prev = pow((d->length_base + d->step - 1.0) / (d->length_base + 1.0), d->alpha);
+    lp_new = pow((d->length_base + d->step) / (d->length_base + 1.0), d->alpha);
+    REQUIRE(isfinite(lp_prev) && lp_new >= 1e-30 && lp_new <= 1e30,
+            "length penalty %g / %g out of range", lp_prev, lp_new);
+  }
   if (d->N == 0) return GNLP_OK;
   REQUIRE(out_scores && out_parents && out_tokens && out_finished && outputs && scores,
           "NULL tensor");
+  const int64_t beams = d->N * d->K;
+  auto apart = [&](const void *p, int64_t n, const void *q, int64_t m) {
+    return (const char *)p + n <= (const char *)q || (const char *)q + m <= (const char *)p;
+  };
+  REQUIRE(apart(out_scores, 4 * beams, scores, 4 * beams) &&
+              (!finished || apart(out_finished, beams, finished, beams)),
+          "outputs must not alias scores or finished");
   const size_t need = gnlp_beam_select_workspace_bytes(d);
   REQUIRE(workspace && workspace_bytes >= need, "workspace too small: %zu < %zu", workspace_bytes,
           need);
@@ -1903,10 +1920,7 @@ int gnlp_beam_select(float *out_scores, int32_t *out_parents, int32_t *out_token
   a.exp_scale = (float)(1.4426950408889634 * a.inv_temperature);
   a.alpha = d->alpha; a.length_base = d->length_base;
   a.step = d->step_dev; a.step_dtype = (int)d->step_dtype;
-  if (!d->step_dev) {
-    a.lp_prev = pow((d->length_base + d->step - 1.0) / (d->length_base + 1.0), d->alpha);
-    a.lp_new = pow((d->length_base + d->step) / (d->length_base + 1.0), d->alpha);
-  }
+  a.lp_prev = lp_prev; a.lp_new = lp_new;
   a.has_eos = d->eos >= 0; a.eos = d->eos;
   a.out_scores = out_scores; a.out_parents = out_parents; a.out_tokens = out_tokens;
   a.out_finished = out_finished;
@@ -1936,6 +1950,17 @@ int gnlp_reorder_states(const gnlp_state *states, int count, int64_t N, int64_t 
     REQUIRE((t.src == t.dst) == in_place, "state %d: all in place or none", i);
     REQUIRE(t.slots_per_unit == 0 || (t.slots_per_unit > 0 && t.unit_bytes > 0),
             "state %d: bad units", i);
+    // rows, segments and outer indices have their own bytes
+    std::pair<int64_t, int64_t> dims[3] = {
+        {t.row_stride, N * K}, {t.seg_stride, t.nseg}, {t.outer_stride, t.outer}};
+    std::sort(dims, dims + 3);
+    int64_t size = t.seg_bytes;
+    for (const auto &e : dims) {
+      if (e.second == 1) continue;
+      REQUIRE(e.first >= size, "state %d: strides let rows overlap", i);
+      REQUIRE(e.first < (1LL << 61) / e.second, "state %d: strides out of range", i);
+      size += e.first * (e.second - 1);
+    }
   }
   // no destination may be read by another row, or written twice
   for (int i = 0; i < count; ++i)

@@ -166,14 +166,14 @@ __global__ void __launch_bounds__(256, E == 32 && !VEC ? 4 : 8) beam_chunk_kerne
   const uint32_t bound = wave_bound<16>(at(0) < V ? ordered(most) : 0u, a.K);
   const float wm = all_max(most);
   float s = 0.f;
-  if (wm > NEG && wm < 1e37f) {
+  if (fabsf(wm) * a.exp_scale < 4096.f) {
     // exp2(x scale - c), c = wm scale rounded: one fma; what the rounding of c adds to every term
-    // comes off the sum, r = wm scale - c exactly
+    // comes off the sum, r = wm scale - c exactly (at most 2^-13 here: 2^-r = 1 - r ln 2 to 4e-9)
     const float c = wm * a.exp_scale, r = fmaf(wm, a.exp_scale, -c);
 #pragma unroll
     for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f(fmaf(x[e], a.exp_scale, -c));
     s = all_sum(s) * (1.f - 0.6931471806f * r);
-  } else if (wm > NEG) {                   // (the product could overflow)
+  } else if (wm > NEG) {                   // (a mask of -1e9 or of the type's lowest number)
 #pragma unroll
     for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((x[e] - wm) * a.exp_scale);
     s = all_sum(s);
@@ -349,6 +349,7 @@ __global__ void __launch_bounds__(MERGE) beam_merge_kernel(BeamSelect a) {
         x = ((double)prev * lp_prev +
              (((double)z - (double)peak[k]) * a.inv_temperature - lse[k])) * per_lp;
     }
+    if (!(x == x)) x = -__builtin_inf();   // (penalties of a step on the device out of range)
   };
   auto get = [&](uint32_t c, int j, double &x, int64_t &i) {
     int32_t v = -1;

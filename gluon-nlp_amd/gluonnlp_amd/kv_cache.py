@@ -23,6 +23,7 @@ __all__ = ['QuantKVCache', 'QuantDecoderStates']
 _TIME = {'NKT': 2, 'NTK': 1, 'TNK': 0}
 _PERM = {'NKT': (0, 1, 2), 'NTK': (0, 2, 1), 'TNK': (1, 2, 0)}
 _pack3 = struct.Struct('3q').pack
+_DTYPES = {'float32': torch.float32, 'bfloat16': torch.bfloat16}
 
 
 class QuantKVCache:
@@ -35,8 +36,8 @@ class QuantKVCache:
     captured graph replays with the lengths of its time.  ``layout`` is that of the keys and values
     ('NTK', 'NKT' or 'TNK' as in ``multi_head_dot_attn``).
 
-    Tokens that would lie beyond ``max_length`` are not stored; ``extend`` refuses what it can see
-    (inside a graph it cannot).  Two writes, or a write and a reading call, on different streams
+    ``extend`` refuses tokens beyond ``max_length``; the replays of a graph cannot: there, tokens
+    beyond the buffer (``max_length`` rounded up to 32) are not stored.  Two writes, or a write and a reading call, on different streams
     have to be ordered by the caller, like any two uses of a tensor."""
 
     def __init__(self, batch_size, num_heads, head_units, max_length, num_layers=1, ctx=None,
@@ -202,7 +203,7 @@ class QuantKVCache:
             shape, strides = (B, H, n, d), _pack3(H * n * d, n * d, d)
         else:
             shape, strides = (n, B, H, d), _pack3(H * d, d, B * H * d)
-        key = self.length.new_empty(shape, dtype=T.torch_dtype(dtype))
+        key = self._length.new_empty(shape, dtype=_DTYPES.get(dtype) or T.torch_dtype(dtype))
         value = torch.empty_like(key)
         T.launch(dev, _lib.load().gnlp_kv4_read, self.layer_desc(layer), key.data_ptr(),
                  value.data_ptr(), T.code(key), n, strides, strides, self._length_ptr, _lib.I32, st,

@@ -654,7 +654,9 @@ int gnlp_kv4_attn(void *ctx, const void *q, const gnlp_kv4_cache *cache,
  * finished beams last.  NaN outputs count as -inf, +inf as the largest float; a beam whose score is
  * not above -1e15 is dead: its candidates count as -inf.  outputs of finished beams are not read.
  * out_finished = parent finished or token == eos (eos < 0: none).  step_dev: the step as a device
- * integer (graphs), else NULL and `step`.  Outputs must not alias inputs. */
+ * integer (graphs), else NULL and `step`.  Outputs must not alias inputs.  temperature: 1e-30 ..
+ * 1e30; a candidate whose score comes out as NaN (a step on the device out of range) counts as
+ * -inf. */
 typedef struct {
   int64_t N, K, V, row_stride;           /* outputs: (N * K, V), rows row_stride elements apart */
   int64_t normalize, eos, step;

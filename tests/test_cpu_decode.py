@@ -126,6 +126,47 @@ def test_bad_selections_are_refused(lib):
     assert rc(N=0) == 0
 
 
+def test_selections_out_of_range_are_refused(lib):
+    from gluonnlp_amd import _lib
+
+    def rc(out=1 << 20, out_finished=1 << 21, scores=1 << 22, finished=1 << 23, **kw):
+        d = _lib.BeamDesc()
+        d.N, d.K, d.V, d.row_stride, d.normalize, d.eos, d.step = 2, 4, 100, 100, 1, -1, 1
+        d.temperature, d.alpha, d.length_base = 1.0, 0.0, 4.0
+        for k, v in kw.items():
+            setattr(d, k, v)
+        # (no workspace: a call that gets that far ends there)
+        return lib.gnlp_beam_select(out, P, P, out_finished, P, _lib.F32, scores, finished,
+                                    ctypes.byref(d), None, 0, None), lib.gnlp_last_error()
+    assert b'workspace' in rc()[1]
+    for bad in (dict(temperature=1e-31), dict(temperature=1e31), dict(temperature=math.nan),
+                dict(alpha=1e6, step=50), dict(alpha=-1e6, step=50)):
+        code, why = rc(**bad)
+        assert code < 0 and b'range' in why or b'temperature' in why, bad
+    for bad in (dict(out=(1 << 22) + 28), dict(out_finished=1 << 23)):
+        code, why = rc(**bad)
+        assert code < 0 and b'alias' in why, bad
+
+
+def test_states_whose_rows_overlap_are_refused(lib):
+    from gluonnlp_amd import _lib
+
+    def rc(in_place=True, **kw):
+        s = _lib.State()
+        s.src, s.dst = 1 << 40, (1 << 40) if in_place else 1 << 41
+        s.outer, s.outer_stride, s.row_stride = 3, 8 * 128, 128
+        s.nseg, s.seg_stride, s.seg_bytes = 2, 64, 64
+        for k, v in kw.items():
+            setattr(s, k, v)
+        return lib.gnlp_reorder_states(ctypes.byref(s), 1, 2, 4, P, _lib.I32, None, 0, None), \
+            lib.gnlp_last_error()
+    for bad in (dict(row_stride=0), dict(row_stride=100), dict(seg_stride=32), dict(outer_stride=0),
+                dict(outer_stride=8 * 128 - 16), dict(outer_stride=1 << 62)):
+        for in_place in (True, False):
+            code, why = rc(in_place, **bad)
+            assert code < 0 and b'strides' in why, bad
+
+
 def test_bad_reorderings_are_refused(lib):
     from gluonnlp_amd import _lib
 

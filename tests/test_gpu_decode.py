@@ -475,6 +475,45 @@ def test_select_masked_places(nlp):
     assert got[3][1].all() and (got[2][1] == -1).all()
 
 
+@pytest.mark.parametrize('dtype', [BF16, F32])
+@pytest.mark.parametrize('low', [-1e4, -1e9, 'lowest'])
+def test_select_masks_of_low_values(nlp, dtype, low):
+    """Masks that are numbers: over all of a chunk of the vocabulary, over all of a row."""
+    low = torch.finfo(dtype).min if low == 'lowest' else low
+    N, K, V = 2, 4, 20000
+    g = _gen(8)
+    x = torch.randn(N, K, V, generator=g)
+    x[0, :, 3000:] = low                                   # whole chunks, and the end of one
+    x[1, 0] = low                                          # all of a beam: its tokens tie
+    x[1, 1, :19000] = low
+    s = -torch.rand(N, K, generator=g)
+    s[1, 0] = 6.0                                          # (log 20000 = 9.9: among the best)
+    for temperature in (1.0, 0.01, 30.0):
+        _check_select(nlp, x.to(dtype).cuda(), s.cuda(), None, temperature=temperature)
+
+
+def test_select_large_logits(nlp):
+    """Logits whose product with the temperature leaves float32's precise range: the differences
+    count."""
+    g = _gen(9)
+    steps = torch.randint(0, 12, (2, 3, 9000), generator=g).float()
+    s = -torch.rand(2, 3, generator=g).cuda()
+    for x in (1e9 + 64 * steps, -1e9 + 64 * steps, 3e38 + 1e37 * (steps / 4 - 1), 40000 + steps):
+        for temperature in (1.0, 100.0):
+            _check_select(nlp, x.cuda(), s, None, temperature=temperature)
+
+
+def test_select_step_on_the_device_out_of_range(nlp):
+    """lp is not a number: scores -inf, and candidates that exist (of a beam, only its K best logits
+    become candidates; they tie here, to the lowest index)."""
+    x = torch.randn(1, 3, 700, generator=_gen(10)).cuda()
+    s = -torch.rand(1, 3, generator=_gen(11)).cuda()
+    step = torch.tensor([-50], dtype=torch.int32).cuda()
+    sc, parents, tokens, done = nlp.sequence_sampler.beam_search_select(x, s, step=step, alpha=0.5)
+    assert (sc == -math.inf).all() and parents.tolist() == [[0, 0, 0]]
+    assert tokens.tolist() == [sorted(x[0, 0].topk(3).indices.tolist())] and not done.any()
+
+
 def test_select_strides_log_probabilities_and_device_step(nlp):
     N, K, V = 2, 3, 777
     g = _gen(5)
