@@ -126,12 +126,18 @@ __device__ __forceinline__ bool flag_at(const uint8_t *p, int64_t i) {
   return (*reinterpret_cast<const uint32_t *>(at & ~(uintptr_t)3) >> (8 * (at & 3))) & 0xff;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {   // (fmaxf would quieten NaNs)
+  asm("v_max3_f32 %0, %0, %1, %2" : "+v"(a) : "v"(b), "v"(c));
+  return a;
+}
+
 // E: values of a thread
 template <typename T, bool VEC, int E>
 __global__ void __launch_bounds__(256, E == 32 && !VEC ? 4 : 8) beam_chunk_kernel(BeamSelect a) {
   __shared__ uint64_t list[CAP];           // ordered value above, complement of the index below
   __shared__ uint32_t sh_n, sh_bound[4];
   __shared__ float sh_m[4], sh_s[4];
+  constexpr int GROUP = 4;                 // values that are compared with the bound together
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t row = blockIdx.y;
@@ -144,7 +150,7 @@ __global__ void __launch_bounds__(256, E == 32 && !VEC ? 4 : 8) beam_chunk_kerne
   // value e of a thread is element base + at(e)
   constexpr int PER = VEC ? 16 / (int)sizeof(T) : 1;
   auto at = [&](int e) -> uint32_t { return base + (e / PER) * (256 * PER) + tid * PER + e % PER; };
-  float x[E];
+  float x[E], top[E / GROUP];
   const bool whole = base + 256 * E <= V;
   if (VEC && whole) {
     typename VecOf<T>::type w[E / PER];
@@ -157,27 +163,48 @@ __global__ void __launch_bounds__(256, E == 32 && !VEC ? 4 : 8) beam_chunk_kerne
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = at(e) < V ? to_f32(src[at(e)]) : NEG;
   }
-  float most = NEG;
+  if (dead) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    x[e] = dead ? NEG : sane(x[e]);
-    most = fmaxf(most, x[e]);
+    for (int e = 0; e < E; ++e) x[e] = NEG;
   }
-  const uint32_t bound = wave_bound<16>(at(0) < V ? ordered(most) : 0u, a.K);
-  const float wm = all_max(most);
-  float s = 0.f;
-  if (fabsf(wm) * a.exp_scale < 4096.f) {
+  auto tops = [&]() -> float {
+    float most = NEG;
+#pragma unroll
+    for (int q = 0; q < E / GROUP; ++q) {
+      top[q] = x[q * GROUP];
+      top[q] = max3(top[q], x[q * GROUP + 1], x[q * GROUP + 2]);
+      most = max3(most, top[q], x[q * GROUP + 3]);
+      top[q] = fmaxf(top[q], x[q * GROUP + 3]);
+    }
+    return most;
+  };
+  float most = tops(), wm = all_max(most), s = 0.f;
+  bool plain = fabsf(wm) * a.exp_scale < 4096.f;
+  if (plain) {
     // exp2(x scale - c), c = wm scale rounded: one fma; what the rounding of c adds to every term
     // comes off the sum, r = wm scale - c exactly (at most 2^-13 here: 2^-r = 1 - r ln 2 to 4e-9)
     const float c = wm * a.exp_scale, r = fmaf(wm, a.exp_scale, -c);
 #pragma unroll
     for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f(fmaf(x[e], a.exp_scale, -c));
     s = all_sum(s) * (1.f - 0.6931471806f * r);
-  } else if (wm > NEG) {                   // (a mask of -1e9 or of the type's lowest number)
-#pragma unroll
-    for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((x[e] - wm) * a.exp_scale);
-    s = all_sum(s);
+    plain = s == s;
   }
+  if (!plain) {      // NaN, +inf, nothing but -inf, masks of -1e9 or of the type's lowest number
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = sane(x[e]);
+    most = tops();
+    wm = all_max(most);
+    s = 0.f;
+    if (wm > NEG) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((x[e] - wm) * a.exp_scale);
+      s = all_sum(s);
+    }
+  }
+  // A bound that K values reach: K / 4 lanes of each wave and so its least over the waves, or,
+  // where the vocabulary ends before every lane has a value, K lanes of one.
+  const bool full = V - base >= 256 * PER;
+  const uint32_t bound = wave_bound<16>(at(0) < V ? ordered(most) : 0u, full ? (a.K + 3) / 4 : a.K);
   if (lane == 0) {
     sh_bound[wave] = bound;
     sh_m[wave] = wm;
@@ -193,13 +220,19 @@ __global__ void __launch_bounds__(256, E == 32 && !VEC ? 4 : 8) beam_chunk_kerne
     a.stats[slot * 2] = m;
     a.stats[slot * 2 + 1] = t;
   }
-  const float least = unordered(max(max(sh_bound[0], sh_bound[1]), max(sh_bound[2], sh_bound[3])));
+  const uint32_t b0 = sh_bound[0], b1 = sh_bound[1], b2 = sh_bound[2], b3 = sh_bound[3];
+  const float least =
+      unordered(full ? min(min(b0, b1), min(b2, b3)) : max(max(b0, b1), max(b2, b3)));
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (x[e] >= least && (whole || at(e) < V)) {
-      const uint32_t pos = atomicAdd(&sh_n, 1u);
-      if (pos < CAP)                       // (x + 0: -0 and +0 are one value)
-        list[pos] = ((uint64_t)ordered(x[e] + 0.0f) << 32) | (uint32_t)~at(e);
+  for (int q = 0; q < E / GROUP; ++q)
+    if (top[q] >= least) {
+#pragma unroll
+      for (int e = q * GROUP; e < q * GROUP + GROUP; ++e)
+        if (x[e] >= least && (whole || at(e) < V)) {
+          const uint32_t pos = atomicAdd(&sh_n, 1u);
+          if (pos < CAP)                     // (x + 0: -0 and +0 are one value)
+            list[pos] = ((uint64_t)ordered(x[e] + 0.0f) << 32) | (uint32_t)~at(e);
+        }
     }
   __syncthreads();
   const uint32_t n = sh_n;
@@ -608,7 +641,7 @@ static int chunk_values(int64_t rows, int64_t V, int dtype) {
 }
 
 size_t beam_workspace_bytes(int64_t rows, int64_t V, int K) {     // for either dtype
-  const int64_t ch = 256 * chunk_values(rows, V, GNLP_F32), slots = rows * ((V + ch - 1) / ch);
+  const int64_t ch = 256 * 16, slots = rows * ((V + ch - 1) / ch);
   return (size_t)slots * (8 + 8 * (size_t)K);
 }
 
