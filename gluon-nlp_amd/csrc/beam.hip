@@ -634,8 +634,8 @@ __global__ void __launch_bounds__(256) reorder_kernel(Reorder a) {
 }  // namespace
 
 // Values of a thread: 64 bytes, 32 of bfloat16 where that still gives every CU a few workgroups.
-// (128 rows of 250112 bfloat16 logits: 24 us, 27 with 16; 512 rows of 32128 float32: 17 us with 16
-// and with 32; 4 rows of 32128: 5.2 us with 16, 6.3 with 32.)
+// (128 rows of 250112 bfloat16 logits: 20 us, 22 with 16, and the merge 10 us instead of 13; 512
+// rows of 32128 float32: 18 us, 20 with 32.)
 static int chunk_values(int64_t rows, int64_t V, int dtype) {
   return dtype == GNLP_BF16 && rows * ((V + 8191) / 8192) >= 1024 ? 32 : 16;
 }

@@ -690,10 +690,16 @@ void launch(const Kv4Attn &a, hipStream_t s) {
 
 }  // namespace
 
+// Splits of a sequence: up to 1024 workgroups in all at head dim 64, 512 at 128 (4 and 2 a CU, what
+// stays resident), a round of tiles for each wave at least.  bf16, one query, us with 256 / 512 /
+// 1024 workgroups: head dim 128, 32 x 8 heads x 2048 tokens 19.8 / 18.8 / 21.5, 4 x 8 heads of 4
+// queries x 32768 tokens - / 31.6 / 35.9; head dim 64, 12 heads x 131072 tokens - / 25.6 / 21.8,
+// 2 x 16 heads x 65536 tokens - / 27.4 / 26.6 (2048 workgroups, 64 x 16 heads x 1024 tokens: 24.0 and
+// a join, 1024: 18.7).
 int kv4_attn_plan(int64_t B, int64_t H, int64_t rows, int64_t keys, int64_t d) {
-  const int64_t tile = d > 64 ? 64 : 128;
+  const int64_t tile = d > 64 ? 64 : 128, aim = d > 64 ? 512 : 1024;
   const int64_t wgs = B * H * ((rows + 15) / 16), most = (keys + 4 * tile - 1) / (4 * tile);
-  int64_t n = (1024 + wgs - 1) / wgs;
+  int64_t n = (aim + wgs - 1) / wgs;
   n = n > most ? most : n;
   return (int)(n < 1 ? 1 : (n > KV4_MAX_SPLITS ? KV4_MAX_SPLITS : n));
 }
