@@ -38,16 +38,23 @@ __device__ __forceinline__ float dpp(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf,
                                                             0xf, true));
 }
+// a NaN makes these NaN
+__device__ __forceinline__ float lesser(float x, float y) {
+  return __builtin_elementwise_minimum(x, y);
+}
+__device__ __forceinline__ float greater(float x, float y) {
+  return __builtin_elementwise_maximum(x, y);
+}
 // over the 8 lanes that hold one group: quad exchanges, then the mirror of the half row
 __device__ __forceinline__ float min8(float x) {
-  x = fminf(x, dpp<0xB1>(x));
-  x = fminf(x, dpp<0x4E>(x));
-  return fminf(x, dpp<0x141>(x));
+  x = lesser(x, dpp<0xB1>(x));
+  x = lesser(x, dpp<0x4E>(x));
+  return lesser(x, dpp<0x141>(x));
 }
 __device__ __forceinline__ float max8(float x) {
-  x = fmaxf(x, dpp<0xB1>(x));
-  x = fmaxf(x, dpp<0x4E>(x));
-  return fmaxf(x, dpp<0x141>(x));
+  x = greater(x, dpp<0xB1>(x));
+  x = greater(x, dpp<0x4E>(x));
+  return greater(x, dpp<0x141>(x));
 }
 
 // word of lane row r (nibble k = element (r, k)) -> nibble t = element (t, r), over lanes 8 apart
@@ -124,39 +131,41 @@ template <typename T, bool VEC> struct Values {
   __device__ __forceinline__ float get(int e) const { return to_f32((T)v[e / N][e % N]); }
 };
 
-template <typename T, bool VEC, int UN>
-__global__ void __launch_bounds__(256) kv4_write_kernel(Kv4Io a) {
+// WHOLE: all slots of the unit are stored
+template <typename T, bool VEC, int UN, bool WHOLE>
+__device__ __forceinline__ void store(const Kv4Io &a, const Unit &u) {
   const int lane = threadIdx.x & 63;
-  const Unit u = unit_of<UN>(a);
-  if (!u.on) return;
-  const int r = lane >> 3, c = lane & 7, S = (int)a.S, d = (int)a.d;
+  const int r = lane >> 3, c = lane & 7, S = (int)a.S, d = (int)a.d, tok = tok_of(r);
   const int c0 = u.grp * 64 + 8 * c;
   const int64_t head = (int64_t)u.b * a.H + u.h;
   uint32_t *codes = (uint32_t *)(u.which ? a.v_codes : a.k_codes);
   uint32_t *par = (uint32_t *)(u.which ? a.v_par : a.k_par) + ((head << a.g_shift) + u.grp) * S;
+  const int64_t step = u.which ? a.v_stride[2] : a.k_stride[2];
   const T *src = (const T *)(u.which ? a.v : a.k) +
                  (u.which ? u.b * a.v_stride[0] + u.h * a.v_stride[1]
-                          : u.b * a.k_stride[0] + u.h * a.k_stride[1]);
-  const int64_t step = u.which ? a.v_stride[2] : a.k_stride[2];
+                          : u.b * a.k_stride[0] + u.h * a.k_stride[1]) +
+                 (u.slot0 - u.first) * step;
+  const int64_t mine = tok * step;         // (what differs between lanes)
+  const uint32_t word = u.which ? c0 + r : (uint32_t)(tok * (int)a.DP + c0) >> 3;
+  auto stored = [&](int slot) {
+    return WHOLE || (slot >= u.first && slot < u.end && slot >= 0 && slot < S);
+  };
   Values<T, VEC> in[UN];
 #pragma unroll
-  for (int k = 0; k < UN; ++k) {
-    const int slot = u.slot0 + 8 * k + tok_of(r);
-    in[k].load(slot >= u.first && slot < u.end && slot >= 0 && slot < S,
-               src + (slot - u.first) * step, c0, d);
-  }
+  for (int k = 0; k < UN; ++k)
+    in[k].load(stored(u.slot0 + 8 * k + tok), src + 8 * k * step + mine, c0, d);
 #pragma unroll
   for (int k = 0; k < UN; ++k) {
-    const int block = u.slot0 + 8 * k, slot = block + tok_of(r);
-    const bool live = slot >= u.first && slot < u.end && slot >= 0 && slot < S;
-    const uint64_t on = __ballot(live);
-    if (on == 0) continue;
+    const int block = u.slot0 + 8 * k;
+    const bool live = stored(block + tok);
+    const uint64_t on = WHOLE ? ~0ull : __ballot(live);
+    if (!WHOLE && on == 0) continue;
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = in[k].get(e);
+    uint32_t *word_at = codes + (u.which ? (head * (S >> 3) + (block >> 3)) * a.DP
+                                         : ((head * S + block) * a.DP) >> 3) + word;
     // a block that this call stores in part: nibbles of the other tokens are kept
-    uint32_t *word_at = u.which ? codes + (head * (S >> 3) + (block >> 3)) * a.DP + c0 + r
-                                : codes + (((head * S + slot) * a.DP + c0) >> 3);
     uint32_t keep = 0xffffffffu, old = 0;
     if (u.which && on != ~0ull) {
       keep = 0;
@@ -166,28 +175,25 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(Kv4Io a) {
       old = *word_at;
     }
 
-    float lo = x[0], hi = x[0], odd = 0.f;
+    float lo = x[0], hi = x[0];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 1; e < 8; ++e) {
       if (VEC || c0 + e < d) {
-        lo = fminf(lo, x[e]);
-        hi = fmaxf(hi, x[e]);
+        lo = lesser(lo, x[e]);
+        hi = greater(hi, x[e]);
       }
-      odd = fmaf(x[e], 0.f, odd);             // NaN where a value is not finite
     }
     if (c0 >= d) { lo = __builtin_inff(); hi = -__builtin_inff(); }   // (no channel of the head)
     lo = min8(lo);
     hi = max8(hi);
-    const uint64_t odds = __ballot(!(odd == 0.f));
     const bf16 sb = (bf16)((hi - lo) * (float)(1.0 / 15.0)), mb = (bf16)lo;
     float s = (float)sb;
     const float m = (float)mb, largest = 3.4028234663852886e38f;
-    const bool bad = ((odds >> (lane & 56)) & 0xff) != 0 || !(s <= largest) ||
-                     !(fabsf(m) <= largest);
+    const bool bad = !(s <= largest) || !(fabsf(m) <= largest);   // (NaN and infinities end here)
     s = s < 1.1754943508222875e-38f ? 0.f : s;
-    uint32_t word = (uint32_t)__builtin_bit_cast(uint16_t, (bf16)s) |
-                    ((uint32_t)__builtin_bit_cast(uint16_t, mb) << 16);
-    if (bad) { word = 0x7fc07fc0u; s = 0.f; }
+    uint32_t group = (uint32_t)__builtin_bit_cast(uint16_t, (bf16)s) |
+                     ((uint32_t)__builtin_bit_cast(uint16_t, mb) << 16);
+    if (bad) { group = 0x7fc07fc0u; s = 0.f; }
     // The quotient (x - m) / s, rounded as a division rounds it: the residual of an approximate
     // quotient is exact in one fma, another corrects it (exact halves, which a few in a hundred
     // bf16 values are, stay exact).  Outside the range where reciprocal and residual are normal
@@ -224,12 +230,21 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(Kv4Io a) {
     w -= high;
     if (u.which) {
       w = transpose8(w, r);
-      *word_at = (old & ~keep) | (w & keep);
+      *word_at = WHOLE ? w : (old & ~keep) | (w & keep);
     } else if (live) {
       *word_at = w;
     }
-    if (live && c == 0) par[slot] = word;
+    if (live && c == 0) par[block + tok] = group;
   }
+}
+
+template <typename T, bool VEC, int UN>
+__global__ void __launch_bounds__(256) kv4_write_kernel(Kv4Io a) {
+  const Unit u = unit_of<UN>(a);
+  if (!u.on) return;
+  const int last = u.end < (int)a.S ? u.end : (int)a.S;
+  if (u.slot0 >= u.first && u.slot0 >= 0 && u.slot0 + 8 * UN <= last) store<T, VEC, UN, true>(a, u);
+  else store<T, VEC, UN, false>(a, u);
 }
 
 template <typename T, bool VEC, int UN>
