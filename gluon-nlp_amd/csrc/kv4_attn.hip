@@ -13,9 +13,12 @@
 // Roundings: bf16 queries are exact operands, float32 ones are split into three bf16 parts; p s_v
 // is split into two (bf16 tensors: 16 bits, what they lose times 16 + n is 3e-5 of a result, a bf16
 // rounding 2e-3) or three parts (float32: all 24 bits).  For float32 23.5 = 16 + 7.5 is taken off
-// inside the matrix products (a product with a constant operand starts the accumulators, every 32
-// channels or tokens): sums over a long context would otherwise grow to 23.5 sum(p s_v) and lose the
-// digits of a result that averages out.
+// inside the matrix products, every 32 channels or tokens: their accumulators start with the largest
+// part's product with a constant operand, so that the sums that are rounded are of q (n - 7.5), not
+// of q (16 + n), which are 5 times as large and in a long average over tokens many times.  What that
+// start was rounded by is the same product once more, minus the start; it joins the lower parts,
+// which have sums of their own.  (Root of the mean square against 64 bits 4e-7 of the result for 777
+// tokens; with the start rounded 1.2e-6; a float32 attention over the dequantised cache 6e-7.)
 //
 // Work: a wave takes tiles of TT = 128 (head dim 64) or 64 tokens, 8 KB of codes, on its own, with
 // its own running maximum; four waves of a workgroup and, for few heads, several workgroups
@@ -68,6 +71,8 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
+__device__ __forceinline__ f32x4 all4(float x) { return (f32x4){x, x, x, x}; }
+
 // base: the same in all lanes
 template <typename V>
 __device__ __forceinline__ V load_at(const void *base, uint32_t off) {
@@ -86,8 +91,8 @@ __device__ __forceinline__ void split(float x, bf16 (&part)[N]) {
 
 // Waves a SIMD that the registers are cut for: as many as nothing spills with.
 constexpr int waves_of(bool f32, int DP, int R, bool bias) {
-  if (R <= 4) return (f32 ? (DP == 64 ? 3 : 2) : (DP == 64 ? 4 : 3)) -
-                     (DP == 64 && (bias || (f32 && R == 4)) ? 1 : 0);
+  if (R <= 4 && f32) return DP == 64 ? (R == 1 && !bias ? 3 : 2) : (R == 4 && bias ? 1 : 2);
+  if (R <= 4) return DP == 64 && !bias ? 4 : 3;
   return f32 ? (bias ? 1 : 2) : (bias ? 2 : 3);
 }
 
@@ -113,7 +118,6 @@ kv4_attn_kernel(Kv4Attn a) {
   constexpr float LOG2E = 1.4426950408889634f;
   // scores in units of log2 where no bias of the type's lowest number can overflow them
   constexpr float STEP = BIAS ? 8.0f : 8.0f * LOG2E, UNIT = BIAS ? LOG2E : 1.f;
-  constexpr float CENTER = F32 ? 23.5f : 16.f;    // taken off a code inside the first product
   constexpr int KROW = DP / 2, VROW = DP * 4;     // bytes of a token's K, of 8 tokens' V
 
   // per wave: scores (G, R, SROW) float, P (G, PS, R, PROW) bf16, parameters (2, G, TT), alpha (R)
@@ -226,7 +230,10 @@ kv4_attn_kernel(Kv4Attn a) {
 
   // ---- queries: operand B of K Q^T, channel 64 grp + 16 g + 8 s + j of row col ----
   bf16x8 qf[G][2][QS];
-  f32x4 start[G][F32 ? 2 : 1];           // what the accumulators start with: -CENTER sum(q)
+  // what the accumulators start with: - 16 (F32: 23.5) sum(q); F32: for the 32 channels of each product, and
+  // what its rounding lost, with the lower parts of q
+  // (the same number for all tokens)
+  float start[G][F32 ? 2 : 1], rest[G];
   float qsum[G];
   {
     const int qr = row0 + col, i = (int)((uint32_t)qr / (uint32_t)a.share);
@@ -279,13 +286,15 @@ kv4_attn_kernel(Kv4Attn a) {
     if (F32) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        start[grp][s] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        const f32x4 sum = mfma16(center, qf[grp][s][0], all4(0.f));
+        f32x4 lost = mfma16(center, qf[grp][s][0], -sum);
 #pragma unroll
-        for (int k = 0; k < QS; ++k) start[grp][s] = mfma16(center, qf[grp][s][k], start[grp][s]);
+        for (int k = 1; k < QS; ++k) lost = mfma16(center, qf[grp][s][k], lost);
+        start[grp][s] = sum[0];
+        rest[grp] = s == 0 ? lost[0] : rest[grp] + lost[0];
       }
     } else {
-      const float q0 = -CENTER * qsum[grp];
-      start[grp][0] = (f32x4){q0, q0, q0, q0};
+      start[grp][0] = -16.f * qsum[grp];
     }
   }
   int row = col;                                           // the lane's row in the softmax
@@ -309,7 +318,7 @@ kv4_attn_kernel(Kv4Attn a) {
   const T *table = BIAS && a.table ? (const T *)a.table + hq * a.table_len : nullptr;
   const uint8_t *mask = BIAS && a.mask ? a.mask + b * a.mask_stride[0] + qi * a.mask_stride[1] : nullptr;
 
-  // a score from the product without CENTER, for the token of parameters w
+  // a score from the product, for the token of parameters w
   auto scaled = [&](float dot, uint32_t w, int grp) -> float {
     const float s = scale_of(w);
     const float c = F32 ? fmaf(7.5f, s, min_of(w)) : min_of(w);
@@ -372,22 +381,28 @@ kv4_attn_kernel(Kv4Attn a) {
     const float pv = off ? 0.f : p * scale_of(w), pm = off ? 0.f : min_of(w);
     split(pv, part);
     // (the product takes 16 + n, or, F32, n - 7.5)
-    csum[grp] = fmaf(p, pm, csum[grp]);
-    csum[grp] = fmaf(F32 ? 7.5f : -16.f, pv, csum[grp]);
+    if (F32) {
+      csum[grp] = fmaf(p, off ? 0.f : fmaf(7.5f, scale_of(w), min_of(w)), csum[grp]);
+    } else {
+      csum[grp] = fmaf(p, pm, csum[grp]);
+      csum[grp] = fmaf(-16.f, pv, csum[grp]);
+    }
   };
   // O^T += V^T P^T of 32 tokens: channel 64 grp + 4 row + i of operand A's row
   auto products = [&](int s, int grp, const bf16x8 (&pb)[PS]) {
     if (F32) {
-      f32x4 from = {0.f, 0.f, 0.f, 0.f};
+      const f32x4 from = mfma16(center, pb[0], all4(0.f));
+      f32x4 lost = mfma16(center, pb[0], -from);
 #pragma unroll
-      for (int k = 0; k < PS; ++k) from = mfma16(center, pb[k], from);
+      for (int k = 1; k < PS; ++k) lost = mfma16(center, pb[k], lost);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const bf16x8 v8 = codes16(vw[s][grp][i]);
-        f32x4 o = from;
+        const f32x4 o = mfma16(v8, pb[0], from);
+        f32x4 low = lost;
 #pragma unroll
-        for (int k = 0; k < PS; ++k) o = mfma16(v8, pb[k], o);
-        acc[grp][i] += o;
+        for (int k = 1; k < PS; ++k) low = mfma16(v8, pb[k], low);
+        acc[grp][i] += o + low;
       }
     } else {
 #pragma unroll
@@ -432,16 +447,18 @@ kv4_attn_kernel(Kv4Attn a) {
           for (int e = 0; e < 4; ++e) x[(s * 2 + blk) * 4 + e] = 0.f;
 #pragma unroll
         for (int grp = 0; grp < G; ++grp) {
-          f32x4 d = start[grp][0];
+          f32x4 d = all4(start[grp][0]);
           if (F32) {
-            f32x4 d2 = start[grp][F32 ? 1 : 0];
+            f32x4 d2 = all4(start[grp][F32 ? 1 : 0]), low = all4(0.f);
             const bf16x8 k0 = codes16(kw[s][blk][grp][0]), k1 = codes16(kw[s][blk][grp][1]);
+            d = mfma16(k0, qf[grp][0][0], d);
+            d2 = mfma16(k1, qf[grp][1][0], d2);
 #pragma unroll
-            for (int k = 0; k < QS; ++k) {
-              d = mfma16(k0, qf[grp][0][k], d);
-              d2 = mfma16(k1, qf[grp][1][k], d2);
+            for (int k = 1; k < QS; ++k) {
+              low = mfma16(k0, qf[grp][0][k], low);
+              low = mfma16(k1, qf[grp][1][k], low);
             }
-            d += d2;
+            d = (d + d2) + (low + rest[grp]);
           } else {
             d = mfma16(codes16(kw[s][blk][grp][0]), qf[grp][0][0], d);
             d = mfma16(codes16(kw[s][blk][grp][1]), qf[grp][1][0], d);
