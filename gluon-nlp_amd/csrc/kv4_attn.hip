@@ -35,7 +35,10 @@
 // The next tile's K codes are requested when this one's scores are done, its V codes when this
 // one's products are: a code is dequantised out of the register that it was loaded into.
 //
-// Bound by memory: 72 bytes a token and cached head at head dim 64 (256 in bf16).
+// Bound by memory: 72 bytes a token and cached head at head dim 64 (256 in bf16).  bf16, 64 x 16
+// heads x 1024 tokens, one query: 18 us (75 MB, 4.1 TB/s; a large copy reaches 4.95); 8 x 8 heads of
+// 4 queries x 32768 tokens at head dim 128: 59 us and 5 for the join (265 MB, 4.5 TB/s).  Short calls
+// are bound by the chain of loads: 40 tokens of one sentence's 8 heads 6.5 us, an empty kernel 2.5.
 #include "common.h"
 #include "kernels.h"
 
@@ -192,7 +195,8 @@ kv4_attn_kernel(Kv4Attn a) {
     }
   };
   // the first tile does not depend on the length where no split does; where sequences are expected
-  // to reach it, it is requested before the length is known
+  // to reach it, it is requested before the length is known (64 x 16 heads x 1000 tokens: 18.7 us,
+  // 19.5 without)
   if (a.ahead) {
     fetch_k(wave, S / 32 - 1);
     fetch_v(wave, S / 32 - 1);
@@ -230,9 +234,8 @@ kv4_attn_kernel(Kv4Attn a) {
 
   // ---- queries: operand B of K Q^T, channel 64 grp + 16 g + 8 s + j of row col ----
   bf16x8 qf[G][2][QS];
-  // what the accumulators start with: - 16 (F32: 23.5) sum(q); F32: for the 32 channels of each product, and
-  // what its rounding lost, with the lower parts of q
-  // (the same number for all tokens)
+  // what the accumulators start with, the same for all tokens: -16 sum(q); F32: -23.5 sum(q) over the
+  // 32 channels of each product, and what its rounding lost, with the lower parts of q
   float start[G][F32 ? 2 : 1], rest[G];
   float qsum[G];
   {
@@ -316,7 +319,8 @@ kv4_attn_kernel(Kv4Attn a) {
     edge = (const T *)a.edge + b * a.edge_stride[0] + hq * a.edge_stride[1] +
            qi * a.edge_stride[2];
   const T *table = BIAS && a.table ? (const T *)a.table + hq * a.table_len : nullptr;
-  const uint8_t *mask = BIAS && a.mask ? a.mask + b * a.mask_stride[0] + qi * a.mask_stride[1] : nullptr;
+  const uint8_t *mask =
+      BIAS && a.mask ? a.mask + b * a.mask_stride[0] + qi * a.mask_stride[1] : nullptr;
 
   // a score from the product, for the token of parameters w
   auto scaled = [&](float dot, uint32_t w, int grp) -> float {
@@ -683,6 +687,9 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(Kv4Attn a) {
       from_f32<T>(total == 0.f ? 0.f : sum / total);
 }
 
+// Rows of a workgroup.  One query: 64 x 16 heads x 1000 tokens 18.7 us with R = 1, 21.0 with 4, 27.1
+// with 16; 8 heads x 40 tokens 6.6, 7.6 and 11.0; four queries x 32768 tokens 60 us with R = 4, 75
+// with 16.
 template <typename T, int DP, bool BIAS>
 void launch_rows(const Kv4Attn &a, hipStream_t s) {
   const int64_t rows = a.Lq * a.share;

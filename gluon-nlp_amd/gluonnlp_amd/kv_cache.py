@@ -37,8 +37,9 @@ class QuantKVCache:
     ('NTK', 'NKT' or 'TNK' as in ``multi_head_dot_attn``).
 
     ``extend`` refuses tokens beyond ``max_length``; the replays of a graph cannot: there, tokens
-    beyond the buffer (``max_length`` rounded up to 32) are not stored.  Two writes, or a write and a reading call, on different streams
-    have to be ordered by the caller, like any two uses of a tensor."""
+    beyond the buffer (``max_length`` rounded up to 32) are not stored.  Two writes, or a write and a
+    reading call, on different streams have to be ordered by the caller, like any two uses of a
+    tensor."""
 
     def __init__(self, batch_size, num_heads, head_units, max_length, num_layers=1, ctx=None,
                  layout='NTK'):
@@ -67,7 +68,8 @@ class QuantKVCache:
         self._k_par = torch.zeros(lead + (groups, slots), dtype=torch.int32, device=dev)
         self._v_par = torch.zeros(lead + (groups, slots), dtype=torch.int32, device=dev)
         self._length = torch.zeros(batch_size, dtype=torch.int32, device=dev)
-        self._bound = 0            # no sequence holds more tokens
+        self._bound = 0            # no sequence holds more tokens, as far as the host knows
+        self._replays = False      # a graph's replays may change the lengths behind its back
         self._desc = []
         for i in range(num_layers):
             c = _lib.Kv4Cache()
@@ -107,13 +109,21 @@ class QuantKVCache:
         return v if v.is_contiguous() else v.contiguous()
 
     # ---- lengths ----
+    def _capturing(self):
+        if self.device.type != 'cuda' or not torch.cuda.is_current_stream_capturing():
+            return False
+        self._replays = True
+        return True
+
     def reset(self):
         """Forget all tokens."""
+        self._capturing()
         self.length.zero_()
         self._bound = 0
 
     def set_length(self, length):
         """Set the number of tokens held, an int or a (batch_size,) vector."""
+        self._capturing()
         if isinstance(length, int):
             if not 0 <= length <= self.max_length:
                 raise ValueError('length={} is outside [0, {}]'.format(length, self.max_length))
@@ -130,9 +140,11 @@ class QuantKVCache:
             raise ValueError('n={} is outside [0, max_length={}]'.format(n, self.max_length))
         if new_length is not None:
             new_length = self._lengths(new_length, 'new_length')
-        capturing = self.device.type == 'cuda' and torch.cuda.is_current_stream_capturing()
-        if self._bound + n > self.max_length and not capturing:
-            # the bound is loose after ragged steps: look (the one place that waits for the device)
+        if self._capturing():
+            self._bound = self.max_length      # (the replays go on from lengths of their own)
+        elif self._replays or self._bound + n > self.max_length:
+            # the bound is loose after ragged steps and unknown after replays: look (the one place
+            # that waits for the device)
             self._bound = max(0, int(self.length.max()))
             grown = self._bound + n if new_length is None else \
                 int((self.length + new_length.clamp(0, n)).max())
@@ -178,7 +190,7 @@ class QuantKVCache:
             new_length = self._lengths(new_length, 'new_length')
             nl = new_length.data_ptr()
             code = _lib.I64 if new_length.dtype == torch.int64 else _lib.I32
-        elif n > self._bound:
+        elif n > self._bound and not self._replays:
             raise ValueError('write of {} tokens, {} are counted in: call extend() first'
                              .format(n, self._bound))
         T.launch(dev, _lib.load().gnlp_kv4_write, self.layer_desc(layer), k.data_ptr(),
@@ -253,6 +265,17 @@ class QuantDecoderStates:
     @property
     def length(self):
         return self.self_cache.length
+
+    def begin(self, decoder, x):
+        """Count a token in for a step of ``decoder`` on x; a call that asks for gradients is
+        refused before."""
+        if torch.is_grad_enabled() and (x.requires_grad or
+                                        any(p.requires_grad for p in decoder.parameters())):
+            raise NotImplementedError('a 4-bit cache has no gradient: decode under torch.no_grad()')
+        if x.numel() != self.self_cache.batch_size * x.shape[-1]:
+            raise ValueError('a step of {} does not fit states of {} rows'.format(
+                tuple(x.shape), self.self_cache.batch_size))
+        self.self_cache.extend(1)
 
     def reorder(self, parents):
         """Beam search: row n K + k goes on from row n K + parents[n, k].  The memory stays: the

@@ -432,7 +432,8 @@ class T5Decoder(nn.Module):
         d_model) / (L_src, items, d_model), is projected here."""
         # the bias depends on the distance alone, and not on it from max_distance on
         R = min(max_length, self.relative_position_encoder._max_distance + 1)
-        table = self.relative_position_encoder.self_attn_bias_table(R)[:, :R].contiguous()
+        table = self.relative_position_encoder.self_attn_bias_table(R)[:, :R]
+        table = table.detach().contiguous()
         return quant_decoder_states(
             mem_states, mem_valid_length, [(b.cross_attn_k, b.cross_attn_v) for b in self.layers],
             self._num_heads, self._d_kv, max_length, beam_size, self.layout, table)
@@ -445,7 +446,7 @@ class T5Decoder(nn.Module):
         torch.no_grad(); the states are updated and returned)."""
         if isinstance(past_key_values, QuantDecoderStates):
             x = T.as_tensor(step_hidden_states)
-            past_key_values.self_cache.extend(1)
+            past_key_values.begin(self, x)
             for i, layer in enumerate(self.layers):
                 x = T.as_tensor(layer.decode_cached(x, past_key_values, i))
             return T.like_caller(T.as_tensor(self.final_layer_norm(x)), step_hidden_states), \

@@ -608,7 +608,7 @@ class TransformerDecoder(nn.Module):
         if self._data_norm:
             out = self.ln_data(out)
         if isinstance(states, QuantDecoderStates):
-            states.self_cache.extend(1)
+            states.begin(self, T.as_tensor(data))
             for i in range(self.num_layers):
                 out = (self.layers[0] if self.recurrent else self.layers[i]).decode_cached(
                     out, states, i)

@@ -123,8 +123,8 @@ def reorder_states(states, parents, batch_axis=0, out=None):
     """Reorder decoding states after a selection: row n K + k along the batch axis of every tensor
     becomes its row n K + parents[n, k] (parents (N, K), values in [0, K); others are clamped).
 
-    states: a tensor, a ``QuantKVCache``, ``QuantDecoderStates``, None, or nested lists / tuples of them, as
-    ``incremental_decode`` returns them; ``batch_axis``: one int, or axes nested like the states
+    states: a tensor, a ``QuantKVCache``, ``QuantDecoderStates``, None, or nested lists / tuples of
+    them, as ``incremental_decode`` returns them; ``batch_axis``: one int, or axes nested like the states
     (a decoder's ``state_batch_axis``).  Returns the same structure: new tensors, or the tensors of
     ``out`` (nested like the states, contiguous, no overlap with the states), or, with
     ``out=states``, the states themselves, rewritten in place (K <= 32; each tensor once).  Caches

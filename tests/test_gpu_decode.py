@@ -386,6 +386,40 @@ def test_captured_steps(nlp):
         assert torch.equal(got, want[i])
 
 
+def test_lengths_that_replays_moved(nlp):
+    """After a graph's replays the host does not know the lengths: extend looks, and refuses what
+    does not fit; replays beyond the buffer store nothing and leave the rest as it was."""
+    B, H, d, room = 2, 2, 64, 32
+    c = nlp.kv_cache.QuantKVCache(B, H, d, room, ctx='cuda')
+    k = torch.randn(B, 1, H, d, generator=_gen(16)).to(BF16).cuda()
+    q = torch.ones(B, 1, H, d, dtype=BF16).cuda()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.extend(1)
+        c.write(k, k)
+        out = nlp.attention_cell.multi_head_dot_attn_cached(q, c)
+    c.reset()
+    c.extend(2)
+    c.write(torch.cat([k, -k], 1), torch.cat([k, -k], 1))
+    for _ in range(28):
+        graph.replay()
+    assert c.length.tolist() == [30, 30]
+    with pytest.raises(ValueError, match='33 tokens'):
+        c.extend(3)
+    assert c.length.tolist() == [30, 30]
+    c.extend(2)
+    c.write(torch.cat([k, k], 1), torch.cat([k, k], 1))
+    with pytest.raises(ValueError, match='33 tokens'):
+        c.extend(1)
+    before = [x.clone() for x in c.read()]
+    want = nlp.attention_cell.multi_head_dot_attn_cached(q, c)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(c.read(), before))
+        assert torch.equal(out, want)
+
+
 def test_another_stream(nlp):
     g = _gen(15)
     c, _, _, _ = _filled(nlp, g, 2, 2, 64, 1500, 1500, [1500, 700], BF16)

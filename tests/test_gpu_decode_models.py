@@ -203,6 +203,28 @@ def test_gradients_are_refused(nlp):
         m.incremental_decode(torch.randn(1, 1, 64).cuda(), None, states, None, None)
 
 
+def test_a_refused_step_counts_no_token(nlp):
+    """Gradients and steps of another shape are refused before the lengths move."""
+    for kind, shape in (('t5', (2, 1, 64)), ('post', (2, 64))):
+        m = _decoder(nlp, kind, 'NT')
+        states = m.init_quant_states(torch.randn(2, 4, 64).cuda(), None, 4)
+        assert states.bias_table is None or not states.bias_table.requires_grad
+
+        def step(x):
+            return m.incremental_decode(x, None, states, None, None) if kind == 't5' else \
+                m.incremental_decode(x, states, None, None)
+        with torch.no_grad():
+            step(torch.randn(*shape).cuda())
+            with pytest.raises(ValueError, match='rows'):
+                step(torch.randn(*((3,) + shape[1:])).cuda())
+        with pytest.raises(NotImplementedError, match='no_grad'):
+            step(torch.randn(*shape).cuda().requires_grad_(True))
+        m.requires_grad_(True)
+        with pytest.raises(NotImplementedError, match='no_grad'):
+            step(torch.randn(*shape).cuda())
+        assert states.length.tolist() == [1, 1]
+
+
 # ------------------------------------------------------------------------------------ beam search
 def _bigram(V, seed):
     g = torch.Generator().manual_seed(seed)
