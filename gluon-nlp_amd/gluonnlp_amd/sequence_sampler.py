@@ -194,8 +194,22 @@ def reorder_states(states, parents, batch_axis=0, out=None):
             outs = o if isinstance(o, (list, tuple)) else (o,) * n
             if len(axes) != n or len(outs) != n or (o is not None and outs is not o):
                 raise ValueError('batch_axis / out are not nested like the states')
-            r = [one(x, ax, ox) if type(x) is torch.Tensor else walk(x, ax, ox)
-                 for x, ax, ox in zip(s, axes, outs)]
+            r = []
+            for x, ax, ox in zip(s, axes, outs):
+                if type(x) is not torch.Tensor:
+                    r.append(walk(x, ax, ox))
+                    continue
+                # (states are mostly alike: one that is like the one before needs no more checks)
+                d = x if in_place else ox
+                if tail is None or type(d) is not torch.Tensor or ax is not last[2] or \
+                        x.shape != last[0] or x.dtype is not last[1] or x.get_device() != dev or \
+                        not x.is_contiguous() or grad and x.requires_grad or d is not x and (
+                            d.shape != last[0] or d.dtype is not last[1] or
+                            d.get_device() != dev or not d.is_contiguous()):
+                    r.append(one(x, ax, ox))
+                    continue
+                flat.extend((x.data_ptr(), d.data_ptr()) + tail)
+                r.append(d)
             return r if isinstance(s, list) else tuple(r)
         return one(s, axis, o)
 
