@@ -309,8 +309,10 @@ kv4_attn_kernel(Kv4Attn a) {
     for (int grp = 0; grp < G; ++grp) qsum[grp] = sc[grp * 16 + row];
     wave_lds_sync();
   }
-  const int qi = (int)((uint32_t)(row0 + row) / (uint32_t)a.share);
-  const int64_t hq = (int64_t)h * a.share + (row0 + row - qi * a.share);
+  // (lanes without a row see nothing, but what they load has to exist: the last row's)
+  const int at_row = row0 + (row < tile_rows ? row : tile_rows - 1);
+  const int qi = (int)((uint32_t)at_row / (uint32_t)a.share);
+  const int64_t hq = (int64_t)h * a.share + (at_row - qi * a.share);
   const int vis = row < tile_rows ? seen(qi) : 0;
   const int pos = len - ql + qi;
   const T *edge = nullptr;

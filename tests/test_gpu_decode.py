@@ -276,6 +276,29 @@ def test_attention_ragged_queries_and_empty_rows(nlp, dtype):
 
 
 @pytest.mark.parametrize('dtype', [BF16, F32])
+@pytest.mark.parametrize('Lq,share', [(5, 1), (3, 1), (19, 1), (2, 17)])
+def test_attention_biases_that_end_an_allocation(nlp, dtype, Lq, share):
+    """Bias and mask lie at the end of their memory: queries that fill a tile of rows in part read
+    nothing behind them."""
+    B, T, d = 2, 720, 64
+    g = _gen(Lq)
+    c, k, v, size = _filled(nlp, g, B, 1, d, T, T, [T, 300], dtype)
+    q = torch.randn(B, Lq, share, d, generator=g).to(dtype)
+    e = torch.randn(B, share, Lq, T, generator=g).to(dtype)
+    m = torch.rand(B, Lq, T, generator=g) < 0.8
+    room = 32 << 20                                        # (an allocation of its own)
+    ends = []
+    for x in (e, m):
+        own = torch.zeros(room // x.element_size(), dtype=x.dtype, device='cuda')
+        own[-x.numel():] = x.reshape(-1).cuda()
+        ends.append(own[-x.numel():].view(x.shape))
+    got = nlp.attention_cell.multi_head_dot_attn_cached(q.cuda(), c, edge_scores=ends[0],
+                                                        mask=ends[1])
+    want = ref.attention(q, k, v, [T, 300], share, edge=e, mask=m, temperature=8.0)
+    _check(got.reshape(B, Lq, share, d), want, ref.attention_tolerance(q, *size, T, 8.0, dtype))
+
+
+@pytest.mark.parametrize('dtype', [BF16, F32])
 def test_attention_extreme_biases(nlp, dtype):
     """-inf and the type's lowest number as masks, in part of a row and all over it; what masked
     places hold cannot matter."""
