@@ -54,10 +54,11 @@ __device__ __forceinline__ float unordered(uint32_t bits) {
   return __builtin_bit_cast(float, (bits & 0x80000000u) ? bits & 0x7fffffffu : ~bits);
 }
 
-// NaN counts as -inf (the median of three with a NaN is the smaller of the others), +inf as the
-// largest number
+// NaN counts as -inf, +inf as the largest number (by comparisons: a median of three with -inf is
+// folded to a minimum, which is the largest number for a NaN)
 __device__ __forceinline__ float sane(float x) {
-  return __builtin_amdgcn_fmed3f(x, NEG, 3.4028234663852886e38f);
+  const float largest = 3.4028234663852886e38f;
+  return x <= largest ? x : (x > largest ? largest : NEG);
 }
 
 template <int CTRL, int ROWS>

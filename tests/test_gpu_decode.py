@@ -571,6 +571,27 @@ def test_select_step_on_the_device_out_of_range(nlp):
     assert tokens.tolist() == [sorted(x[0, 0].topk(3).indices.tolist())] and not done.any()
 
 
+@pytest.mark.parametrize('dtype', [BF16, F32])
+@pytest.mark.parametrize('V', [300, 9000, 9003])
+@pytest.mark.parametrize('normalize', [False, True])
+def test_select_nan_and_infinities(nlp, dtype, V, normalize):
+    """In a few places, in most of a row, in all of a chunk and of a row; of both signs."""
+    N, K = 2, 5
+    g = _gen(V)
+    x = torch.randn(N, K, V, generator=g)
+    x[0, 0, ::3] = math.nan
+    x[0, 1, 4:] = math.nan
+    x[0, 2] = -math.nan
+    x[0, 3, : V // 2] = -math.inf
+    x[1, 0, V // 2:] = math.nan
+    x[1, 0, 7] = math.inf
+    x[1, 1, 5] = -math.nan
+    x[1, 2, 1:] = -math.inf
+    x[1, 2, 11] = math.nan
+    s = -torch.rand(N, K, generator=g)
+    _check_select(nlp, x.to(dtype).cuda(), s.cuda(), None, normalize=normalize)
+
+
 def test_select_strides_log_probabilities_and_device_step(nlp):
     N, K, V = 2, 3, 777
     g = _gen(5)
