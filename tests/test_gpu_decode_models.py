@@ -203,6 +203,17 @@ def test_gradients_are_refused(nlp):
         m.incremental_decode(torch.randn(1, 1, 64).cuda(), None, states, None, None)
 
 
+def test_bias_table_reaches_all_distances(nlp):
+    """The states keep T5's bias up to max_distance; what lies further has the last entry's."""
+    m = _decoder(nlp, 't5', 'NT')
+    far = 400
+    full = m.relative_position_encoder.self_attn_bias_table(far)[:, :far]
+    table = m.init_quant_states(torch.randn(1, 4, 64).cuda(), None, far).bias_table
+    R = table.shape[1]
+    assert R < far and torch.equal(table, full[:, far - R:])
+    assert torch.equal(full[:, :far - R], table[:, :1].expand(-1, far - R))
+
+
 def test_a_refused_step_counts_no_token(nlp):
     """Gradients and steps of another shape are refused before the lengths move."""
     for kind, shape in (('t5', (2, 1, 64)), ('post', (2, 64))):
