@@ -716,18 +716,23 @@ void launch(const Kv4Attn &a, hipStream_t s) {
 
 }  // namespace
 
-// Splits of a sequence: up to 1024 workgroups in all at head dim 64, 512 at 128 (4 and 2 a CU, what
-// stays resident), a round of tiles for each wave at least.  bf16, one query, us with 256 / 512 /
-// 1024 workgroups: head dim 128, 32 x 8 heads x 2048 tokens 19.8 / 18.8 / 21.5, 4 x 8 heads of 4
-// queries x 32768 tokens - / 31.6 / 35.9; head dim 64, 12 heads x 131072 tokens - / 25.6 / 21.8,
-// 2 x 16 heads x 65536 tokens - / 27.4 / 26.6 (2048 workgroups, 64 x 16 heads x 1024 tokens: 24.0 and
-// a join, 1024: 18.7).
+// Splits of a sequence: as many as keep all workgroups resident, 1024 at head dim 64 (4 a CU) and
+// 512 at 128 (2 a CU), and no more than give each the same number of rounds of four tiles.  One query
+// a head, us:
+//   32 x 8 heads of 128, 2048 tokens: 512 workgroups 18.8, 256 19.8, 1024 21.5
+//   64 x 16 heads of 64, 1000 tokens: 1024 workgroups 18.7, 2048 24.0 and a join
+//   4 x 12 heads of 64, 16384 tokens: 16 splits (768 workgroups, 2 rounds each) 16.0, 22 (1056; 1.5
+//   rounds, and 32 workgroups that wait for the others to end) 19.6; float32 20.8 and 27.2
+//   5 x 8 heads of 128 with 4 queries, 20000 tokens: 12 splits (480) 27.8, 13 (520) 32.4
+// 300 to 800 workgroups that hold a sequence each gain as much from 2 splits as the join costs.
 int kv4_attn_plan(int64_t B, int64_t H, int64_t rows, int64_t keys, int64_t d) {
   const int64_t tile = d > 64 ? 64 : 128, aim = d > 64 ? 512 : 1024;
-  const int64_t wgs = B * H * ((rows + 15) / 16), most = (keys + 4 * tile - 1) / (4 * tile);
-  int64_t n = (aim + wgs - 1) / wgs;
-  n = n > most ? most : n;
-  return (int)(n < 1 ? 1 : (n > KV4_MAX_SPLITS ? KV4_MAX_SPLITS : n));
+  const int64_t wgs = B * H * ((rows + 15) / 16);
+  const int64_t rounds = keys > 0 ? (keys + 4 * tile - 1) / (4 * tile) : 1;   // of four tiles
+  int64_t n = aim / wgs;
+  n = n < 1 ? 1 : (n > KV4_MAX_SPLITS ? KV4_MAX_SPLITS : n);
+  const int64_t each = (rounds + n - 1) / n;
+  return (int)((rounds + each - 1) / each);
 }
 
 void launch_kv4_attn(const Kv4Attn &a, int dtype, hipStream_t s) {
