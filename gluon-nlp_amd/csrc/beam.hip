@@ -15,9 +15,9 @@
 // (beam_merge_kernel: beams that come near each other are told apart by the logsumexp's last
 // digits).
 //   The K best of a chunk: a wave's 64 lane maxima are bisected, by ballots over the high bits of an
-//   order-preserving integer, for a bound that K lanes reach; the best bound of the four waves
+//   order-preserving integer, for a bound that K / 4 lanes reach; the least of the four waves' bounds
 //   leaves little more than K values, which a list in LDS ranks by counting.  Where ties overfill
-//   the list (a constant row), K rounds of a block-wide maximum do it.
+//   the list (a masked or a constant row), the exact bound and the first K of its ties do it.
 //   The merge does the same with the chunks' best candidates and reads on only in the lists that
 //   reach its bound, all of them at once.
 // Bound by memory (the logits once) and by the instructions of the pass: a logit's maximum, fma,
@@ -151,6 +151,17 @@ __global__ void __launch_bounds__(256, E == 32 && !VEC ? 4 : 8) beam_chunk_kerne
   if (a.finished && flag_at(a.finished, row)) return;
   const bool dead = !(a.scores[row] > -1e15f);
   const T *src = (const T *)a.outputs + row * a.row_stride;
+  const int64_t slot = row * a.chunks + chunk;
+  float *ox = a.cand_x + slot * a.K;
+  int32_t *oi = a.cand_i + slot * a.K;
+  if (dead) {                              // all of its candidates tie at -inf
+    for (int r = tid; r < a.K; r += 256) {
+      ox[r] = NEG;
+      oi[r] = base + r < V ? (int32_t)(base + r) : -1;
+    }
+    if (tid < 2) a.stats[slot * 2 + tid] = tid ? 0.f : NEG;
+    return;
+  }
   if (tid == 0) sh_n = 0;
 
   // value e of a thread is element base + at(e)
@@ -168,10 +179,6 @@ __global__ void __launch_bounds__(256, E == 32 && !VEC ? 4 : 8) beam_chunk_kerne
   } else {
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = at(e) < V ? to_f32(src[at(e)]) : NEG;
-  }
-  if (dead) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = NEG;
   }
   auto tops = [&]() -> float {
     float most = NEG;
@@ -210,14 +217,18 @@ __global__ void __launch_bounds__(256, E == 32 && !VEC ? 4 : 8) beam_chunk_kerne
   // A bound that K values reach: K / 4 lanes of each wave and so its least over the waves, or,
   // where the vocabulary ends before every lane has a value, K lanes of one.
   const bool full = V - base >= 256 * PER;
-  const uint32_t bound = wave_bound<16>(at(0) < V ? ordered(most) : 0u, full ? (a.K + 3) / 4 : a.K);
+  const int of_wave = full ? (a.K + 3) / 4 : a.K;
+  const uint32_t key = at(0) < V ? ordered(most) : 0u, bound = wave_bound<16>(key, of_wave);
+  auto shared_bound = [&]() -> float {
+    const uint32_t b0 = sh_bound[0], b1 = sh_bound[1], b2 = sh_bound[2], b3 = sh_bound[3];
+    return unordered(full ? min(min(b0, b1), min(b2, b3)) : max(max(b0, b1), max(b2, b3)));
+  };
   if (lane == 0) {
     sh_bound[wave] = bound;
     sh_m[wave] = wm;
     sh_s[wave] = s;
   }
   __syncthreads();
-  const int64_t slot = row * a.chunks + chunk;
   if (tid == 0) {
     const float m = fmaxf(fmaxf(sh_m[0], sh_m[1]), fmaxf(sh_m[2], sh_m[3]));
     float t = 0.f;
@@ -226,24 +237,51 @@ __global__ void __launch_bounds__(256, E == 32 && !VEC ? 4 : 8) beam_chunk_kerne
     a.stats[slot * 2] = m;
     a.stats[slot * 2 + 1] = t;
   }
-  const uint32_t b0 = sh_bound[0], b1 = sh_bound[1], b2 = sh_bound[2], b3 = sh_bound[3];
-  const float least =
-      unordered(full ? min(min(b0, b1), min(b2, b3)) : max(max(b0, b1), max(b2, b3)));
+  auto push = [&](float v, uint32_t i) {
+    const uint32_t pos = atomicAdd(&sh_n, 1u);
+    if (pos < CAP)                         // (v + 0: -0 and +0 are one value)
+      list[pos] = ((uint64_t)ordered(v + 0.0f) << 32) | (uint32_t)~i;
+  };
+  const float least = shared_bound();
 #pragma unroll
   for (int q = 0; q < E / GROUP; ++q)
     if (top[q] >= least) {
 #pragma unroll
       for (int e = q * GROUP; e < q * GROUP + GROUP; ++e)
-        if (x[e] >= least && (whole || at(e) < V)) {
-          const uint32_t pos = atomicAdd(&sh_n, 1u);
-          if (pos < CAP)                     // (x + 0: -0 and +0 are one value)
-            list[pos] = ((uint64_t)ordered(x[e] + 0.0f) << 32) | (uint32_t)~at(e);
-        }
+        if (x[e] >= least && (whole || at(e) < V)) push(x[e], at(e));
     }
   __syncthreads();
-  const uint32_t n = sh_n;
-  float *ox = a.cand_x + slot * a.K;
-  int32_t *oi = a.cand_i + slot * a.K;
+  uint32_t n = sh_n;
+  if (n > CAP) {
+    // Ties overfill the list (a mask, a constant row): the same with the bound to its last bit, what
+    // lies above it and, in the order of their indices, K of what equals it.
+    const uint32_t last = wave_bound<0>(key, of_wave);
+    __syncthreads();
+    if (lane == 0) sh_bound[wave] = last;
+    if (tid == 0) sh_n = 0;
+    __syncthreads();
+    const float tie = shared_bound();
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (x[e] > tie && (whole || at(e) < V)) push(x[e], at(e));
+    int ties = 0;
+    for (int v = 0; v < E && ties < a.K; ++v) {
+      const uint32_t i = base + v * 256 + tid;
+      const bool is = i < V && sane(to_f32(src[i])) == tie;
+      const uint64_t on = __ballot(is);
+      __syncthreads();
+      if (lane == 0) sh_bound[wave] = (uint32_t)__popcll(on);
+      __syncthreads();
+      int before = ties + (int)__popcll(on & ((1ull << lane) - 1));
+      for (int w = 0; w < 4; ++w) {
+        if (w < wave) before += (int)sh_bound[w];
+        ties += (int)sh_bound[w];
+      }
+      if (is && before < a.K) push(tie, i);
+    }
+    __syncthreads();
+    n = sh_n;
+  }
   if (n <= CAP) {
     for (uint32_t c = tid; c < n; c += 256) {
       const uint64_t key = list[c];
@@ -258,7 +296,8 @@ __global__ void __launch_bounds__(256, E == 32 && !VEC ? 4 : 8) beam_chunk_kerne
     for (int r = (int)n + tid; r < a.K; r += 256) oi[r] = -1;
     return;
   }
-  // ties overfill the list: K times the best of what is left, over the whole workgroup
+  // still too many (values that differ in their last bits): K times the best of what is left, over
+  // the whole workgroup
   __syncthreads();
   float tx = __builtin_inff();
   uint32_t ti = 0;
@@ -420,7 +459,7 @@ __global__ void __launch_bounds__(MERGE) beam_merge_kernel(BeamSelect a) {
     any |= i != none;
     mx = fmax(mx, x);
   }
-  const uint32_t bound = wave_bound<8>(any ? (uint32_t)(ordered(mx) >> 32) : 0u, K);
+  const uint32_t key = any ? (uint32_t)(ordered(mx) >> 32) : 0u, bound = wave_bound<8>(key, K);
   if (lane == 0) sh_bound[wave] = bound;
   __syncthreads();
   uint32_t least = 0;
@@ -433,29 +472,49 @@ __global__ void __launch_bounds__(MERGE) beam_merge_kernel(BeamSelect a) {
       if (pos < LIST) live[pos] = c;
     }
   };
+  uint32_t nlive, found;
+  for (int again = 0;; ++again) {
 #pragma unroll
-  for (int r = 0; r < AHEAD; ++r) keep(tid + r * MERGE, hx[r], has[r]);
-  for (uint32_t c = tid + AHEAD * MERGE; c < lists; c += MERGE) {
-    double x;
-    int64_t i;
-    get(c, 0, x, i);
-    keep(c, x, i != none);
-  }
-  __syncthreads();
-  const uint32_t nlive = sh_live;
-  if (nlive <= LIST)
-    for (uint32_t q = tid; q < nlive * (uint32_t)K; q += MERGE) {
-      const uint32_t l = q / (uint32_t)K;
+    for (int r = 0; r < AHEAD; ++r) keep(tid + r * MERGE, hx[r], has[r]);
+    for (uint32_t c = tid + AHEAD * MERGE; c < lists; c += MERGE) {
       double x;
       int64_t i;
-      get(live[l], (int)(q - l * K), x, i);
-      if (i != none && (uint32_t)(ordered(x) >> 32) >= least) {
-        const uint32_t pos = atomicAdd(&sh_n, 1u);
-        if (pos < LIST) { sx[pos] = x; si[pos] = i; }
-      }
+      get(c, 0, x, i);
+      keep(c, x, i != none);
     }
-  __syncthreads();
-  const uint32_t found = sh_n;
+    __syncthreads();
+    nlive = sh_live;
+    if (nlive <= LIST)
+      for (uint32_t q = tid; q < nlive * (uint32_t)K; q += MERGE) {
+        const uint32_t l = q / (uint32_t)K;
+        double x;
+        int64_t i;
+        get(live[l], (int)(q - l * K), x, i);
+        if (i != none && (uint32_t)(ordered(x) >> 32) >= least) {
+          const uint32_t pos = atomicAdd(&sh_n, 1u);
+          if (pos < LIST) { sx[pos] = x; si[pos] = i; }
+        }
+      }
+    __syncthreads();
+    found = sh_n;
+    // (ranking is quadratic)
+    const bool fits = nlive <= LIST && found <= LIST / 4;
+    if (again || fits) {
+      if (again && found < (uint32_t)K) nlive = LIST + 1;   // (-inf is among the K best)
+      break;
+    }
+    // too many, most likely of -inf (dead beams, masks): once more without those, and above what
+    // K / 8 lanes of every wave reach
+    const uint32_t every = wave_bound<8>(key, (K + WAVES - 1) / WAVES);
+    __syncthreads();
+    if (lane == 0) sh_bound[wave] = every;
+    if (tid == 0) { sh_n = 0; sh_live = 0; }
+    __syncthreads();
+    uint32_t shared = 0xffffffffu;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) shared = min(shared, sh_bound[w]);
+    least = max(max(least, shared), 0x00100000u);
+  }
   auto put = [&](int rank, double x, int64_t i) {
     const int64_t to = item * K + rank;
     const bool was = (i >> 32) == K;
@@ -488,7 +547,9 @@ __global__ void __launch_bounds__(MERGE) beam_merge_kernel(BeamSelect a) {
         int64_t i;
         get(c, j, x, i);
         if (i == none) break;
-        if ((r == 0 || better(tx, ti, x, i)) && better(x, i, bx, bi)) { bx = x; bi = i; }
+        if (r > 0 && !better(tx, ti, x, i)) continue;      // (taken)
+        if (better(x, i, bx, bi)) { bx = x; bi = i; }
+        break;                                             // (the best that the list has left)
       }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {

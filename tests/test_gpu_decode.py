@@ -549,6 +549,34 @@ def test_select_masks_of_low_values(nlp, dtype, low):
         _check_select(nlp, x.to(dtype).cuda(), s.cuda(), None, temperature=temperature)
 
 
+@pytest.mark.parametrize('dtype', [BF16, F32])
+@pytest.mark.parametrize('N,K,V', [(2, 16, 40000), (1, 32, 9000), (3, 8, 250112), (2, 5, 4099)])
+def test_select_ties_that_overfill_the_lists(nlp, dtype, N, K, V):
+    """Masks but for a few tokens, constant rows, two values, dead and finished beams among them."""
+    g = _gen(K)
+    s = -torch.rand(N, K, generator=g)
+    dead = s.clone()
+    dead[:, 1:] = -math.inf
+    base = torch.randn(N, K, V, generator=g)
+    masked = base.clone()
+    masked[:, :, 100:] = -math.inf
+    few = torch.full_like(base, -math.inf)
+    few[:, :, V // 2] = 1.0
+    few[:, :, V - 1] = 2.0
+    two = (base > 1.0).float()
+    most = torch.where(base < 3.0, torch.zeros_like(base), base)
+    f = torch.rand(N, K, generator=g) < 0.4
+    for x in (masked, few, two, most, torch.full_like(base, -3.0)):
+        x = x.to(dtype).cuda()
+        for scores in (s, dead):
+            _check_select(nlp, x, scores.cuda(), None)
+            _check_select(nlp, x, scores.cuda(), f.cuda(), eos_id=V // 2)
+    _check_select(nlp, base.to(dtype).cuda(), dead.cuda(), None)
+    close = (1.0 + 1e-6 * base).float()                    # values that differ in their last bits
+    if dtype == F32:
+        _check_select(nlp, close.cuda(), s.cuda(), None)
+
+
 def test_select_large_logits(nlp):
     """Logits whose product with the temperature leaves float32's precise range: the differences
     count."""
