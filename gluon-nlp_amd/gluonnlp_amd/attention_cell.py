@@ -374,7 +374,8 @@ def multi_head_dot_attn_cached(query, cache, layer=0, *, causal: bool = True, ed
     if B != cache.batch_size or d != cache.head_units or H % cache.num_heads or H == 0:
         raise ValueError('query {} (layout {}) does not match {}'.format(tuple(shape), layout,
                                                                         cache))
-    if (q.requires_grad or e is not None or table is not None) and wants_grad(q, e, table):
+    if torch.is_grad_enabled() and (q.requires_grad or e is not None and e.requires_grad or
+                                    table is not None and table.requires_grad):
         raise NotImplementedError('attention over a 4-bit cache has no gradient: decode under '
                                   'torch.no_grad()')
     st = q.stride()
