@@ -141,7 +141,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {   // (fmaxf w
 template <typename T, bool VEC, int E>
 __global__ void __launch_bounds__(256, E == 32 && !VEC ? 4 : 8) beam_chunk_kernel(BeamSelect a) {
   __shared__ uint64_t list[CAP];           // ordered value above, complement of the index below
-  __shared__ uint32_t sh_n, sh_bound[4];
+  __shared__ uint32_t sh_n, sh_bound[4], sh_same[4];
   __shared__ float sh_m[4], sh_s[4];
   constexpr int GROUP = 4;                 // values that are compared with the bound together
   const int tid = threadIdx.x, lane = tid & 63;
@@ -223,8 +223,10 @@ __global__ void __launch_bounds__(256, E == 32 && !VEC ? 4 : 8) beam_chunk_kerne
     const uint32_t b0 = sh_bound[0], b1 = sh_bound[1], b2 = sh_bound[2], b3 = sh_bound[3];
     return unordered(full ? min(min(b0, b1), min(b2, b3)) : max(max(b0, b1), max(b2, b3)));
   };
+  const bool alike = __all(most == wm);
   if (lane == 0) {
     sh_bound[wave] = bound;
+    sh_same[wave] = alike;
     sh_m[wave] = wm;
     sh_s[wave] = s;
   }
@@ -242,28 +244,37 @@ __global__ void __launch_bounds__(256, E == 32 && !VEC ? 4 : 8) beam_chunk_kerne
     if (pos < CAP)                         // (v + 0: -0 and +0 are one value)
       list[pos] = ((uint64_t)ordered(v + 0.0f) << 32) | (uint32_t)~i;
   };
-  const float least = shared_bound();
+  // one largest value in every lane (a chunk that is masked throughout): nothing lies above it
+  const bool constant = (sh_same[0] & sh_same[1] & sh_same[2] & sh_same[3]) && sh_m[0] == sh_m[1] &&
+                        sh_m[0] == sh_m[2] && sh_m[0] == sh_m[3];
+  uint32_t n = CAP + 1;
+  if (!constant) {
+    const float least = shared_bound();
 #pragma unroll
-  for (int q = 0; q < E / GROUP; ++q)
-    if (top[q] >= least) {
+    for (int q = 0; q < E / GROUP; ++q)
+      if (top[q] >= least) {
 #pragma unroll
-      for (int e = q * GROUP; e < q * GROUP + GROUP; ++e)
-        if (x[e] >= least && (whole || at(e) < V)) push(x[e], at(e));
-    }
-  __syncthreads();
-  uint32_t n = sh_n;
+        for (int e = q * GROUP; e < q * GROUP + GROUP; ++e)
+          if (x[e] >= least && (whole || at(e) < V)) push(x[e], at(e));
+      }
+    __syncthreads();
+    n = sh_n;
+  }
   if (n > CAP) {
     // Ties overfill the list (a mask, a constant row): the same with the bound to its last bit, what
     // lies above it and, in the order of their indices, K of what equals it.
-    const uint32_t last = wave_bound<0>(key, of_wave);
-    __syncthreads();
-    if (lane == 0) sh_bound[wave] = last;
-    if (tid == 0) sh_n = 0;
-    __syncthreads();
-    const float tie = shared_bound();
+    float tie = sh_m[0];
+    if (!constant) {
+      const uint32_t last = wave_bound<0>(key, of_wave);
+      __syncthreads();
+      if (lane == 0) sh_bound[wave] = last;
+      if (tid == 0) sh_n = 0;
+      __syncthreads();
+      tie = shared_bound();
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (x[e] > tie && (whole || at(e) < V)) push(x[e], at(e));
+      for (int e = 0; e < E; ++e)
+        if (x[e] > tie && (whole || at(e) < V)) push(x[e], at(e));
+    }
     int ties = 0;
     for (int v = 0; v < E && ties < a.K; ++v) {
       const uint32_t i = base + v * 256 + tid;
