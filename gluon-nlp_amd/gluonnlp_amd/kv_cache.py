@@ -37,7 +37,8 @@ class QuantKVCache:
     ('NTK', 'NKT' or 'TNK' as in ``multi_head_dot_attn``).
 
     ``extend`` refuses tokens beyond ``max_length``; the replays of a graph cannot: there, tokens
-    beyond the buffer (``max_length`` rounded up to 32) are not stored.  Two writes, or a write and a
+    beyond the buffer (``max_length`` rounded up to 32) are not stored.  Once a graph has captured a
+    change of the lengths, an ``extend`` outside of it reads them back first.  Two writes, or a write and a
     reading call, on different streams have to be ordered by the caller, like any two uses of a
     tensor."""
 

@@ -39,3 +39,12 @@ def test_gemm_with_the_build_flags(tmp_path):
     for key in ('vgpr_spill_count', 'private_segment_fixed_size'):
         vals = [int(v) for v in re.findall(r'\.%s:\s+(\d+)' % key, text)]
         assert len(vals) == 24 and not any(vals), (key, vals)
+
+
+@pytest.mark.parametrize('name', ['kv4.hip', 'kv4_attn.hip', 'beam.hip'])
+def test_decoding_kernels_with_the_build_flags(tmp_path, name):
+    """Registers are cut to the waves that a SIMD is to hold: nothing may be spilled for it."""
+    text = _assembly(name, tmp_path / 'k.s')
+    assert not re.search(r'v_pk_(add|mul|fma)_f32', text)
+    vals = [int(v) for v in re.findall(r'\.vgpr_spill_count:\s+(\d+)', text)]
+    assert vals and not any(vals), vals
