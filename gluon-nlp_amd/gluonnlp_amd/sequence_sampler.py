@@ -26,6 +26,21 @@ def _select_workspace(N, K, V):
     return _lib.load().gnlp_beam_select_workspace_bytes(ctypes.byref(d))
 
 
+def _row_stride(shape, stride):
+    """Elements between the rows of logits (N, K, V) or (rows, V); 0 where they are not V neighbouring
+    elements each, at one distance.  The stride of an axis of one element says nothing: a transposed
+    or sliced view keeps whatever it was, and ``contiguous`` leaves it."""
+    V = shape[-1]
+    if V > 1 and stride[-1] != 1:
+        return 0
+    axes = [(n, st) for n, st in zip(shape[:-1], stride) if n != 1]
+    if not axes:
+        return V
+    if len(axes) == 2 and axes[0][1] != axes[1][0] * axes[1][1]:
+        return 0
+    return axes[-1][1]
+
+
 def beam_search_select(outputs, scores, finished=None, *, eos_id=None, step=1, alpha=0.0,
                        length_base=None, temperature=1.0, normalize=True):
     """One step of a beam search over N items of K beams (K <= 32).
@@ -60,10 +75,10 @@ def beam_search_select(outputs, scores, finished=None, *, eos_id=None, step=1, a
         raise ValueError('outputs {} do not match scores {}'.format(tuple(shape), tuple(s.shape)))
     if (x.requires_grad or s.requires_grad) and torch.is_grad_enabled():
         raise NotImplementedError('the selection has no gradient: search under torch.no_grad()')
-    V, st = shape[-1], x.stride()
-    if st[-1] != 1 and V > 1 or len(st) == 3 and st[0] != K * st[1] or st[-2] < V:
-        x = x.contiguous()
-        st = x.stride()
+    V = shape[-1]
+    row_stride = V if x.is_contiguous() else _row_stride(shape, x.stride())
+    if row_stride < V:
+        x, row_stride = x.contiguous(), V
     if not s.is_contiguous():
         s = s.contiguous()
     fp = None
@@ -84,9 +99,9 @@ def beam_search_select(outputs, scores, finished=None, *, eos_id=None, step=1, a
         step_ptr = step.data_ptr()
         step_code = _lib.I64 if step.dtype == torch.int64 else _lib.I32
         step = 0
-    desc = _BEAM_DESC.pack(N, K, V, st[-2], bool(normalize), -1 if eos_id is None else int(eos_id),
-                           step, step_ptr, step_code, temperature, alpha,
-                           K if length_base is None else length_base)
+    desc = _BEAM_DESC.pack(N, K, V, row_stride, bool(normalize),
+                           -1 if eos_id is None else int(eos_id), step, step_ptr, step_code,
+                           temperature, alpha, K if length_base is None else length_base)
     out_scores = torch.empty_like(s)
     parents, tokens = s.new_empty((2, N, K), dtype=torch.int32).unbind(0)
     out_finished = s.new_empty((N, K), dtype=torch.bool)

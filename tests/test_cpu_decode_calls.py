@@ -1,0 +1,75 @@
+"""What the wrappers of the decoding operators hand to the C entries, seen with the launch taken out:
+strides, what is refused, and what has run when it is.  No GPU."""
+import ctypes
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope='module')
+def nlp():
+    import gluonnlp_amd
+    return gluonnlp_amd
+
+
+@pytest.fixture
+def calls(nlp, monkeypatch):
+    """The arguments of the launches that a call would make; CPU tensors count as device 0's."""
+    got = []
+    monkeypatch.setattr(nlp._tensor, 'device_index', lambda first, *rest: 0)
+    monkeypatch.setattr(nlp._tensor, 'require_device', lambda *tensors: torch.device('cpu'))
+    monkeypatch.setattr(nlp._tensor, 'launch', lambda index, fn, *args: got.append(args))
+    return got
+
+
+# logits (N, K, V) or (N K, V) as views -> (view, beams); element (r, v) of all rows is 1000 r + v
+def _views():
+    N, V = 4, 50
+    rows = torch.arange(N)[:, None] * 1000.0 + torch.arange(V)
+    return {
+        'time-major, one beam': (rows[None].transpose(0, 1), 1),
+        'unsqueezed': (rows.unsqueeze(1), 1),
+        'one beam, wide rows': (torch.cat([rows, rows], 1)[:, :V].unsqueeze(1), 1),
+        'one row, 3-d': (rows[:1, None], 1),
+        'one row of many columns': (rows.t().contiguous()[:, :1].t(), 1),
+        'a column as a row': (rows[0].reshape(V, 1).t(), 1),
+        'a column as a row, 3-d': (rows[0].reshape(V, 1, 1).transpose(0, 2), 1),
+        'one item': (rows[None], N),
+        'one item, last of a wider tensor': (torch.stack([rows, rows])[1:], N),
+        'one item, wide rows': (torch.cat([rows, rows], 1)[None, :, :V], N),
+        'two items': (rows.reshape(2, 2, V), 2),
+        'two items, beams first': (rows.reshape(2, 2, V).transpose(0, 1).contiguous()
+                                   .transpose(0, 1), 2),
+        'two items, wide': (torch.cat([rows, rows], 1).reshape(2, 2, 2 * V)[..., :V], 2),
+        'every other beam': (rows.reshape(2, 2, V).repeat_interleave(2, 1)[:, ::2], 2),
+        'beams of longer items': (torch.cat([rows.reshape(2, 2, V)] * 2, 1)[:, :2], 2),
+        'expanded': (rows[:1].expand(4, V), 2),
+        'one token': (rows[:, :1], 2),
+        'one token, expanded': (rows[:1, :1].expand(4, 1), 2),
+        'one token, 3-d, one beam': (rows[:, :1, None].transpose(1, 2), 1),
+    }
+
+
+@pytest.mark.parametrize('name', sorted(_views()))
+def test_rows_of_the_logits(nlp, monkeypatch, calls, name):
+    """Row r is V neighbouring elements, r row strides from the pointer, whatever the view's strides
+    of axes of one element are; none of it lies outside the tensor."""
+    x, K = _views()[name]
+    V = x.shape[-1]
+    N = x.numel() // V // K
+    first = x.untyped_storage().data_ptr()
+    end = first + x.untyped_storage().nbytes()
+    seen = []
+
+    def read(index, fn, *args):             # (at the call: a copy made for it lives that long)
+        d, at = nlp._lib.BeamDesc.from_buffer_copy(args[8]), args[4]
+        assert (d.N, d.K, d.V) == (N, K, V) and d.row_stride >= V
+        if first <= at < end:
+            assert at + 4 * ((N * K - 1) * d.row_stride + V) <= end
+        else:
+            assert d.row_stride == V
+        seen.append(torch.stack([torch.tensor((ctypes.c_float * V).from_address(
+            at + 4 * r * d.row_stride)[:]) for r in range(N * K)]))
+    monkeypatch.setattr(nlp._tensor, 'launch', read)
+    nlp.sequence_sampler.beam_search_select(x, torch.zeros(N, K))
+    assert len(seen) == 1 and torch.equal(seen[0], x.reshape(N * K, V))

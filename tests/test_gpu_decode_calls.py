@@ -1,0 +1,41 @@
+"""Calls of the decoding operators that their documentation allows and ordinary use does not make, on
+the GPU against the plain evaluations in 64 bits (tests/decode_ref.py)."""
+import math
+
+import pytest
+import torch
+
+from tests import decode_ref as ref
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope='module')
+def nlp():
+    import gluonnlp_amd
+    return gluonnlp_amd
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+@pytest.mark.parametrize('dtype', [BF16, F32])
+def test_select_from_views_with_axes_of_one(nlp, dtype):
+    """One beam an item, logits as a view of a time-major output; one row as a view of a column."""
+    N, V = 4, 1000
+    g = _gen(1)
+    rows = (3 * torch.randn(N, V, generator=g)).to(dtype).cuda()
+    s = -torch.rand(N, 1, generator=g).cuda()
+    want = ref.select(rows, s, None)
+    for x in (rows[None].transpose(0, 1), rows.unsqueeze(1), rows):
+        got = nlp.sequence_sampler.beam_search_select(x, s)
+        assert torch.equal(got[1].cpu().long(), want[1])
+        assert torch.equal(got[2].cpu().long(), want[2])
+        # a logsumexp off by a few half steps of the largest term, the score rounded once
+        assert ((got[0].cpu().double() - want[0]).abs()
+                <= (want[0].abs() + 20) * 2.0 ** -24 * 8).all()
+    for x in (rows[0].reshape(V, 1).t(), rows[0].reshape(V, 1, 1).transpose(0, 2)):
+        got = nlp.sequence_sampler.beam_search_select(x, s[:1])
+        assert got[2].cpu().long().tolist() == want[2][:1].tolist()
