@@ -399,7 +399,9 @@ def multi_head_dot_attn_cached(query, cache, layer=0, *, causal: bool = True, ed
         if e.dtype != q.dtype:
             e = e.to(q.dtype)
         e, Lm = _expand_keys(e, (B, H, Lq), slots)
-        ep, es = e.data_ptr(), e.stride()
+        # (a tensor without elements has no address, and NULL would say that there is none: one over no
+        # keys is passed as another address, which is not read)
+        ep, es = e.data_ptr() or ctx.data_ptr(), e.stride()
     elif table is not None:
         if table.dim() != 2 or table.shape[0] != H or table.shape[1] < 1:
             raise ValueError('edge_table {} != (heads = {}, R >= 1)'.format(tuple(table.shape), H))
@@ -413,7 +415,7 @@ def multi_head_dot_attn_cached(query, cache, layer=0, *, causal: bool = True, ed
         if e is not None and Lm != Lmm and slots not in (Lm, Lmm):
             raise ValueError('edge_scores reach {} keys, mask {}'.format(Lm, Lmm))
         Lm = min(Lm, Lmm)
-        mp, ms = m.data_ptr(), m.stride()
+        mp, ms = m.data_ptr() or ctx.data_ptr(), m.stride()
     t = math.sqrt(d if query_head_units is None else query_head_units) if scaled else 0.0
     share = H // cache.num_heads
     keys = (cache._bound + 255) // 256 * 256       # (a hint: rounded so that plans repeat)

@@ -73,3 +73,18 @@ def test_rows_of_the_logits(nlp, monkeypatch, calls, name):
     monkeypatch.setattr(nlp._tensor, 'launch', read)
     nlp.sequence_sampler.beam_search_select(x, torch.zeros(N, K))
     assert len(seen) == 1 and torch.equal(seen[0], x.reshape(N * K, V))
+
+
+@pytest.mark.parametrize('given', ['edge_scores', 'mask', 'both'])
+def test_a_bias_or_mask_over_no_keys_is_given(nlp, calls, given):
+    """Its address is not NULL, which would let every key through, and it reaches 0 keys."""
+    B, H, Lq, d = 2, 3, 2, 64
+    c = nlp.kv_cache.QuantKVCache(B, H, d, 40, ctx='cpu')
+    c.set_length(40)
+    e, m = torch.zeros(B, H, Lq, 40), torch.ones(B, Lq, 40, dtype=torch.bool)
+    kw = {'edge_scores': dict(edge_scores=e[..., :0]), 'mask': dict(mask=m[..., :0]),
+          'both': dict(edge_scores=e[:1, ..., :0], mask=m[..., :1])}[given]
+    nlp.attention_cell.multi_head_dot_attn_cached(torch.zeros(B, Lq, H, d), c, **kw)
+    a = nlp._lib.Kv4AttnDesc.from_buffer_copy(calls[0][3])
+    assert a.Lm == 0
+    assert bool(a.edge_scores) == ('edge_scores' in kw) and bool(a.mask) == ('mask' in kw)

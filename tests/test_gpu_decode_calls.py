@@ -39,3 +39,26 @@ def test_select_from_views_with_axes_of_one(nlp, dtype):
     for x in (rows[0].reshape(V, 1).t(), rows[0].reshape(V, 1, 1).transpose(0, 2)):
         got = nlp.sequence_sampler.beam_search_select(x, s[:1])
         assert got[2].cpu().long().tolist() == want[2][:1].tolist()
+
+
+@pytest.mark.parametrize('dtype', [BF16, F32])
+def test_attention_with_a_bias_or_mask_over_no_keys(nlp, dtype):
+    """Keys from Lm on are not seen; with Lm = 0 nothing is, and the result is zeros."""
+    B, H, Lq, d, T = 2, 3, 2, 64, 700
+    g = _gen(2)
+    c = nlp.kv_cache.QuantKVCache(B, H, d, T, ctx='cuda')
+    c.set_length(T)
+    x = torch.randn(B, T, H, d, generator=g).to(dtype).cuda()
+    c.write(x, x)
+    q = torch.randn(B, Lq, H, d, generator=g).to(dtype).cuda()
+    e, m = torch.zeros(B, H, Lq, T).cuda(), torch.ones(B, Lq, T, dtype=torch.bool).cuda()
+    table = torch.zeros(H, 5).to(dtype).cuda()
+    for kw in (dict(edge_scores=e[..., :0]), dict(mask=m[..., :0]), dict(mask=m[:1, :1, :0]),
+               dict(edge_scores=e[..., :0], mask=m[..., :1]),
+               dict(edge_scores=e[..., :0], mask=m[..., :0]),
+               dict(edge_table=table, mask=m[..., :0])):
+        for causal in (True, False):
+            for bound in (1, T):                   # one and several workgroups a sequence
+                c._bound = bound
+                got = nlp.attention_cell.multi_head_dot_attn_cached(q, c, causal=causal, **kw)
+                assert got.shape == (B, Lq, H * d) and (got == 0).all()
