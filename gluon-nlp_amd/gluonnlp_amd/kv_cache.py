@@ -123,7 +123,8 @@ class QuantKVCache:
         self._bound = 0
 
     def set_length(self, length):
-        """Set the number of tokens held, an int or a (batch_size,) vector."""
+        """Set the number of tokens held, an int or a (batch_size,) vector (int32 / int64; its values
+        stay on the device and are not looked at)."""
         self._capturing()
         if isinstance(length, int):
             if not 0 <= length <= self.max_length:
@@ -309,6 +310,8 @@ def quant_decoder_states(mem, mem_valid_length, projections, num_heads, head_uni
             memory.write(*(T.as_tensor(p(m)).reshape(m.shape[0], m.shape[1], num_heads, head_units)
                            for p in (key, value)), layer=i)
         if mem_valid_length is not None:
-            memory.set_length(T.as_tensor(mem_valid_length))
+            # (as the float states' mask takes them: any number, more than Lm is all of it; the
+            # buffer has a few more slots)
+            memory.set_length(T.valid_length_arg(mem_valid_length)[0].clamp(0, Lm))
         rows = QuantKVCache(items * beam_size, num_heads, head_units, max_length, n, m.device, kv)
     return QuantDecoderStates(rows, memory, bias_table)

@@ -88,3 +88,16 @@ def test_a_bias_or_mask_over_no_keys_is_given(nlp, calls, given):
     a = nlp._lib.Kv4AttnDesc.from_buffer_copy(calls[0][3])
     assert a.Lm == 0
     assert bool(a.edge_scores) == ('edge_scores' in kw) and bool(a.mask) == ('mask' in kw)
+
+
+@pytest.mark.parametrize('dtype', [torch.int32, torch.int64, torch.int16, torch.float32])
+@pytest.mark.parametrize('layout', ['NT', 'TN'])
+def test_memory_lengths_end_at_the_memory(nlp, calls, layout, dtype):
+    """Lengths beyond the memory mean all of it, as in gen_mem_attn_mask: not the rest of the buffer,
+    which is rounded up to 32 slots."""
+    items, Lm, H, d = 4, 11, 2, 8
+    mem = torch.zeros((items, Lm, H * d) if layout == 'NT' else (Lm, items, H * d))
+    states = nlp.kv_cache.quant_decoder_states(mem, torch.tensor([11, 40, 3, 0]).to(dtype),
+                                               [(lambda m: m, lambda m: m)], H, d, 5, 2, layout)
+    assert states.memory_cache.length.tolist() == [11, 11, 3, 0]
+    assert states.length.tolist() == [0] * 8

@@ -62,3 +62,20 @@ def test_attention_with_a_bias_or_mask_over_no_keys(nlp, dtype):
                 c._bound = bound
                 got = nlp.attention_cell.multi_head_dot_attn_cached(q, c, causal=causal, **kw)
                 assert got.shape == (B, Lq, H * d) and (got == 0).all()
+
+
+def test_memory_lengths_beyond_the_memory(nlp):
+    """A decoder's step on 4-bit states: lengths beyond the memory are all of it."""
+    torch.manual_seed(3)
+    m = nlp.models.T5Decoder(d_model=64, d_kv=16, d_ff=96, num_layers=1, num_heads=4).cuda()
+    for p in m.parameters():
+        with torch.no_grad():
+            p.copy_(0.2 * torch.randn(p.shape))
+    g = _gen(4)
+    mem, x = torch.randn(3, 11, 64, generator=g).cuda(), torch.randn(3, 1, 64, generator=g).cuda()
+    outs = []
+    with torch.no_grad():
+        for vl in ([11, 11, 4], [12, 500, 4]):
+            states = m.init_quant_states(mem, torch.tensor(vl).cuda(), 4)
+            outs.append(m.incremental_decode(x, None, states, None, None)[0])
+    assert torch.isfinite(outs[0]).all() and torch.equal(outs[0], outs[1])
