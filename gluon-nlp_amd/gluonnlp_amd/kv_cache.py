@@ -228,11 +228,22 @@ class QuantKVCache:
         """Beam search: sequence n K + k goes on from sequence n K + parents[n, k]; ``parents``
         (items, K) whole numbers in [0, K), K <= 32.  In place, all layers in one launch; only the
         tokens held are moved."""
+        self.check_reorder(parents)
+        self._move(parents)
+
+    def check_reorder(self, parents):
+        """The errors of ``reorder``, before anything moves -> the caches that it moves."""
+        from .sequence_sampler import check_parents
+        p, N, K = check_parents(parents, self.batch_size)
+        T.device_index(self.length, p)
+        if K > 32:
+            raise ValueError('beam size {} > 32'.format(K))
+        return [self]
+
+    def _move(self, parents):
         from .sequence_sampler import check_parents, launch_reorder
         p, N, K = check_parents(parents, self.batch_size)
         dev = T.device_index(self.length, p)
-        if K > 32:
-            raise ValueError('beam size {} > 32'.format(K))
         flat = []
         L, B, H, S = self.num_layers, self.batch_size, self.num_heads, self._slots
         groups = self._padded // 64
@@ -282,12 +293,20 @@ class QuantDecoderStates:
     def reorder(self, parents):
         """Beam search: row n K + k goes on from row n K + parents[n, k].  The memory stays: the
         beams of an item share it."""
+        for c in self.check_reorder(parents):
+            c._move(parents)
+
+    def check_reorder(self, parents):
+        """The errors of ``reorder``, before anything moves -> the caches that it moves."""
         if self.memory_cache.batch_size not in (parents.shape[0], self.self_cache.batch_size):
             raise ValueError('{} items, the states hold {} memories'.format(
                 parents.shape[0], self.memory_cache.batch_size))
+        moved = [self.self_cache]
         if self.memory_cache.batch_size != parents.shape[0]:
-            self.memory_cache.reorder(parents)
-        self.self_cache.reorder(parents)
+            moved.append(self.memory_cache)
+        for c in moved:
+            c.check_reorder(parents)
+        return moved
 
     def memory_queries(self, q):
         """(rows, 1, H, d) or (1, rows, H, d) -> (memories, beams, H, d)."""

@@ -200,8 +200,8 @@ def reorder_states(states, parents, batch_axis=0, out=None):
         if s is None:
             return None
         if isinstance(s, (QuantKVCache, QuantDecoderStates)):
-            if not any(c is s for c in caches):
-                caches.append(s)
+            # (refused before anything moves; each cache once, also where states and their cache come)
+            caches.extend(c for c in s.check_reorder(p) if not any(c is x for x in caches))
             return s
         if isinstance(s, (list, tuple)):
             n = len(s)
@@ -232,7 +232,7 @@ def reorder_states(states, parents, batch_axis=0, out=None):
     if flat:
         launch_reorder(dev, flat, N, K, p, None)
     for c in caches:
-        c.reorder(p)
+        c._move(p)
     return result
 
 

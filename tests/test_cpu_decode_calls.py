@@ -101,3 +101,42 @@ def test_memory_lengths_end_at_the_memory(nlp, calls, layout, dtype):
                                                [(lambda m: m, lambda m: m)], H, d, 5, 2, layout)
     assert states.memory_cache.length.tolist() == [11, 11, 3, 0]
     assert states.length.tolist() == [0] * 8
+
+
+def _cache(nlp, B, **kw):
+    return nlp.kv_cache.QuantKVCache(B, 1, 8, 4, ctx='cpu', **kw)
+
+
+def test_a_reordering_is_refused_before_anything_moves(nlp, calls):
+    """Tensors stay as they are when a cache that comes with them does not fit."""
+    Q = nlp.kv_cache.QuantDecoderStates
+    x = torch.zeros(6, 4)
+    p = torch.zeros(2, 3, dtype=torch.int32)
+    big = torch.zeros(1, 40, dtype=torch.int32)
+    for parents, t, cache in ((p, x, _cache(nlp, 5)), (p, x, Q(_cache(nlp, 9), _cache(nlp, 3))),
+                              (p, x, Q(_cache(nlp, 8), _cache(nlp, 2))),
+                              (big, torch.zeros(40, 4), _cache(nlp, 40))):
+        for states, out in (([t, cache], None), ([cache, t], None), ([[t], (cache,)], None)):
+            with pytest.raises(ValueError):
+                nlp.sequence_sampler.reorder_states(states, parents, out=out)
+            with pytest.raises(ValueError):
+                nlp.sequence_sampler.reorder_states(states, parents, out=states)
+        with pytest.raises(ValueError):
+            cache.reorder(parents)
+    assert not calls
+
+
+def test_a_cache_moves_once(nlp, calls):
+    """Also when it is listed beside the states that hold it, or twice."""
+    Q = nlp.kv_cache.QuantDecoderStates
+    rows, memory = _cache(nlp, 6), _cache(nlp, 6)
+    p = torch.zeros(2, 3, dtype=torch.int32)
+    s = Q(rows, memory)
+    for states, moved in (([rows, rows], [rows]), ([s, rows], [rows, memory]),
+                          ([rows, s, memory], [rows, memory]), ([s, s], [rows, memory]),
+                          ([Q(rows, _cache(nlp, 2)), rows], [rows])):
+        del calls[:]
+        nlp.sequence_sampler.reorder_states(states, p)
+        assert len(calls) == 2 * len(moved)                  # tokens, then lengths
+        at = [(ctypes.c_int64 * 1).from_address(c.length.data_ptr()) for c in moved]
+        assert sorted(args[6] for args in calls if args[6]) == sorted(map(ctypes.addressof, at))
