@@ -270,7 +270,7 @@ class BeamSearchSampler:
             scores = torch.full((N, K), -float('inf'), dtype=torch.float32, device=first.device)
             scores[:, 0] = 0.0
             finished = None
-            pad = torch.full_like(step_input[:1], 0 if self._eos_id is None else self._eos_id)
+            pad = 0 if self._eos_id is None else self._eos_id
             steps = 0
             for step in range(1, self._max_length + 1):
                 outputs, states = self._decoder(step_input, states)
@@ -286,7 +286,7 @@ class BeamSearchSampler:
                 states = reorder_states(states, parents, batch_axis=self._axis)
                 # (a finished beam is decoded on, from the end of sentence; nothing reads it)
                 step_input = torch.where(tokens < 0, pad, tokens).reshape(-1)
-        samples = samples[:, :steps + 1].reshape(N, K, -1)
+        samples = samples[:, :steps + 1].reshape(N, K, steps + 1)
         valid_length = (samples >= 0).sum(-1).to(torch.int32)
         return tuple(T.like_caller(o, inputs) for o in (samples, scores, valid_length))
 

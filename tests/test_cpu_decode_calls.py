@@ -140,3 +140,16 @@ def test_a_cache_moves_once(nlp, calls):
         assert len(calls) == 2 * len(moved)                  # tokens, then lengths
         at = [(ctypes.c_int64 * 1).from_address(c.length.data_ptr()) for c in moved]
         assert sorted(args[6] for args in calls if args[6]) == sorted(map(ctypes.addressof, at))
+
+
+@pytest.mark.parametrize('early_return', [True, False])
+@pytest.mark.parametrize('K', [1, 3])
+def test_beam_search_of_no_items(nlp, calls, K, early_return):
+    def decoder(tokens, states):
+        assert tokens.shape == (0,) and tokens.dtype == torch.int32
+        return torch.zeros(0, 7), states
+    sampler = nlp.sequence_sampler.BeamSearchSampler(K, decoder, 1, max_length=4,
+                                                     early_return=early_return)
+    samples, scores, valid = sampler(torch.zeros(0, dtype=torch.int64), [torch.zeros(0, 5)])
+    assert samples.shape == (0, K, 2 if early_return else 5) and samples.dtype == torch.int32
+    assert scores.shape == (0, K) and valid.shape == (0, K)
