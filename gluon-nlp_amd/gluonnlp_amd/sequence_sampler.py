@@ -4,6 +4,7 @@ import array
 import ctypes
 import functools
 import struct
+import warnings
 
 import torch
 
@@ -240,19 +241,29 @@ class BeamSearchSampler:
     """Beam search with a step decoder (the reference's sequence_sampler.BeamSearchSampler).
 
     decoder(step_input (N * K,), states) -> (outputs (N * K, V), states): logits (or, with
-    ``from_logits=False``, log-probabilities) of the next token, and the states after the step;
+    ``normalize=False``, log-probabilities) of the next token, and the states after the step;
     the states hold N * K rows along ``state_batch_axis``.  A candidate's score is its
-    log-probability sum over ((length_base + length) / (length_base + 1)) ** alpha."""
+    log-probability sum over ((length_base + length) / (length_base + 1)) ** alpha.
+
+    ``from_logits`` is the earlier name of ``normalize`` and means the same (true: the outputs are
+    unnormalised); elsewhere the name says the opposite, that the outputs are log-probabilities
+    already, so giving it warns."""
 
     def __init__(self, beam_size, decoder, eos_id, alpha=1.0, length_base=5, max_length=100,
-                 temperature=1.0, from_logits=True, state_batch_axis=0, early_return=True):
+                 temperature=1.0, normalize=True, state_batch_axis=0, early_return=True, *,
+                 from_logits=None):
+        if from_logits is not None:
+            warnings.warn('BeamSearchSampler: from_logits={0} means normalize={0} here (true: the '
+                          'decoder gives unnormalised logits); give normalize'.format(from_logits),
+                          FutureWarning, stacklevel=2)
+            normalize = from_logits
         if not 1 <= beam_size <= MAX_BEAMS:
             raise ValueError('beam size {} is outside [1, {}]'.format(beam_size, MAX_BEAMS))
         if max_length < 1:
             raise ValueError('max_length={} must be positive'.format(max_length))
         self._beam_size, self._decoder, self._eos_id = beam_size, decoder, eos_id
         self._alpha, self._length_base, self._max_length = alpha, length_base, max_length
-        self._temperature, self._from_logits = temperature, from_logits
+        self._temperature, self._normalize = temperature, normalize
         self._axis, self._early_return = state_batch_axis, early_return
 
     def __call__(self, inputs, states):
@@ -277,7 +288,7 @@ class BeamSearchSampler:
                 scores, parents, tokens, finished = beam_search_select(
                     outputs, scores, finished, eos_id=self._eos_id, step=step, alpha=self._alpha,
                     length_base=self._length_base, temperature=self._temperature,
-                    normalize=self._from_logits)
+                    normalize=self._normalize)
                 steps = step
                 reorder_states(samples, parents, out=samples)
                 samples[:, step] = tokens.reshape(-1)

@@ -1,6 +1,7 @@
 """What the wrappers of the decoding operators hand to the C entries, seen with the launch taken out:
 strides, what is refused, and what has run when it is.  No GPU."""
 import ctypes
+import warnings
 
 import pytest
 import torch
@@ -153,3 +154,25 @@ def test_beam_search_of_no_items(nlp, calls, K, early_return):
     samples, scores, valid = sampler(torch.zeros(0, dtype=torch.int64), [torch.zeros(0, 5)])
     assert samples.shape == (0, K, 2 if early_return else 5) and samples.dtype == torch.int32
     assert scores.shape == (0, K) and valid.shape == (0, K)
+
+
+def _normalizes(nlp, calls, *args, **kw):
+    """What BeamSearchSampler(*args, **kw) asks the selection for."""
+    del calls[:]
+    sampler = nlp.sequence_sampler.BeamSearchSampler(
+        2, lambda tokens, states: (torch.zeros(2, 7), states), 1, 1.0, 5, 1, *args, **kw)
+    sampler(torch.zeros(1, dtype=torch.int64), [])
+    return nlp._lib.BeamDesc.from_buffer_copy(calls[0][8]).normalize
+
+
+def test_beam_search_of_log_probabilities(nlp, calls):
+    """``normalize`` as in the selection; its earlier name, which elsewhere says the opposite, works
+    on and warns."""
+    with warnings.catch_warnings():
+        warnings.simplefilter('error')
+        assert _normalizes(nlp, calls) == 1
+        assert _normalizes(nlp, calls, normalize=False) == 0
+        assert _normalizes(nlp, calls, 1.0, False) == 0       # (the place that from_logits had)
+    for given in (True, False):
+        with pytest.warns(FutureWarning, match='normalize'):
+            assert _normalizes(nlp, calls, from_logits=given) == given
