@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from tests import decode_ref as ref
+from tests.test_gpu_decode import _check, _filled
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
@@ -79,3 +80,107 @@ def test_memory_lengths_beyond_the_memory(nlp):
             states = m.init_quant_states(mem, torch.tensor(vl).cuda(), 4)
             outs.append(m.incremental_decode(x, None, states, None, None)[0])
     assert torch.isfinite(outs[0]).all() and torch.equal(outs[0], outs[1])
+
+
+# ------------------------------------------------------------------ attention, past a wave's first tile
+def _rising(nlp, g, B, Hc, d, T, lengths, dtype):
+    """_filled with keys that grow five-fold towards the end: the largest score comes late, and what is
+    summed up until then is scaled down."""
+    c, _, _, _ = _filled(nlp, g, B, Hc, d, T, T, lengths, dtype)
+    grow = 1 + 4 * torch.arange(T)[None, :, None, None] / T
+    k = (torch.randn(B, T, Hc, d, generator=g) * grow).to(dtype)
+    v = (torch.randn(B, T, Hc, d, generator=g) + 0.5).to(dtype)
+    c.set_length(T)
+    kk, vv = k.clone(), v.clone()
+    for b in range(B):
+        kk[b, int(lengths[b]):] = math.nan
+        vv[b, int(lengths[b]):] = math.nan
+    c.write(kk.cuda(), vv.cuda())
+    c.set_length(torch.as_tensor(lengths).int().cuda())
+    (qk, ks, km), (qv, _, _) = ref.quantise(k), ref.quantise(v)
+    return c, qk, qv, (ks.max().item(), km.abs().max().item(), qv.abs().max().item())
+
+
+@pytest.mark.parametrize('dtype', [BF16, F32])
+@pytest.mark.parametrize('d', [64, 128, 72])
+@pytest.mark.parametrize('Lq,share', [(1, 1), (2, 1), (1, 4), (3, 3), (10, 2)])
+def test_attention_over_many_tiles(nlp, dtype, d, Lq, share):
+    """One workgroup a sequence, and several with a few rounds of tiles each: rows of 1, 2, 4 and 16,
+    with and without bias and mask; lengths that end inside a round."""
+    B, Hc = 3, 1
+    for T, lengths in ((2100, [2100, 1337, 513]), (1025, [1025, 1024, 1])):
+        g = _gen(T + d + Lq)
+        c, k, v, size = _rising(nlp, g, B, Hc, d, T, lengths, dtype)
+        q = torch.randn(B, Lq, share, d, generator=g).to(dtype)
+        e = torch.randn(1, share, Lq, T, generator=g).to(dtype)
+        table = torch.randn(share, 300, generator=g).to(dtype)
+        m = torch.rand(B, Lq, T, generator=g) < 0.8
+        m[1, 0, 300:] = False                               # nothing left after the first tiles
+        m[0, Lq - 1, :1000] = False                         # nothing in them
+        t = math.sqrt(d)
+        tol = ref.attention_tolerance(q, *size, T, t, dtype)
+        for kw in ({}, dict(edge=e, mask=m), dict(table=table)):
+            want = ref.attention(q, k, v, lengths, share, temperature=t, **kw)
+            names = {'edge': 'edge_scores', 'table': 'edge_table', 'mask': 'mask'}
+            dev = {names[n]: x.cuda() for n, x in kw.items()}
+            for bound in (1, 700, T):
+                c._bound = bound
+                got = nlp.attention_cell.multi_head_dot_attn_cached(q.cuda(), c, **dev)
+                _check(got.reshape(B, Lq, share, d), want, tol)
+
+
+@pytest.mark.parametrize('dtype', [BF16, F32])
+@pytest.mark.parametrize('d,B,Hc,T', [(64, 65, 8, 520), (128, 33, 8, 270)])
+def test_attention_of_many_sequences(nlp, dtype, d, B, Hc, T):
+    """More sequences and heads than are split: the first tiles are requested before the lengths are
+    known.  Lengths of 0 and 1 among them; NaN behind all of them."""
+    g = _gen(d)
+    lengths = torch.randint(2, T + 1, (B,), generator=g)
+    lengths[:6] = torch.tensor([0, 1, T, 0, T - 1, 65])
+    c, k, v, size = _filled(nlp, g, B, Hc, d, T, T, lengths, dtype)
+    c._bound = T
+    t = math.sqrt(d)
+    for Lq in (1, 2, 3, 5):
+        q = torch.randn(B, Lq, Hc, d, generator=g).to(dtype)
+        got = nlp.attention_cell.multi_head_dot_attn_cached(q.cuda(), c)
+        want = ref.attention(q, k, v, lengths, temperature=t)
+        _check(got.reshape(B, Lq, Hc, d), want,
+               ref.attention_tolerance(q, *size, T, t, dtype))
+        assert (got[0] == 0).all() and (got[3] == 0).all()
+        m = torch.rand(B, Lq, T, generator=g) < 0.7
+        got = nlp.attention_cell.multi_head_dot_attn_cached(q.cuda(), c, mask=m.cuda())
+        want = ref.attention(q, k, v, lengths, mask=m, temperature=t)
+        _check(got.reshape(B, Lq, Hc, d), want,
+               ref.attention_tolerance(q, *size, T, t, dtype))
+
+
+def test_reordering_with_a_cache_that_does_not_fit(nlp):
+    """Refused with everything as it was."""
+    g = _gen(7)
+    x = torch.randn(6, 33, generator=g).cuda()
+    before = x.clone()
+    c = nlp.kv_cache.QuantKVCache(5, 2, 64, 8, ctx='cuda')
+    p = torch.tensor([[2, 0, 1], [1, 1, 0]]).cuda()
+    states = [x, c]
+    with pytest.raises(ValueError):
+        nlp.sequence_sampler.reorder_states(states, p, out=states)
+    assert torch.equal(x, before)
+
+
+def test_states_and_their_cache_move_once(nlp):
+    g = _gen(8)
+    rows = nlp.kv_cache.QuantKVCache(6, 2, 64, 20, ctx='cuda')
+    lengths = torch.tensor([3, 20, 7, 0, 12, 1])
+    k = torch.randn(6, 20, 2, 64, generator=g).cuda()
+    rows.set_length(20)
+    rows.write(k, -k)
+    rows.set_length(lengths.cuda())
+    memory = nlp.kv_cache.QuantKVCache(2, 2, 64, 5, ctx='cuda')
+    before = rows.read()
+    p = torch.tensor([[2, 0, 1], [1, 2, 0]])
+    nlp.sequence_sampler.reorder_states(
+        [nlp.kv_cache.QuantDecoderStates(rows, memory), rows], p.cuda())
+    at = (torch.arange(2)[:, None] * 3 + p).reshape(-1)
+    assert torch.equal(rows.length.cpu().long(), lengths[at])
+    for a, b in zip(rows.read(), before):
+        assert torch.equal(a.cpu(), b.cpu()[at])
