@@ -11,7 +11,8 @@
 // 16 .. 32); the 16 comes off in the epilogue, q . n = q . (16 + n) - 16 sum(q).
 //
 // Roundings: bf16 queries are exact operands, float32 ones are split into three bf16 parts; p s_v
-// is split into two (bf16 tensors: 16 bits, what they lose times 16 + n is 3e-5 of a result, a bf16
+// is split into two (bf16 tensors: 16 bits; 23.5 times the same parts comes off the sum, so that what
+// they lose is weighted by n - 7.5 and not by 16 + n: 6e-6 of a result of many tokens, where a bf16
 // rounding 2e-3) or three parts (float32: all 24 bits).  For float32 23.5 = 16 + 7.5 is taken off
 // inside the matrix products, every 32 channels or tokens: their accumulators start with the largest
 // part's product with a constant operand, so that the sums that are rounded are of q (n - 7.5), not
@@ -384,14 +385,12 @@ kv4_attn_kernel(Kv4Attn a) {
   };
   // weight p of a token with V parameters w: parts of p s_v, its share of the per-row sum
   auto weigh = [&](float p, bool off, uint32_t w, int grp, bf16 (&part)[PS]) {
-    const float pv = off ? 0.f : p * scale_of(w), pm = off ? 0.f : min_of(w);
-    split(pv, part);
-    // (the product takes 16 + n, or, F32, n - 7.5)
-    if (F32) {
-      csum[grp] = fmaf(p, off ? 0.f : fmaf(7.5f, scale_of(w), min_of(w)), csum[grp]);
-    } else {
-      csum[grp] = fmaf(p, pm, csum[grp]);
-      csum[grp] = fmaf(-16.f, pv, csum[grp]);
+    split(off ? 0.f : p * scale_of(w), part);
+    csum[grp] = fmaf(p, off ? 0.f : fmaf(7.5f, scale_of(w), min_of(w)), csum[grp]);
+    // (the products take 16 + n, of the parts as they are; F32: n - 7.5)
+    if (!F32) {
+#pragma unroll
+      for (int k = 0; k < PS; ++k) csum[grp] = fmaf(-23.5f, (float)part[k], csum[grp]);
     }
   };
   // O^T += V^T P^T of 32 tokens: channel 64 grp + 4 row + i of operand A's row

@@ -184,3 +184,37 @@ def test_states_and_their_cache_move_once(nlp):
     assert torch.equal(rows.length.cpu().long(), lengths[at])
     for a, b in zip(rows.read(), before):
         assert torch.equal(a.cpu(), b.cpu()[at])
+
+
+@pytest.mark.parametrize('Lq', [1, 2, 4, 9])
+def test_attention_averages_that_cancel(nlp, Lq):
+    """bfloat16, 16 tokens of one weight whose values cancel, beside a token of zeros: what the two
+    bfloat16 parts of a weight lose must not come in times 16 + n (the form in which codes are
+    multiplied), but cancel as the values do."""
+    H, d, T = 2, 64, 17
+    b = -torch.arange(20, 200).float() / 64                     # (bfloat16 numbers, to 8 bits)
+    b = b[b == b.bfloat16().float()]
+    pv = torch.exp(b) * 0.125
+    part = pv.bfloat16().float()
+    lost = (pv - part - (pv - part).bfloat16().float()).abs() / pv
+    b = b[lost.argmax()].item()
+    assert lost.max() > 0.8 * 2.0 ** -18
+    v = torch.empty(1, T, H, d)
+    v[:, 0::2], v[:, 1::2] = -0.0625, 0.0625                    # codes 7 and 8
+    v[..., 0], v[..., 1] = -0.9375, 0.9375                      # scale 1/8, minimum -0.9375, exactly
+    v[:, 16] = 0
+    assert torch.equal(ref.quantise(v)[0], v.double())
+    c = nlp.kv_cache.QuantKVCache(1, H, d, T, ctx='cuda')
+    c.extend(T)
+    c.write(torch.zeros_like(v).cuda(), v.cuda())
+    e = torch.full((1, 1, 1, T), b)
+    e[..., 16] = 0
+    q = torch.zeros(1, Lq, H, d, dtype=BF16)
+    got = nlp.attention_cell.multi_head_dot_attn_cached(q.cuda(), c, causal=False, scaled=False,
+                                                        edge_scores=e.cuda())
+    want = ref.attention(q, torch.zeros_like(v).double(), v.double(), [T], causal=False, edge=e)
+    # 32-bit sums over 17 tokens of products of at most 23.5 scales (half a step each, and 8 more to
+    # join lanes and waves), the output's half step and that of exp(b) in the two large channels
+    tol = 25 * 2.0 ** -24 * 23.5 * 0.125 + want.abs() * (2.0 ** -8 + 2.0 ** -20)
+    err = (got.reshape(1, Lq, H, d).cpu().double() - want).abs()
+    assert (err <= tol).all(), (err - tol).max()
