@@ -29,7 +29,8 @@
 // Reordering.  out[row] = in[parent's row] for a list of tensors of any size, in one launch.  In
 // place, a thread holds its 16 bytes of all K beams before it writes any, and rows that keep their
 // place are not written.  Bound by memory: the chosen rows once, the changed rows once (24 tensors
-// of 80 rows, 630 MB moved, in 116 us).
+// of 80 rows, 630 MB moved, in 116 us); in place with 5 beams, whose pieces take 174 registers, by the
+// two waves a SIMD that this leaves (the same tensors, 538 MB moved, in 264 us).
 #include "common.h"
 #include "kernels.h"
 
@@ -762,8 +763,8 @@ bool launch_reorder(Reorder a, bool in_place, hipStream_t s) {
     e.piece = (all & 15) == 0 ? 16 : (all & 3) == 0 ? 4 : 1;
     const int64_t pieces = e.seg_bytes / e.piece, rows = in_place ? a.N : a.N * a.K;
     const int64_t un = in_place ? 1 : REORDER_UNROLL;
-    // short segments (time-major states: 64 steps of 512 rows of 1536 bytes): 67 us so, 170 with a
-    // workgroup for each; in place 91 and 179
+    // short segments (4 time-major states of 64 steps of 512 rows of 1536 bytes, 340 MB moved): 77 us
+    // so, 176 with a workgroup for each; in place 51 and 57 with 4 beams, 98 and 185 with 8
     e.flat = pieces < 256 * un && rows * pieces < (1LL << 31);
     const int64_t span = e.flat ? rows * pieces : pieces;
     e.nb = (span + 256 * un - 1) / (256 * un);

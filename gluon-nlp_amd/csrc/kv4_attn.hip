@@ -93,7 +93,8 @@ __device__ __forceinline__ void split(float x, bf16 (&part)[N]) {
   }
 }
 
-// Waves a SIMD that the registers are cut for: as many as nothing spills with.
+// Waves a SIMD that the registers are cut for, nothing spilled (bf16 / 64 / R = 1, float32 / 64 / R = 1
+// and float32 / 128 / R = 4, all with a bias, come out with room for one more).
 constexpr int waves_of(bool f32, int DP, int R, bool bias) {
   if (R <= 4 && f32) return DP == 64 ? (R == 1 && !bias ? 3 : 2) : (R == 4 && bias ? 1 : 2);
   if (R <= 4) return DP == 64 && !bias ? 4 : 3;
@@ -715,9 +716,10 @@ void launch(const Kv4Attn &a, hipStream_t s) {
 
 }  // namespace
 
-// Splits of a sequence: as many as keep all workgroups resident, 1024 at head dim 64 (4 a CU) and
-// 512 at 128 (2 a CU), and no more than give each the same number of rounds of four tiles.  One query
-// a head, us:
+// Splits of a sequence: up to 1024 workgroups at head dim 64 and 512 at 128, and no more than give each
+// the same number of rounds of four tiles.  bf16 kernels up to 4 rows without a bias keep them all
+// resident (4 a CU, 3 at head dim 128); of the others' (bf16 3, with a bias 4 to 2, float32 3 to 1 a
+// CU) some may wait for the first to end.  Measured where all are resident, one query a head, us:
 //   32 x 8 heads of 128, 2048 tokens: 512 workgroups 18.8, 256 19.8, 1024 21.5
 //   64 x 16 heads of 64, 1000 tokens: 1024 workgroups 18.7, 2048 24.0 and a join
 //   4 x 12 heads of 64, 16384 tokens: 16 splits (768 workgroups, 2 rounds each) 16.0, 22 (1056; 1.5

@@ -53,8 +53,9 @@ def beam_search_select(outputs, scores, finished=None, *, eos_id=None, step=1, a
         (scores[k] * lp(step - 1) + z[k, v] - logsumexp(z[k])) / lp(step),  z = outputs / temperature
         lp(s) = ((length_base + s) / (length_base + 1)) ** alpha            (length_base: default K)
 
-    a finished beam is its own only candidate, with its score.  Returns the K best of each item,
-    best first, ties to the lowest k * V + v and finished beams last:
+    (the default of ``length_base`` changes with the beams; ``BeamSearchSampler`` gives 5, whatever
+    they are), a finished beam is its own only candidate, with its score.  Returns the K best of each
+    item, best first, ties to the lowest k * V + v and finished beams last:
 
         scores (N, K) float32, parents (N, K) int32, tokens (N, K) int32 (-1: was finished),
         finished (N, K) bool (the parent was, or the token is ``eos_id``)
@@ -62,7 +63,8 @@ def beam_search_select(outputs, scores, finished=None, *, eos_id=None, step=1, a
     NaN outputs count as -inf, +inf as the largest float.  A beam whose score is not above -1e15 is
     dead (the start of a search: scores [0, -inf, ...]); its candidates count as -inf.  The outputs
     of finished beams are not read.  ``step`` may be a device integer tensor of one element (a
-    captured step then follows it).  Candidates are compared in 64 bits."""
+    captured step then follows it).  Candidates are compared in 64 bits (the exponentials of a
+    logsumexp are summed in 32 bits within 4096 or 8192 logits, in 64 over them)."""
     x, s, f = T.as_tensor(outputs), T.as_tensor(scores), T.as_tensor(finished)
     dev = T.device_index(x, s, f)
     if s.dim() != 2 or s.dtype != torch.float32:
