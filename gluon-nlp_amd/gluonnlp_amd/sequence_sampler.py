@@ -283,7 +283,7 @@ class BeamSearchSampler:
             scores = torch.full((N, K), -float('inf'), dtype=torch.float32, device=first.device)
             scores[:, 0] = 0.0
             finished = None
-            pad = 0 if self._eos_id is None else self._eos_id
+            pad = 0 if self._eos_id is None else int(self._eos_id)
             steps = 0
             for step in range(1, self._max_length + 1):
                 outputs, states = self._decoder(step_input, states)

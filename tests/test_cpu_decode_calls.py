@@ -3,6 +3,7 @@ strides, what is refused, and what has run when it is.  No GPU."""
 import ctypes
 import warnings
 
+import numpy as np
 import pytest
 import torch
 
@@ -176,3 +177,25 @@ def test_beam_search_of_log_probabilities(nlp, calls):
     for given in (True, False):
         with pytest.warns(FutureWarning, match='normalize'):
             assert _normalizes(nlp, calls, from_logits=given) == given
+
+
+@pytest.mark.parametrize('eos', [1, np.int64(1), torch.tensor(1), None])
+def test_beam_search_feeds_the_end_to_finished_beams(nlp, monkeypatch, eos):
+    """Whole numbers of any kind as the end of sentence; tokens stay int32."""
+    fed = []
+
+    def decoder(tokens, states):
+        fed.append(tokens.clone())
+        return torch.zeros(tokens.shape[0], 7), states
+
+    def select(outputs, scores, finished, **kw):
+        return (scores, torch.zeros(2, 3, dtype=torch.int32),
+                torch.tensor([[-1, 4, 5], [6, -1, -1]], dtype=torch.int32),
+                torch.zeros(2, 3, dtype=torch.bool))
+    monkeypatch.setattr(nlp._tensor, 'require_device', lambda *tensors: torch.device('cpu'))
+    monkeypatch.setattr(nlp.sequence_sampler, 'beam_search_select', select)
+    monkeypatch.setattr(nlp.sequence_sampler, 'reorder_states', lambda states, *a, **kw: states)
+    nlp.sequence_sampler.BeamSearchSampler(3, decoder, eos, max_length=2)(torch.tensor([2, 3]), [])
+    pad = 0 if eos is None else 1
+    assert [t.tolist() for t in fed] == [[2, 2, 2, 3, 3, 3], [pad, 4, 5, 6, pad, pad]]
+    assert all(t.dtype == torch.int32 for t in fed)
