@@ -153,7 +153,7 @@ def reorder_states(states, parents, batch_axis=0, out=None):
         raise ValueError('in place: beam size {} > {}'.format(K, MAX_BEAMS))
     dev = T.device_index(p)
     rows, grad = N * K, torch.is_grad_enabled()
-    flat, sources, caches = [], [], []
+    flat, sources, caches, written = [], [], [], []
     last = (None, None, None)              # (shape, dtype, axis) of the state before, and its rows
     tail = None
 
@@ -191,6 +191,8 @@ def reorder_states(states, parents, batch_axis=0, out=None):
                     d.get_device() != dev:
                 raise ValueError('out {} {} does not fit the state {} {}'.format(
                     tuple(d.shape), d.dtype, tuple(shape), dtype))
+        if o is not None or in_place:
+            written.append(d)
         if tail is not None:
             flat.append(t.data_ptr())
             flat.append(d.data_ptr())
@@ -227,6 +229,7 @@ def reorder_states(states, parents, batch_axis=0, out=None):
                     r.append(one(x, ax, ox))
                     continue
                 flat.extend((x.data_ptr(), d.data_ptr()) + tail)
+                written.append(d)
                 r.append(d)
             return r if isinstance(s, list) else tuple(r)
         return one(s, axis, o)
@@ -234,6 +237,8 @@ def reorder_states(states, parents, batch_axis=0, out=None):
     result = walk(states, batch_axis, None if in_place else out)
     if flat:
         launch_reorder(dev, flat, N, K, p, None)
+        if written:       # (what is kept for a tensor as it was -- a memory's projections, what autograd
+            torch.autograd.graph.increment_version(written)     # saved -- shall see that it changed)
     for c in caches:
         c._move(p)
     return result

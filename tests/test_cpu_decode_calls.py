@@ -199,3 +199,24 @@ def test_beam_search_feeds_the_end_to_finished_beams(nlp, monkeypatch, eos):
     pad = 0 if eos is None else 1
     assert [t.tolist() for t in fed] == [[2, 2, 2, 3, 3, 3], [pad, 4, 5, 6, pad, pad]]
     assert all(t.dtype == torch.int32 for t in fed)
+
+
+def test_tensors_that_a_reordering_writes_count_it(nlp, monkeypatch, calls):
+    """Their version moves, as in any change in place: a memory's projections, which the decoders
+    keep with the states, are those of its values at the time."""
+    monkeypatch.setattr(nlp._tensor, 'device_index', lambda *tensors: -1)    # (a CPU tensor's own)
+    p = torch.zeros(2, 3, dtype=torch.int32)
+    states = [torch.zeros(6, 4), (torch.zeros(6, 4), torch.zeros(5, 6, 2)), None]
+    axes = [0, (0, 1), 0]
+    flat = [states[0], *states[1]]
+
+    def versions(x):
+        return [t._version for t in x]
+    before = versions(flat)
+    nlp.sequence_sampler.reorder_states(states, p, axes)
+    assert versions(flat) == before
+    nlp.sequence_sampler.reorder_states(states, p, axes, out=states)
+    assert all(a > b for a, b in zip(versions(flat), before))
+    before, out = versions(flat), [torch.empty(6, 4), (torch.empty(6, 4), torch.empty(5, 6, 2)), None]
+    nlp.sequence_sampler.reorder_states(states, p, axes, out=out)
+    assert versions(flat) == before and all(versions([out[0], *out[1]]))

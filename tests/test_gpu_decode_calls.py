@@ -218,3 +218,30 @@ def test_attention_averages_that_cancel(nlp, Lq):
     tol = 25 * 2.0 ** -24 * 23.5 * 0.125 + want.abs() * (2.0 ** -8 + 2.0 ** -20)
     err = (got.reshape(1, Lq, H, d).cpu().double() - want).abs()
     assert (err <= tol).all(), (err - tol).max()
+
+
+def test_a_memory_reordered_in_place_is_projected_again(nlp):
+    """Float states, the memory among them: after a reordering in place a step gives what it gives
+    after one into new tensors."""
+    torch.manual_seed(5)
+    m = nlp.models.T5Decoder(d_model=64, d_kv=16, d_ff=96, num_layers=1, num_heads=4).cuda()
+    for p in m.parameters():
+        with torch.no_grad():
+            p.copy_(0.2 * torch.randn(p.shape))
+    g = _gen(9)
+    mem = torch.randn(4, 7, 64, generator=g).cuda()
+    x = torch.randn(4, 1, 64, generator=g).cuda()
+    vl = torch.tensor([7, 5, 6, 7]).cuda()
+    parents = torch.tensor([[1, 0], [1, 1]]).cuda()
+    outs = []
+    with torch.no_grad():
+        for in_place in (False, True):
+            mine = mem.clone()
+            out, caches = m.incremental_decode(x, None, m._init_key_values(4, 'cuda'), mine, vl)
+            states = (mine, caches)
+            states = nlp.sequence_sampler.reorder_states(states, parents,
+                                                         out=states if in_place else None)
+            assert (states[0] is mine) == in_place
+            out, _ = m.incremental_decode(x, None, states[1], states[0], vl)
+            outs.append(out)
+    assert torch.equal(*outs)
